@@ -102,6 +102,36 @@ int mncclLmLossBackward(const void* logits, int64_t ld, int T, int V, const int6
 /* dst[cols, rows] = src[rows, cols]^T, bf16, rows laid out as above. */
 int mncclTransposeBf16(const void* src, int64_t lds, int rows, int cols, void* dst, int64_t ldd, cudaStream_t stream);
 
+/* ---- 8-bit floating point with block scales --------------------------------------------------------
+ * Types: 6 fp16, 7 fp32, 9 bf16 (ncclDataType_t).  e4m3 matrices are 16-byte aligned, their row strides multiples of 16.
+ *
+ * Quantise x [M, K] (row stride ldx elements): a block of block_rows (1 or 128) x 128 elements has the scale 2^e, the
+ * smallest with e >= -126 and 448 * 2^e >= its largest magnitude; q = x / scale, rounded to nearest even.  A block with an
+ * infinity or a NaN becomes NaN.  Rows of q hold K rounded up to 16; the padding is written.  block_rows 1:
+ * scale[K blocks][M]; 128: scale[M blocks][K blocks].  qt (may be null): the transpose [K, M], for block_rows 1 quantised
+ * along M with scale_t[M blocks][K]; for 128 with the same scales (scale_t unused). */
+int mncclQuantizeFp8(const void* x, int type, int64_t ldx, int M, int K, int block_rows, void* q, int64_t ldq, float* scale, void* qt,
+                     int64_t ldt, float* scale_t, cudaStream_t stream);
+/* C[M, N] = A[M, K] * B[N, K]^T (+ bias[N]) of e4m3 operands: the fp32 sum of each block of 128 along K times
+ * sa[(m / sa_rows) * sa_row + block * sa_blk] and sb likewise (any fp32 scales), added in fp32 and rounded once.  C and
+ * bias (null: none) are of `type`. */
+int mncclGemmFp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_blk, int sa_rows, const void* b, int64_t ldb,
+                 const float* sb, int64_t sb_row, int64_t sb_blk, int sb_rows, void* c, int64_t ldc, int type, const void* bias, int M, int N,
+                 int K, cudaStream_t stream);
+
+/* ---- distillation from a teacher's top logits -----------------------------------------------------------
+ * Student logits [T, V] of `type` (6, 7 or 9), row stride ld; ids and top [T, K], K <= 1024, tau in [1e-3, 1e3].  With
+ * p = softmax(top / tau) over the entries whose id is not negative and whose logit is above -infinity, a token's loss is
+ * tau^2 * sum p (log p - log softmax(logits / tau)[id]); tokens without entries count for nothing; an id of V or more makes
+ * its token NaN.  Forward writes p [T, K], stats [T, 2] (8-byte aligned), counts [T] for the backward pass, row_loss [T] and
+ * mean[3] = {sum, mean, tokens that count}.  Backward: d [T, V], the gradient of every token's loss times grad[t]
+ * (grad_per_row) or grad[0], over tokens[0] if not null. */
+int mncclDistillForward(const void* logits, int type, int64_t ld, int T, int V, const int64_t* ids, const float* top, int K, float tau,
+                        float* p, float* stats, float* row_loss, int* counts, float* mean, cudaStream_t stream);
+int mncclDistillBackward(const void* logits, int type, int64_t ld, int T, int V, const int64_t* ids, const float* p, int K, float tau,
+                         const float* stats, const int* counts, const float* grad, int grad_per_row, const float* tokens, void* d,
+                         int64_t ldd, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -110,6 +110,14 @@ def lib() -> C.CDLL:
         sig("mncclLmLossForward", i32, vp, C.c_int64, i32, i32, vp, vp, vp, vp, vp, vp)
         sig("mncclLmLossBackward", i32, vp, C.c_int64, i32, i32, vp, vp, vp, vp, vp, C.c_int64, vp, C.c_int64, vp)
         sig("mncclTransposeBf16", i32, vp, C.c_int64, i32, i32, vp, C.c_int64, vp)
+    if hasattr(L, "mncclQuantizeFp8"):
+        sig("mncclQuantizeFp8", i32, vp, i32, C.c_int64, i32, i32, i32, vp, C.c_int64, vp, vp, C.c_int64, vp, vp)
+    if hasattr(L, "mncclGemmFp8"):
+        sig("mncclGemmFp8", i32, vp, C.c_int64, vp, C.c_int64, C.c_int64, i32, vp, C.c_int64, vp, C.c_int64, C.c_int64, i32, vp, C.c_int64, i32,
+            vp, i32, i32, i32, vp)
+    if hasattr(L, "mncclDistillForward"):
+        sig("mncclDistillForward", i32, vp, i32, C.c_int64, i32, i32, vp, vp, i32, C.c_float, vp, vp, vp, vp, vp, vp)
+        sig("mncclDistillBackward", i32, vp, i32, C.c_int64, i32, i32, vp, vp, i32, C.c_float, vp, vp, vp, i32, vp, vp, C.c_int64, vp)
     if hasattr(L, "mncclGemmReduceScatterBf16"):
         sig("mncclGemmRsStageBytes", sz, i32, i32, i32)
         sig("mncclGemmRsFlagWords", sz, i32, i32, i32)

@@ -1,0 +1,219 @@
+"""Distillation from a teacher's top logits: the loss of a student's logits against K entries (token id, logit) of a teacher for every
+token, on the kernels of csrc/kernels/distill.cu, and the same fused with the output projection of a language model.
+
+Logits are read once forward and once backward, where their gradient is written; elementary operators move them more than
+ten times and hold several copies in fp32."""
+from __future__ import annotations
+
+import math
+
+import torch
+import torch.nn.functional as F
+
+from .._lib import lib
+from .fp8 import _CODES, _check, _on
+from .gemm import gemm_bf16
+from .lm_loss import _MAX_ROWS, _eight, _pays, _plain, _transposed
+from .lm_loss import _rows as _dense_rows
+
+_MAX_ENTRIES = 1024   # mncclDistillForward
+_REDUCTIONS = ("mean", "sum", "none")
+
+
+def _reference(logits, ids, top, tau, reduction):
+    """The plain operators, in fp32 (fp64 for fp64 logits)."""
+    V = logits.shape[-1]
+    z = logits if logits.dtype == torch.float64 else logits.float()
+    there = (ids >= 0) & (top != -math.inf)
+    counts = there.any(-1)
+    t = torch.where(there, top.to(z.dtype), -math.inf) / tau
+    log_p = torch.log_softmax(torch.where(counts.unsqueeze(-1), t, 0.0), -1)
+    p = torch.where(there, log_p.exp(), 0.0)
+    # tokens that count for nothing are taken out before the softmax, so that nothing of theirs reaches a gradient
+    log_q = torch.log_softmax(torch.where(counts.unsqueeze(-1), z, 0.0) / tau, -1)
+    inside = ids < V
+    log_q = torch.where(inside, log_q.gather(-1, torch.where(there & inside, ids, 0)), math.nan)
+    rows = tau * tau * torch.where(p != 0, p * (log_p - log_q), 0.0).sum(-1)
+    if reduction == "none":
+        return rows
+    return rows.sum() if reduction == "sum" else rows.sum() / counts.sum()
+
+
+class _Teacher:
+    """What the kernels keep of a call for its backward pass, and the two calls."""
+
+    @staticmethod
+    def forward(rows, ids, top, tau, stream):
+        (T, V), K = rows.shape, ids.shape[-1]
+        p, row_loss = torch.empty((T, K), dtype=torch.float32, device=rows.device), torch.empty(T, dtype=torch.float32, device=rows.device)
+        stats, mean = torch.empty((T, 2), dtype=torch.float32, device=rows.device), torch.empty(3, dtype=torch.float32, device=rows.device)
+        counts = torch.empty(T, dtype=torch.int32, device=rows.device)
+        _check(lib().mncclDistillForward(rows.data_ptr(), _CODES[rows.dtype], _stride(rows), T, V, ids.data_ptr(), top.data_ptr(), K, tau, p.data_ptr(),
+                                         stats.data_ptr(), row_loss.data_ptr(), counts.data_ptr(), mean.data_ptr(), stream), "mncclDistillForward")
+        return p, stats, counts, row_loss, mean
+
+    @staticmethod
+    def backward(rows, ids, p, stats, counts, mean, tau, reduction, grad, d, stream):
+        T, V = rows.shape
+        _check(lib().mncclDistillBackward(rows.data_ptr(), _CODES[rows.dtype], _stride(rows), T, V, ids.data_ptr(), p.data_ptr(), ids.shape[-1], tau,
+                                          stats.data_ptr(), counts.data_ptr(), grad.data_ptr(), 1 if reduction == "none" else 0,
+                                          mean.data_ptr() + 8 if reduction == "mean" else None, d.data_ptr(), _stride(d), stream),
+               "mncclDistillBackward")
+
+
+def _stride(rows):
+    return rows.stride(0) if rows.shape[0] > 1 else max(rows.stride(0), rows.shape[1])
+
+
+def _logit_rows(logits):
+    """``logits [..., V]`` as a matrix with a unit inner stride (a copy only where the strides need one)."""
+    V = logits.shape[-1]
+    rows = logits.detach().reshape(-1, V)
+    return rows if (V == 1 or rows.stride(1) == 1) and (rows.shape[0] == 1 or rows.stride(0) >= V) else rows.contiguous()
+
+
+def _reduced(row_loss, mean, reduction, shape):
+    return row_loss.view(shape) if reduction == "none" else mean[0 if reduction == "sum" else 1].clone()
+
+
+def _again(ctx, inputs, f, grad):
+    """create_graph: the gradient itself is differentiated, by the plain operators."""
+    fresh = [t.view_as(t) for t in inputs]
+    picks = [i for i in range(len(inputs)) if ctx.needs_input_grad[i]]
+    got = torch.autograd.grad(f(*fresh), [fresh[i] for i in picks], grad, create_graph=True)
+    out = dict(zip(picks, got))
+    return [out.get(i) for i in range(len(inputs))]
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, top, tau, reduction):
+        rows = _logit_rows(logits)
+        with _on(logits.device, None) as stream:
+            p, stats, counts, row_loss, mean = _Teacher.forward(rows, ids, top, tau, stream)
+        ctx.save_for_backward(logits, ids, top, p, stats, counts, mean)
+        ctx.tau, ctx.reduction = tau, reduction
+        return _reduced(row_loss, mean, reduction, logits.shape[:-1])
+
+    @staticmethod
+    def backward(ctx, grad):
+        logits, ids, top, p, stats, counts, mean = ctx.saved_tensors
+        none = (None,) * 4
+        if torch.is_grad_enabled():
+            at = ids.view(*logits.shape[:-1], -1), top.view(*logits.shape[:-1], -1)
+            return (*_again(ctx, [logits], lambda z: _reference(z, *at, ctx.tau, ctx.reduction), grad), *none)
+        rows, V = _logit_rows(logits), logits.shape[-1]
+        # rows of the gradient lie to 16 bytes as the logits' do: padded where those are
+        wide = V
+        if rows.shape[0] > 1 and rows.stride(0) != V:
+            per = 16 // rows.element_size()
+            wide = -(-V // per) * per
+        with _on(logits.device, None) as stream:
+            d = torch.empty((rows.shape[0], wide), dtype=rows.dtype, device=rows.device)[:, :V]
+            _Teacher.backward(rows, ids, p, stats, counts, mean, ctx.tau, ctx.reduction, grad.contiguous(), d, stream)
+        return (d.view(logits.shape), *none)
+
+
+class _LmHeadDistillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, ids, top, tau):
+        V = weight.shape[0]
+        rows, w = _dense_rows(x.detach()).view(-1, x.shape[-1]), _dense_rows(weight.detach())
+        logits = torch.empty((rows.shape[0], _eight(V)), dtype=x.dtype, device=x.device)
+        gemm_bf16(rows, w, out=logits[:, :V])
+        p, stats, counts, row_loss, mean = _Teacher.forward(logits[:, :V], ids, top, tau, torch.cuda.current_stream().cuda_stream)
+        ctx.save_for_backward(x, weight, ids, top, logits, p, stats, counts, mean)
+        ctx.tau = tau
+        return mean[1].clone()
+
+    @staticmethod
+    def backward(ctx, grad):
+        x, weight, ids, top, logits, p, stats, counts, mean = ctx.saved_tensors
+        want_x, want_w = ctx.needs_input_grad[:2]
+        if torch.is_grad_enabled():
+            at = ids.view(*x.shape[:-1], -1), top.view(*x.shape[:-1], -1)
+            return (*_again(ctx, [x, weight], lambda a, b: _reference(F.linear(a, b), *at, ctx.tau, "mean"), grad), None, None, None)
+        stream = torch.cuda.current_stream().cuda_stream
+        V = weight.shape[0]
+        rows, logits = _dense_rows(x).view(-1, x.shape[-1]), _dense_rows(logits)
+        d = torch.empty((rows.shape[0], _eight(V)), dtype=x.dtype, device=x.device)[:, :V]
+        _Teacher.backward(logits[:, :V], ids, p, stats, counts, mean, ctx.tau, "mean", grad.contiguous(), d, stream)
+        dx = dw = None
+        if want_x and V % 8 == 0:
+            dx = gemm_bf16(d, _transposed(_dense_rows(weight), stream)).view(x.shape)
+        elif want_x:   # (why the library: ops/lm_loss.py)
+            dx = torch.mm(d.contiguous(), _dense_rows(weight)).view(x.shape)
+        if want_w:
+            dw = gemm_bf16(_transposed(d, stream), _transposed(rows, stream))
+        return dx, dw, None, None, None
+
+
+def _plain_call():
+    """Nothing is active that looks at or transforms the single operators."""
+    return not (torch.jit.is_tracing() or torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active()
+                or torch._C._len_torch_function_stack() or torch._C._len_torch_dispatch_stack())
+
+
+def _native(logits, ids, top):
+    """Whether the kernels take the call; the plain operators take the others."""
+    if not (logits.is_cuda and _plain(logits) and _plain(ids) and _plain(top) and logits.dtype in _CODES):
+        return False
+    if not (0 < ids.shape[-1] <= _MAX_ENTRIES and 0 < ids[..., 0].numel() < 2**31 and 0 < logits.shape[-1] < 2**31 - 2**12) or not _plain_call():
+        return False
+    return torch.autograd.forward_ad.unpack_dual(logits).tangent is None
+
+
+def _arguments(shape, device, ids, top, temperature, reduction="mean"):
+    """The teacher's entries as the kernels read them, and the temperature."""
+    for t, name in ((ids, "top_ids"), (top, "top_logits")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch tensor")
+        if t.dim() != len(shape) or tuple(t.shape[:-1]) != tuple(shape[:-1]) or t.shape[-1] == 0 or t.device != device:
+            raise ValueError(f"{name} must be {[*shape[:-1], 'K']} on {device}")
+    if ids.shape != top.shape:
+        raise ValueError("top_ids and top_logits must have one shape")
+    if ids.dtype not in (torch.int64, torch.int32) or not top.dtype.is_floating_point:
+        raise TypeError("top_ids must be int64 or int32, top_logits floating point")
+    if not 1e-3 <= float(temperature) <= 1e3:
+        raise ValueError("the temperature must be between 1e-3 and 1e3")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {_REDUCTIONS}")
+    return ids.long(), top.detach(), float(temperature)
+
+
+def distillation_loss(logits, top_ids, top_logits, temperature=1.0, reduction="mean"):
+    """Distillation of a student's ``logits [..., V]`` (bf16, fp16 or fp32; loss in fp32) from a teacher's entries ``top_ids [..., K]`` and
+    ``top_logits [..., K]``, differentiable in ``logits``.
+
+    With ``p`` the softmax of ``top_logits / temperature`` over a token's entries and ``q`` that of ``logits / temperature`` over all
+    classes, a token's loss is ``temperature ** 2 * sum(p * (log p - log q[id]))``.  A negative id or a logit of -inf marks an
+    entry that is not there.  Tokens without entries count for nothing, whatever their logits are: no loss, no gradient, left
+    out of the mean (which is NaN if no token counts).  Ids may repeat; one of V or more makes its token's loss and gradient NaN.
+    ``reduction``: ``"mean"`` over the tokens that count, ``"sum"``, or ``"none"`` for a loss ``[...]`` per token."""
+    if not isinstance(logits, torch.Tensor) or not logits.dtype.is_floating_point or logits.dim() < 1:
+        raise TypeError("logits must be a floating-point tensor [..., V]")
+    if logits.shape[-1] == 0:
+        raise ValueError("logits without classes")
+    ids, top, tau = _arguments(logits.shape, logits.device, top_ids, top_logits, temperature, reduction)
+    if not _native(logits, ids, top):
+        return _reference(logits, ids, top, tau, reduction)
+    K = ids.shape[-1]
+    return _Distillation.apply(logits, ids.reshape(-1, K).contiguous(), top.float().reshape(-1, K).contiguous(), tau, reduction)
+
+
+def lm_head_distillation(x, weight, top_ids, top_logits, temperature=1.0):
+    """Mean :func:`distillation_loss` of ``F.linear(x, weight)`` (logits rounded to x's type) as one node: ``x [..., d]``, ``weight
+    [V, d]``; differentiable in both.  The teacher's entries as there."""
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.shape[0] == 0:
+        raise ValueError("shapes: x [..., d], weight [V, d]")
+    ids, top, tau = _arguments((*x.shape[:-1], weight.shape[0]), x.device, top_ids, top_logits, temperature)
+    V, d = weight.shape
+    T = math.prod(x.shape[:-1])
+    native = (x.dim() >= 2 and x.dtype == weight.dtype == torch.bfloat16 and x.device == weight.device and _plain(x) and _plain(weight)
+              and x.is_cuda and x.device.index == torch.cuda.current_device() and V >= 8 and d >= 8 and d % 8 == 0 and 0 < T
+              and max(T, V) <= _MAX_ROWS and not torch.is_autocast_enabled() and _native(x, ids, top)
+              and torch.autograd.forward_ad.unpack_dual(weight).tangent is None)
+    if not native or not _pays(T, V, d):
+        return distillation_loss(F.linear(x, weight), ids, top, tau)
+    K = ids.shape[-1]
+    return _LmHeadDistillation.apply(x, weight, ids.reshape(-1, K).contiguous(), top.float().reshape(-1, K).contiguous(), tau)
