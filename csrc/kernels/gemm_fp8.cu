@@ -1,78 +1,416 @@
-// C[M, N] = A[M, K] * B[N, K]^T (+ bias) for e4m3 operands with a scale for each block of 128 along K:
+// C[M, N] = A[M, K] * B[N, K]^T (+ bias) for e4m3 operands with a scale for each block of 128 along K (gemm_fp8.cuh has the
+// formula and the division of labour), for products that fill the GPU; gemm_fp8_small.cu has the others.
 //
-//   C[m, n] = sum over blocks b of  sa[m / ra, b] * sb[n / rb, b] * sum over k in b of  a[m, k] * b[n, k]
+// Persistent clusters of two CTAs: tcgen05.mma.cta_group::2 computes the P_b of a 256 x BN tile on two SMs, each CTA loads 128 rows of A and
+// half of the tile's rows of B (32 KB a block of K for BN = 256, which is what lets L2 keep up) and holds the sums of its 128 rows:
 //
-// ra and rb (rows of a scale) are 1 or 128.  Products of e4m3 numbers and a block's sum are taken in fp32, scaled and added
-// in fp32; one rounding to C's type, behind the bias.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-#include <cuda_runtime.h>
+//   both CTAs   warp 0     TMA producer; bytes are counted on the leader's barriers
+//   leader      warp 1     one lane issues the four MMAs of a block into one of two accumulators and commits: the ring stage and the accumulator
+//   both CTAs   warps 2-9  promotion: two warps for each quarter of tensor memory's lanes, half of the columns each; a lane holds the sums
+//                          of its row and BN / 2 columns in registers, then adds the bias, rounds and stores them
+//
+// The tensor cores take 512 cycles for a block of 128 x 256 x 128 an SM; reading it (64 KB from tensor memory) and 256 fused multiply-adds
+// a scheduler overlap with the next block.  Where B has a scale for every row (the gradient of a weight) a column's scale is a second
+// factor: 512 floating-point instructions a scheduler, about as long as the tensor cores take.
+#include <algorithm>
+#include <cstdio>
 
-#include <cstdint>
+#include "kernels/gemm_fp8.cuh"
+#include "mem/cuda_driver.h"
+
+namespace mnccl {
+namespace gemm {
+namespace fp8 {
+
+bool make_tensor_map_e4m3(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t row_stride, uint32_t box_rows, std::string* why) {
+  const CudaDriver* d = CudaDriver::get();
+  if (!d || !d->TensorMapEncodeTiled) {
+    *why = "cuTensorMapEncodeTiled unavailable";
+    return false;
+  }
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {row_stride};
+  cuuint32_t box[2] = {kBlockK, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const auto encode = [&] {
+    return d->TensorMapEncodeTiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  int dev = 0;
+  // a thread's first call: the runtime binds its device's context when it is told the device
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  if (r != CUDA_SUCCESS) {
+    *why = "cuTensorMapEncodeTiled: " + d->error_string(r);
+    return false;
+  }
+  return true;
+}
 
 namespace {
 
-constexpr int kBlock = 128;
+constexpr int kStages = 6;
+constexpr int kPromoters = 8;                                  // warps
+constexpr int kPairThreads = 32 * (2 + kPromoters);
+constexpr int kPitch = 33;                                     // floats of a scratch row
+constexpr int kScratchBytes = 16 * kPitch * 4;                 // per promotion warp: 16 rows of 32 columns on their way out
+template <int BN>
+constexpr int kPairStage = kTileBytes + BN / 2 * kBlockK;      // this CTA's 128 rows of A and BN / 2 rows of B
 
-struct Args {
-  const uint8_t *a, *b;
-  int64_t lda, ldb, ldc;
-  int M, N, K;
-  const float *sa, *sb;
-  int64_t sa_row, sa_blk, sb_row, sb_blk;
-  int a_shift, b_shift;   // rows of a scale: 2^shift
-  void* c;
-  const void* bias;
+struct __align__(16) PairCtl {
+  uint64_t full[kStages];    // used in the leader: 2 arrivals (one per producer) and both CTAs' bytes
+  uint64_t empty[kStages];   // one per CTA, released by the leader's commit
+  uint64_t acc_full[2];      // one per CTA
+  uint64_t acc_empty[2];     // used in the leader: the promotion warps of both CTAs
+  uint32_t tmem_base;
+  volatile uint32_t abort;
 };
 
-__device__ __forceinline__ float e4m3(uint8_t v) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
+// 256 x BN tiles, in groups of four rows of tiles that share B's tiles in L2.
+struct Tiles {
+  int m, n;
+  __device__ __forceinline__ void at(int t, int* tm, int* tn) const {
+    constexpr int kGroup = 4;
+    const int group = t / (kGroup * n), first = group * kGroup, rows = min(m - first, kGroup), in = t - group * kGroup * n;
+    *tm = first + in % rows;
+    *tn = in / rows;
+  }
+};
+
+// A lane's NC sums of row `row`, columns [col, col + NC): bias, one rounding, out.
+template <typename T, int NC>
+__device__ __forceinline__ void store_row(const Args& g, int row, int col, float (&acc)[NC], float* scratch, int lane) {
+  const T* bias = static_cast<const T*>(g.bias);
+  if (bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+      if (col + j < g.N) acc[j] += to_float(__ldg(bias + col + j));
+  }
+  T* c = static_cast<T*>(g.c);
+  constexpr int kPer = 32 / static_cast<int>(sizeof(T));   // elements of a 32-byte store
+  if (col + NC <= g.N && ((reinterpret_cast<uintptr_t>(c) | (static_cast<uintptr_t>(g.ldc) * sizeof(T))) & 31u) == 0 && NC % kPer == 0) {
+    // whole 32-byte sectors of this lane's row (col is a multiple of 32 or 112 elements)
+    if ((static_cast<unsigned>(col) * sizeof(T)) % 32 == 0) {
+      if (row >= g.M) return;
+      T* dst = c + static_cast<size_t>(row) * g.ldc + col;
+#pragma unroll
+      for (int j = 0; j < NC / kPer; ++j) {
+        union { T x[kPer]; uint32_t w[8]; } u;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) u.x[k] = round_to<T>(acc[j * kPer + k]);
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + j * kPer), "r"(u.w[0]), "r"(u.w[1]), "r"(u.w[2]), "r"(u.w[3]), "r"(u.w[4]),
+                     "r"(u.w[5]), "r"(u.w[6]), "r"(u.w[7])
+                     : "memory");
+      }
+      return;
+    }
+  }
+  // Rows that start anywhere: 16 rows of 32 columns at a time through shared memory, a row per instruction.
+  const int row_base = row - lane;
+#pragma unroll
+  for (int p = 0; p < (NC + 31) / 32; ++p) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if ((lane >> 4) == half) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (p * 32 + j < NC) scratch[(lane & 15) * kPitch + j] = acc[p * 32 + j];
+      }
+      __syncwarp();
+      const int n = col + p * 32 + lane;
+#pragma unroll 4
+      for (int r = 0; r < 16; ++r) {
+        const int m = row_base + half * 16 + r;
+        if (m < g.M && n < g.N && p * 32 + lane < NC) c[static_cast<size_t>(m) * g.ldc + n] = round_to<T>(scratch[r * kPitch + lane]);
+      }
+      __syncwarp();
+    }
+  }
 }
 
-// 64 x 64 outputs a block, 4 x 4 a thread.
-template <typename T>
-__global__ void __launch_bounds__(256) gemm_fp8_kernel(const Args g) {
-  __shared__ float as[32][65], bs[32][65];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int m0 = static_cast<int>(blockIdx.x) * 64, n0 = static_cast<int>(blockIdx.y) * 64;
-  float acc[4][4] = {};
-  for (int b = 0; b * kBlock < g.K; ++b) {
-    float sum[4][4] = {};
-    for (int k0 = b * kBlock; k0 < min(g.K, (b + 1) * kBlock); k0 += 32) {
-      for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-        const int r = i >> 5, k = i & 31;
-        as[k][r] = m0 + r < g.M && k0 + k < g.K ? e4m3(g.a[(m0 + r) * g.lda + k0 + k]) : 0.0f;
-        bs[k][r] = n0 + r < g.N && k0 + k < g.K ? e4m3(g.b[(n0 + r) * g.ldb + k0 + k]) : 0.0f;
-      }
-      __syncthreads();
-      for (int k = 0; k < 32; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sum[i][j] += as[k][ty * 4 + i] * bs[k][tx * 4 + j];
-      __syncthreads();
+// B_ROWS: B has a scale for every row instead of for 128.
+template <int BN, bool B_ROWS>
+__global__ void __launch_bounds__(kPairThreads, 1)
+gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const __grid_constant__ Args g) {
+  extern __shared__ uint8_t smem_raw[];
+  constexpr int NS = kStages, NC = BN / 2;
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  PairCtl* ctl = reinterpret_cast<PairCtl*>(smem + NS * kPairStage<BN>);
+  uint8_t* scratch_all = reinterpret_cast<uint8_t*>(ctl + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_ctarank();   // 0: leader
+  const int pair = static_cast<int>(blockIdx.x) >> 1, n_pairs = static_cast<int>(gridDim.x) >> 1;
+  const Tiles tiles{(g.M + 255) / 256, (g.N + BN - 1) / BN};
+  const int num_tiles = tiles.m * tiles.n;
+  const int num_kb = (g.K + kBlockK - 1) / kBlockK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(smem_u32(&ctl->full[s]), 2);
+      mbar_init(smem_u32(&ctl->empty[s]), 1);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = min(m0 + ty * 4 + i, g.M - 1), n = min(n0 + tx * 4 + j, g.N - 1);
-        acc[i][j] += g.sa[(m >> g.a_shift) * g.sa_row + b * g.sa_blk] * g.sb[(n >> g.b_shift) * g.sb_row + b * g.sb_blk] * sum[i][j];
-      }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&ctl->acc_full[b]), 1);
+      mbar_init(smem_u32(&ctl->acc_empty[b]), 2 * kPromoters);
+    }
+    ctl->abort = 0;
+    fence_barrier_init();
+    fence_proxy_async();
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m >= g.M || n >= g.N) continue;
-      const float v = acc[i][j] + (g.bias ? static_cast<float>(static_cast<const T*>(g.bias)[n]) : 0.0f);
-      static_cast<T*>(g.c)[m * g.ldc + n] = static_cast<T>(v);
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&tma_a);
+    prefetch_tensormap(&tma_b);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(&ctl->tmem_base), kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();   // the partner's barriers exist before anything arrives on them
+  tc_fence_after_sync();
+  const uint32_t tmem_base = ctl->tmem_base;
+  const uint64_t budget = g.wait_budget_ns;
+  const bool leader = elect_one();   // the lane that issues for its warp
+
+  if (warp == 0) {
+    uint32_t it = 0, s = 0, ph = 1;   // ring position: count, stage, parity to wait for
+    bool ok = true;
+    const uint32_t leader_full = map_to_cta(smem_u32(&ctl->full[0]), 0);
+    for (int t = pair; t < num_tiles && ok; t += n_pairs) {
+      int tm, tn;
+      tiles.at(t, &tm, &tn);
+      const int row_a = tm * 256 + static_cast<int>(cta) * 128, row_b = tn * BN + static_cast<int>(cta) * (BN / 2);
+      for (int kb = 0; kb < num_kb; ++kb, ++it) {
+        if (!mbar_wait_warp(smem_u32(&ctl->empty[0]) + s * 8u, ph, &ctl->abort, budget)) { ok = false; break; }
+        if (leader) {
+          const uint32_t full = leader_full + s * 8u, dst = base + s * kPairStage<BN>;
+          mbar_arrive_expect_tx_cluster(full, kPairStage<BN>);
+          tma_load_2d_pair(dst, &tma_a, full, kb * kBlockK, row_a);
+          tma_load_2d_pair(dst + kTileBytes, &tma_b, full, kb * kBlockK, row_b);
+        }
+        if (++s == NS) { s = 0; ph ^= 1u; }
+      }
     }
+    // Both CTAs' loads count on the leader's barriers, and its partner stays until the cluster barrier at the end.  Where
+    // this producer gave up, the partner may be up to a ring ahead.
+    if (cta == 0) {
+      loads_land(&ctl->full[0], NS, it, budget);
+      if (!ok) loads_land(&ctl->full[0], NS, it + NS, budget);
+    }
+  } else if (warp == 1) {
+    if (cta == 0) {
+      constexpr uint32_t idesc = make_idesc_e4m3(256, BN);
+      const uint64_t da0 = make_smem_desc_sw128(base), db0 = make_smem_desc_sw128(base + kTileBytes);
+      uint32_t s = 0, ph = 0, it = 0;
+      bool ok = true;
+      for (int t = pair; t < num_tiles && ok; t += n_pairs) {
+        for (int kb = 0; kb < num_kb; ++kb, ++it) {
+          const uint32_t buf = it & 1u, acc_ph = (it >> 1) & 1u;
+          ok = mbar_wait_warp(smem_u32(&ctl->acc_empty[0]) + buf * 8u, acc_ph ^ 1u, &ctl->abort, budget);
+          if (!ok) break;
+          ok = mbar_wait_warp(smem_u32(&ctl->full[0]) + s * 8u, ph, &ctl->abort, budget);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint64_t da = da0 + static_cast<uint64_t>(s * (kPairStage<BN> >> 4)), db = db0 + static_cast<uint64_t>(s * (kPairStage<BN> >> 4));
+          if (leader) {
+#pragma unroll
+            for (int k = 0; k < kBlockK / kMmaK; ++k)
+              umma_e4m3_pair(tmem_base + buf * 256u, da + static_cast<uint64_t>(k * 2), db + static_cast<uint64_t>(k * 2), idesc, k != 0 ? 1u : 0u);
+            umma_commit_pair(smem_u32(&ctl->empty[0]) + s * 8u, 3);      // the stage is free in both CTAs
+            umma_commit_pair(smem_u32(&ctl->acc_full[0]) + buf * 8u, 3);
+          }
+          if (++s == NS) { s = 0; ph ^= 1u; }
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3, first_col = ((warp - 2) >> 2) * NC;
+    float* scratch = reinterpret_cast<float*>(scratch_all + (warp - 2) * kScratchBytes);
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + first_col;
+    const uint32_t acc_empty = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
+    // Scales of the block to come, fetched a block ahead (across tiles too): this lane's row; of B the two blocks of 128 rows that the warp's
+    // columns may touch, or a lane's share of the columns.
+    constexpr int kOwn = B_ROWS ? (NC + 31) / 32 : 2;
+    float rs = 0.0f, cs[kOwn];
+    const auto fetch = [&](int t, int kb) {
+      int tm, tn;
+      tiles.at(t, &tm, &tn);
+      rs = __ldg(g.a.at(min(tm * 256 + static_cast<int>(cta) * 128 + q * 32 + lane, g.M - 1)) + kb * g.a.blk);
+      const int col = tn * BN + first_col;
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j) {
+        const int n = B_ROWS ? col + lane + j * 32 : (col & ~127) + j * 128;
+        cs[j] = __ldg(g.b.at(min(n, g.N - 1)) + kb * g.b.blk);
+      }
+    };
+    uint32_t it = 0;
+    bool ok = true;
+    if (pair < num_tiles) fetch(pair, 0);
+    for (int t = pair; t < num_tiles && ok; t += n_pairs) {
+      int tm, tn;
+      tiles.at(t, &tm, &tn);
+      const int row = tm * 256 + static_cast<int>(cta) * 128 + q * 32 + lane, col = tn * BN + first_col;
+      float acc[NC];
+#pragma unroll
+      for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
+      for (int kb = 0; kb < num_kb; ++kb, ++it) {
+        const uint32_t buf = it & 1u, acc_ph = (it >> 1) & 1u;
+        const float r = rs;
+        float s[2];
+        if constexpr (B_ROWS) {
+#pragma unroll
+          for (int j = 0; j < kOwn; ++j) scratch[(it & 1u) * 128 + lane + j * 32] = cs[j];
+          __syncwarp();   // the scales of two blocks ago have been read, this block's are written
+        } else {
+          s[0] = r * cs[0];
+          s[1] = r * cs[1];
+        }
+        if (kb + 1 < num_kb) fetch(t, kb + 1);
+        else if (t + n_pairs < num_tiles) fetch(t + n_pairs, 0);
+        ok = mbar_wait_warp(smem_u32(&ctl->acc_full[0]) + buf * 8u, acc_ph, &ctl->abort, budget);
+        if (!ok) break;
+        tc_fence_after_sync();
+        promote<NC>(
+            taddr + buf * 256u,
+            [&](int c, const uint32_t (&v)[16]) {
+              if constexpr (B_ROWS) {
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                  const float4 b = *reinterpret_cast<const float4*>(scratch + (it & 1u) * 128 + c * 16 + j);
+                  acc[c * 16 + j] += __uint_as_float(v[j]) * r * b.x;
+                  acc[c * 16 + j + 1] += __uint_as_float(v[j + 1]) * r * b.y;
+                  acc[c * 16 + j + 2] += __uint_as_float(v[j + 2]) * r * b.z;
+                  acc[c * 16 + j + 3] += __uint_as_float(v[j + 3]) * r * b.w;
+                }
+              } else {
+                const float x = (col & 127) + c * 16 < 128 ? s[0] : s[1];   // a piece lies in one block: col is a multiple of 16
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[c * 16 + j] += __uint_as_float(v[j]) * x;
+              }
+            },
+            [&] {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(acc_empty + buf * 8u);
+            });
+      }
+      if (!ok) break;
+      if constexpr (B_ROWS) __syncwarp();   // the scratch holds scales up to here
+      if (col < g.N) {
+        switch (g.type) {
+          case 6: store_row<__half>(g, row, col, acc, scratch, lane); break;
+          case 7: store_row<float>(g, row, col, acc, scratch, lane); break;
+          default: store_row<__nv_bfloat16>(g, row, col, acc, scratch, lane);
+        }
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();   // neither CTA leaves (or frees tensor memory) while its partner may still signal it
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+  if (threadIdx.x == 0 && ctl->abort != 0u && g.err != nullptr) atomicCAS(g.err, 0u, ctl->abort);
+}
+
+template <int BN, bool B_ROWS>
+cudaError_t fire(const CUtensorMap& ta, const CUtensorMap& tb, const Args& g, int tiles, cudaStream_t stream) {
+  auto kernel = gemm_fp8_pair_kernel<BN, B_ROWS>;
+  constexpr int smem_bytes = kStages * kPairStage<BN> + 1024 /*alignment slack*/ + static_cast<int>(sizeof(PairCtl)) + kPromoters * kScratchBytes;
+  static_assert(smem_bytes <= 227 * 1024, "shared memory");
+  static_assert(2 * 128 * 4 <= kScratchBytes, "two blocks' scales fit the scratch");
+  static int most_dev[kMaxDevices] = {};   // pairs that the device holds at once, which a persistent kernel must not exceed
+  int& most = most_dev[current_device_slot()];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * 74);
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = smem_bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (most == 0) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+    if (e != cudaSuccess) return e;
+    int n = 0;
+    e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (e != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = 64;
+    }
+    most = n;
+  }
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min(tiles, most)));
+  return cudaLaunchKernelEx(&cfg, kernel, ta, tb, g);
+}
+
+// The tile width that needs the fewest waves times (columns + 256): a narrower tile pays where it saves a wave.
+int pick_width(int M, int N, int pairs, long* cost) {
+  int best = 256;
+  *cost = -1;
+  for (const int bn : {256, 224, 192, 128}) {
+    const long tiles = static_cast<long>((M + 255) / 256) * ((N + bn - 1) / bn), c = (tiles + pairs - 1) / pairs * (bn + 64);
+    if (*cost < 0 || c < *cost) {
+      *cost = c;
+      best = bn;
+    }
+  }
+  return best;
+}
+
+int run(const void* a, int64_t lda, const void* b, int64_t ldb, Args g, cudaStream_t stream) {
+  std::string why;
+  g.err = error_word();
+  g.wait_budget_ns = 2000000000ull;
+  const int sms = sm_count();
+  long cost = 0, small_ns = 0;
+  const int bn = pick_width(g.M, g.N, sms / 2, &cost);
+  const long num_kb = (g.K + kBlockK - 1) / kBlockK, pair_ns = 6000 + cost * num_kb * 300 / 320;
+  SmallPlan p;
+  cudaError_t e;
+  if (plan_small(g.M, g.N, g.K, sms, &p, &small_ns) && small_ns < pair_ns) {
+    e = launch_small(a, lda, b, ldb, g, p, stream, &why);
+  } else {
+    const long tiles = static_cast<long>((g.M + 255) / 256) * ((g.N + bn - 1) / bn);
+    if (tiles > 0x7fffffff / 2) return -2;
+    CUtensorMap ta, tb;
+    if (!make_tensor_map_e4m3(&ta, a, g.M, g.K, lda, 128, &why) || !make_tensor_map_e4m3(&tb, b, g.N, g.K, ldb, bn / 2, &why)) {
+      e = cudaErrorInvalidValue;
+    } else {
+      const auto go = [&](auto rows) {
+        constexpr bool R = decltype(rows)::value;
+        switch (bn) {
+          case 256: return fire<256, R>(ta, tb, g, static_cast<int>(tiles), stream);
+          case 224: return fire<224, R>(ta, tb, g, static_cast<int>(tiles), stream);
+          case 192: return fire<192, R>(ta, tb, g, static_cast<int>(tiles), stream);
+          default: return fire<128, R>(ta, tb, g, static_cast<int>(tiles), stream);
+        }
+      };
+      e = g.b.shift == 0 ? go(std::true_type{}) : go(std::false_type{});
+    }
+  }
+  if (!why.empty()) {
+    fprintf(stderr, "[Mini-NCCL] 8-bit GEMM: %s\n", why.c_str());
+    return -3;
+  }
+  return e == cudaSuccess ? 0 : static_cast<int>(e) + 1000;
 }
 
 }  // namespace
+}  // namespace fp8
+}  // namespace gemm
+}  // namespace mnccl
 
 extern "C" {
 #define MNCCL_EXPORT __attribute__((visibility("default")))
@@ -83,21 +421,26 @@ extern "C" {
 MNCCL_EXPORT int mncclGemmFp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_blk, int sa_rows, const void* b,
                               int64_t ldb, const float* sb, int64_t sb_row, int64_t sb_blk, int sb_rows, void* c, int64_t ldc, int type,
                               const void* bias, int M, int N, int K, cudaStream_t stream) {
+  using namespace mnccl::gemm::fp8;
   if (!a || !b || !c || !sa || !sb || M <= 0 || N <= 0 || K <= 0) return -1;
   const auto operand = [K](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 16 == 0 && ld >= K; };
-  if (!operand(a, lda) || !operand(b, ldb) || ldc < N) return -2;
-  if ((sa_rows != 1 && sa_rows != kBlock) || (sb_rows != 1 && sb_rows != kBlock)) return -2;
-  const Args g{static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(b), lda, ldb, ldc, M, N, K, sa, sb, sa_row, sa_blk, sb_row, sb_blk,
-               sa_rows == 1 ? 0 : 7, sb_rows == 1 ? 0 : 7, c, bias};
-  const dim3 grid((M + 63) / 64, (N + 63) / 64);
-  switch (type) {
-    case 6: gemm_fp8_kernel<__half><<<grid, 256, 0, stream>>>(g); break;
-    case 7: gemm_fp8_kernel<float><<<grid, 256, 0, stream>>>(g); break;
-    case 9: gemm_fp8_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(g); break;
-    default: return -2;
+  if (!operand(a, lda) || !operand(b, ldb) || ldc < N || (type != 6 && type != 7 && type != 9)) return -2;
+  if ((sa_rows != 1 && sa_rows != 128) || (sb_rows != 1 && sb_rows != 128) || std::max({M, N, K}) > 0x7fffff00) return -2;
+  Args g{};
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.a = Scales{sa, sa_row, sa_blk, sa_rows == 1 ? 0 : 7};
+  g.b = Scales{sb, sb_row, sb_blk, sb_rows == 1 ? 0 : 7};
+  g.c = c;
+  g.ldc = ldc;
+  g.type = type;
+  g.bias = bias;
+  try {
+    return run(a, lda, b, ldb, g, stream);
+  } catch (...) {   // out of host memory for a message
+    return -3;
   }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : static_cast<int>(e) + 1000;
 }
 
 }  // extern "C"

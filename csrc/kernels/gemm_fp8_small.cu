@@ -1,0 +1,315 @@
+// The 8-bit product with block scales for few rows of A, or too few tiles for the persistent kernel.
+//
+// Operands are swapped: the 128 rows of the MMA are rows of B (a weight), its TN columns rows of A, so a tile of 16 tokens costs 2 KB of
+// shared memory a block instead of 16, and a column of the result is 128 consecutive elements of a row of C.  K is split over the CTAs of a
+// cluster where the tiles alone leave SMs idle; the slices meet in distributed shared memory and are added in slice order.  One tile per CTA.
+#include <algorithm>
+
+#include "kernels/gemm_fp8.cuh"
+
+namespace mnccl {
+namespace gemm {
+namespace fp8 {
+
+namespace {
+
+template <int TN>
+constexpr int kStage = kTileBytes + TN * kBlockK;
+template <int TN>
+constexpr int kWarps = TN >= 64 ? 8 : 4;          // promotion warps: one or two for each quarter of tensor memory's lanes
+template <int TN>
+constexpr int kCols = TN / (kWarps<TN> / 4);      // columns a promotion warp holds
+template <int TN>
+constexpr int kBuffers = TN >= 128 ? 2 : 4;       // accumulators
+constexpr int kMostStages = 12;
+
+struct __align__(16) Ctl {
+  uint64_t full[kMostStages], empty[kMostStages];
+  uint64_t acc_full[4], acc_empty[4];
+  uint32_t tmem_base;
+  volatile uint32_t abort;
+};
+
+struct SmallArgs {
+  Args g;
+  int tiles_n, kb_per_slice;
+};
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+__device__ __forceinline__ void store(const Args& g, int m, int n, float v) {
+  if (m >= g.M || n >= g.N) return;
+  const size_t at = static_cast<size_t>(m) * g.ldc + n;
+  switch (g.type) {
+    case 6: static_cast<__half*>(g.c)[at] = __float2half_rn(v); break;
+    case 7: static_cast<float*>(g.c)[at] = v; break;
+    default: static_cast<__nv_bfloat16*>(g.c)[at] = __float2bfloat16_rn(v);
+  }
+}
+__device__ __forceinline__ float bias_of(const Args& g, int n) {
+  if (g.bias == nullptr || n >= g.N) return 0.0f;
+  switch (g.type) {
+    case 6: return __half2float(static_cast<const __half*>(g.bias)[n]);
+    case 7: return static_cast<const float*>(g.bias)[n];
+    default: return __bfloat162float(static_cast<const __nv_bfloat16*>(g.bias)[n]);
+  }
+}
+
+template <int TN, int NS>
+__global__ void __launch_bounds__(32 * (2 + kWarps<TN>))
+gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x, const __grid_constant__ SmallArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  constexpr int NB = kBuffers<TN>, W = kWarps<TN>, NC = kCols<TN>;
+  constexpr uint32_t kTmem = NB * TN;   // 64, 128, 256, 256 columns
+  static_assert(NS <= kMostStages && (NB & (NB - 1)) == 0, "ring depth");
+  const Args& g = args.g;
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  Ctl* ctl = reinterpret_cast<Ctl*>(smem + NS * kStage<TN>);
+  float* col_scales = reinterpret_cast<float*>(ctl + 1);   // [promotion warp][2][NC]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slices = static_cast<int>(cluster_size());
+  const int slice = static_cast<int>(cluster_ctarank());
+  const int tile = static_cast<int>(blockIdx.x) / slices;
+  const int n0 = (tile % args.tiles_n) * 128, m0 = (tile / args.tiles_n) * TN;
+  const int num_kb = (g.K + kBlockK - 1) / kBlockK;
+  const int kb0 = slice * args.kb_per_slice;
+  const int nkb = min(num_kb, kb0 + args.kb_per_slice) - kb0;   // at least 1: the plan leaves no slice empty
+
+  const bool leader = elect_one();
+  auto load = [&](int i, uint32_t s) {
+    const uint32_t full = smem_u32(&ctl->full[0]) + s * 8u, dst = base + s * kStage<TN>;
+    mbar_arrive_expect_tx(full, kStage<TN>);
+    tma_load_2d(dst, &tma_w, full, (kb0 + i) * kBlockK, n0);
+    tma_load_2d(dst + kTileBytes, &tma_x, full, (kb0 + i) * kBlockK, m0);
+  };
+  if (warp == 0) {
+    if (leader) {
+      prefetch_tensormap(&tma_w);
+      prefetch_tensormap(&tma_x);
+      for (int s = 0; s < NS; ++s) {
+        mbar_init(smem_u32(&ctl->full[s]), 1);
+        mbar_init(smem_u32(&ctl->empty[s]), 1);
+      }
+      for (int b = 0; b < NB; ++b) {
+        mbar_init(smem_u32(&ctl->acc_full[b]), 1);
+        mbar_init(smem_u32(&ctl->acc_empty[b]), W);
+      }
+      ctl->abort = 0;
+      fence_barrier_init();
+      fence_proxy_async();
+    }
+    __syncwarp();
+    for (int i = 0; i < NS && i < nkb; ++i)
+      if (leader) load(i, i);
+  }
+  __syncwarp();
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&ctl->tmem_base), kTmem);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = ctl->tmem_base;
+
+  // promotion warps: warp's quarter of the lanes, its columns of the tile, this lane's row of B
+  const int q = warp & 3, first_col = ((warp - 2) >> 2) * NC;
+  const int n = n0 + q * 32 + lane;
+  float acc[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
+  bool ok = true;
+
+  if (warp == 0) {
+    uint32_t s = 0, ph = 0;
+    int i = NS;
+    for (; i < nkb; ++i) {
+      if (!mbar_wait_warp(smem_u32(&ctl->empty[0]) + s * 8u, ph, &ctl->abort, g.wait_budget_ns)) break;
+      if (leader) load(i, s);
+      if (++s == NS) { s = 0; ph ^= 1u; }
+    }
+    loads_land(&ctl->full[0], NS, static_cast<uint32_t>(min(i, nkb)), g.wait_budget_ns);
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = make_idesc_e4m3(128, TN);
+    const uint64_t dw0 = make_smem_desc_sw128(base), dx0 = make_smem_desc_sw128(base + kTileBytes);
+    uint32_t s = 0, ph = 0;
+    for (int i = 0; i < nkb; ++i) {
+      const uint32_t buf = static_cast<uint32_t>(i) % NB, acc_ph = (static_cast<uint32_t>(i) / NB) & 1u;
+      ok = mbar_wait_warp(smem_u32(&ctl->acc_empty[0]) + buf * 8u, acc_ph ^ 1u, &ctl->abort, g.wait_budget_ns);
+      if (!ok) break;
+      ok = mbar_wait_warp(smem_u32(&ctl->full[0]) + s * 8u, ph, &ctl->abort, g.wait_budget_ns);
+      if (!ok) break;
+      tc_fence_after_sync();
+      const uint64_t dw = dw0 + static_cast<uint64_t>(s * (kStage<TN> >> 4)), dx = dx0 + static_cast<uint64_t>(s * (kStage<TN> >> 4));
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < kBlockK / kMmaK; ++k)   // 32 bytes on inside a 128-byte swizzle row: +2 in the address field
+          umma_e4m3(tmem + buf * TN, dw + static_cast<uint64_t>(k * 2), dx + static_cast<uint64_t>(k * 2), idesc, k != 0 ? 1u : 0u);
+        umma_commit(smem_u32(&ctl->empty[0]) + s * 8u);
+        umma_commit(smem_u32(&ctl->acc_full[0]) + buf * 8u);
+      }
+      if (++s == NS) { s = 0; ph ^= 1u; }
+    }
+  } else {
+    const float* row_scale = g.b.at(min(n, g.N - 1));
+    constexpr int kOwn = (NC + 31) / 32;   // column scales a lane fetches for its warp
+    const float* col_scale[kOwn];
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) col_scale[j] = g.a.at(min(m0 + first_col + (lane + j * 32) % NC, g.M - 1));
+    float* box = col_scales + (warp - 2) * 2 * NC;
+    float rs, cs[kOwn];
+    auto fetch = [&](int i) {
+      rs = __ldg(row_scale + (kb0 + i) * g.b.blk);
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j) cs[j] = __ldg(col_scale[j] + (kb0 + i) * g.a.blk);
+    };
+    fetch(0);
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + first_col;
+    for (int i = 0; i < nkb; ++i) {
+      float* mine = box + (i & 1) * NC;
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j)
+        if (lane + j * 32 < NC) mine[lane + j * 32] = cs[j];
+      const float r = rs;
+      __syncwarp();   // the box of two blocks ago has been read, this one's is written
+      if (i + 1 < nkb) fetch(i + 1);
+      const uint32_t buf = static_cast<uint32_t>(i) % NB, acc_ph = (static_cast<uint32_t>(i) / NB) & 1u;
+      ok = mbar_wait_warp(smem_u32(&ctl->acc_full[0]) + buf * 8u, acc_ph, &ctl->abort, g.wait_budget_ns);
+      if (!ok) break;
+      tc_fence_after_sync();
+      promote<NC>(
+          taddr + buf * TN,
+          [&](int c, const uint32_t (&v)[16]) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+              const float4 s = *reinterpret_cast<const float4*>(mine + c * 16 + j);
+              acc[c * 16 + j] += __uint_as_float(v[j]) * r * s.x;
+              acc[c * 16 + j + 1] += __uint_as_float(v[j + 1]) * r * s.y;
+              acc[c * 16 + j + 2] += __uint_as_float(v[j + 2]) * r * s.z;
+              acc[c * 16 + j + 3] += __uint_as_float(v[j + 3]) * r * s.w;
+            }
+          },
+          [&] {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&ctl->acc_empty[0]) + buf * 8u);
+          });
+    }
+  }
+  __syncwarp();
+
+  if (slices == 1) {
+    if (warp >= 2 && ok) {
+      const float bias = bias_of(g, n);
+#pragma unroll
+      for (int j = 0; j < NC; ++j) store(g, m0 + first_col + j, n, acc[j] + bias);
+    }
+  } else {
+    // Every CTA of the cluster has left its main loop: its ring may be overwritten.
+    cluster_sync_all();
+    const int own = TN / slices, own_log2 = 31 - __clz(own);   // columns this slice finishes (a power of two)
+    float* recv = reinterpret_cast<float*>(smem);               // [source slice][own columns][128 rows]
+    if (warp >= 2 && ok) {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const int col = first_col + j;
+        const uint32_t dst = map_to_cta(smem_u32(recv + (slice * own + (col & (own - 1))) * 128 + q * 32 + lane), static_cast<uint32_t>(col >> own_log2));
+        st_cluster_f32(dst, acc[j]);
+      }
+    }
+    cluster_sync_all();
+    if (warp >= 2 && ok) {
+      const float bias = bias_of(g, n);
+      for (int c = (warp - 2) >> 2; c < own; c += W / 4) {
+        const int m = m0 + slice * own + c;
+        if (m >= g.M) break;
+        float v = recv[c * 128 + q * 32 + lane];
+        for (int s = 1; s < slices; ++s) v += recv[(s * own + c) * 128 + q * 32 + lane];
+        store(g, m, n, v + bias);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, kTmem);
+  }
+  if (threadIdx.x == 0 && ctl->abort != 0u && g.err != nullptr) atomicCAS(g.err, 0u, ctl->abort);
+}
+
+template <int TN, int NS>
+cudaError_t fire(const CUtensorMap& tw, const CUtensorMap& tx, const SmallArgs& a, const SmallPlan& p, cudaStream_t stream) {
+  auto kernel = gemm_fp8_small_kernel<TN, NS>;
+  constexpr int smem_bytes = NS * kStage<TN> + 1024 /*alignment slack*/ + static_cast<int>(sizeof(Ctl)) + kWarps<TN> * 2 * kCols<TN> * 4;
+  static_assert(smem_bytes <= 227 * 1024, "shared memory");
+  static_assert(TN * 128 * 4 <= NS * kStage<TN>, "the slices' partial sums fit the ring");
+  static bool configured[kMaxDevices] = {};
+  const int dev = current_device_slot();
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.tiles) * p.slices);
+  cfg.blockDim = dim3(32 * (2 + kWarps<TN>));
+  cfg.dynamicSmemBytes = smem_bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(p.slices);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, tw, tx, a);
+}
+
+}  // namespace
+
+// Fewest CTAs' worth of K while SMs are idle: slices are doubled as long as all CTAs still run at once.
+bool plan_small(int M, int N, int K, int sms, SmallPlan* p, long* ns) {
+  const int num_kb = (K + kBlockK - 1) / kBlockK;
+  const long tiles_n = (N + 127) / 128;
+  p->tn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  const long tiles = tiles_n * ((M + p->tn - 1) / p->tn);
+  if (tiles > (1 << 24)) return false;
+  p->tiles = static_cast<int>(tiles);
+  p->slices = 1;
+  while (p->slices < 8 && tiles * p->slices * 2 <= sms && num_kb >= p->slices * 4) p->slices *= 2;
+  p->kb_per_slice = (num_kb + p->slices - 1) / p->slices;
+  while ((p->slices - 1) * p->kb_per_slice >= num_kb) {   // a slice would be empty
+    p->slices /= 2;
+    p->kb_per_slice = (num_kb + p->slices - 1) / p->slices;
+  }
+  *ns = 5000 + ((tiles * p->slices + sms - 1) / sms) * p->kb_per_slice * (p->tn == 128 ? 300 : 200);
+  return true;
+}
+
+cudaError_t launch_small(const void* a, int64_t lda, const void* b, int64_t ldb, const Args& g, const SmallPlan& p, cudaStream_t stream, std::string* why) {
+  CUtensorMap tw, tx;
+  if (!make_tensor_map_e4m3(&tw, b, g.N, g.K, ldb, 128, why) || !make_tensor_map_e4m3(&tx, a, g.M, g.K, lda, p.tn, why)) return cudaErrorInvalidValue;
+  const SmallArgs s{g, (g.N + 127) / 128, p.kb_per_slice};
+  switch (p.tn) {
+    case 16: return fire<16, 10>(tw, tx, s, p, stream);
+    case 32: return fire<32, 10>(tw, tx, s, p, stream);
+    case 64: return fire<64, 8>(tw, tx, s, p, stream);
+    case 128: return fire<128, 6>(tw, tx, s, p, stream);
+  }
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace fp8
+}  // namespace gemm
+}  // namespace mnccl
