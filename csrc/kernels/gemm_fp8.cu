@@ -6,7 +6,7 @@
 //
 //   both CTAs   warp 0     TMA producer; bytes are counted on the leader's barriers
 //   leader      warp 1     one lane issues the four MMAs of a block into one of two accumulators and commits: the ring stage and the accumulator
-//   both CTAs   warps 2-9  promotion: two warps for each quarter of tensor memory's lanes, half of the columns each; a lane holds the sums
+//   both CTAs   warps 4-11 promotion: two warps for each quarter of tensor memory's lanes, half of the columns each; a lane holds the sums
 //                          of its row and BN / 2 columns in registers, then adds the bias, rounds and stores them
 //
 // The tensor cores take 512 cycles for a block of 128 x 256 x 128 an SM; reading it (64 KB from tensor memory) and 256 fused multiply-adds
@@ -49,19 +49,33 @@ bool make_tensor_map_e4m3(CUtensorMap* map, const void* base, uint64_t rows, uin
 
 namespace {
 
-constexpr int kStages = 6;
 constexpr int kPromoters = 8;                                  // warps
-constexpr int kPairThreads = 32 * (2 + kPromoters);
-constexpr int kPitch = 33;                                     // floats of a scratch row
-constexpr int kScratchBytes = 16 * kPitch * 4;                 // per promotion warp: 16 rows of 32 columns on their way out
+constexpr int kFirst = 4;                                      // first promotion warp: register counts are set for four warps at a time
+constexpr int kPairThreads = 32 * (kFirst + kPromoters);
+// 384 threads start with 168 registers each; what the control warps give back (128 * 96) is what the promotion warps take (256 * 48).
+constexpr int kControlRegs = 72, kPromoterRegs = 216;
+static_assert(128 * kControlRegs + 32 * kPromoters * kPromoterRegs <= kPairThreads * 168, "registers the block was launched with");
+constexpr int kOutRow = 64;                                    // bytes of a row of a piece of the result on its way out
+constexpr int kPieceBytes = 32 * kOutRow;
+constexpr int kScratchBytes = 2 * kPieceBytes;                 // per promotion warp: two pieces
+constexpr int kBiasFloats = 128;                               // per promotion warp: of its columns
+constexpr int kPitch = 33;                                     // floats of a scratch row where rows of C start anywhere
 template <int BN>
 constexpr int kPairStage = kTileBytes + BN / 2 * kBlockK;      // this CTA's 128 rows of A and BN / 2 rows of B
 
+constexpr int kStages = 5;
+template <int BN, bool B_ROWS>
+constexpr int kCols = B_ROWS ? BN : 4;                         // scales of B a block: of the tile's columns, or of the two blocks of rows that a half touches
+template <int BN, bool B_ROWS>
+constexpr int kSlot = kGroup * (128 + kCols<BN, B_ROWS>);      // floats: a group's scales
+
 struct __align__(16) PairCtl {
-  uint64_t full[kStages];    // used in the leader: 2 arrivals (one per producer) and both CTAs' bytes
-  uint64_t empty[kStages];   // one per CTA, released by the leader's commit
-  uint64_t acc_full[2];      // one per CTA
-  uint64_t acc_empty[2];     // used in the leader: the promotion warps of both CTAs
+  uint64_t full[kStages];        // used in the leader: 2 arrivals (one per producer) and both CTAs' bytes
+  uint64_t empty[kStages];       // one per CTA, released by the leader's two commits
+  uint64_t acc_full[2][2];       // [accumulator][half of the tile's columns], one per CTA
+  uint64_t acc_empty[2][2];      // used in the leader: the half's four promotion warps of both CTAs
+  uint64_t scales_full[2];       // 32 arrivals: the lanes of the warp that brings them
+  uint64_t scales_empty[2];      // the promotion warps
   uint32_t tmem_base;
   volatile uint32_t abort;
 };
@@ -77,51 +91,70 @@ struct Tiles {
   }
 };
 
-// A lane's NC sums of row `row`, columns [col, col + NC): bias, one rounding, out.
+// A lane's NC sums of row `row`, columns [col, col + NC): bias, one rounding, out.  With a tensor map of C a warp's 32 rows leave as pieces of 64
+// bytes a row that it lays out in shared memory (64-byte swizzle: no bank conflicts) and the TMA unit writes while the next tile is
+// begun.  (Each lane storing its own row, 32 bytes at a time, held the tensor cores up for a fifth of the time at K = 4096 and for two fifths
+// at K = 1024.)
 template <typename T, int NC>
-__device__ __forceinline__ void store_row(const Args& g, int row, int col, float (&acc)[NC], float* scratch, int lane) {
-  const T* bias = static_cast<const T*>(g.bias);
-  if (bias != nullptr) {
+__device__ __forceinline__ void store_rows(const Args& g, const CUtensorMap* map, bool mapped, int row, int col, float (&acc)[NC], uint8_t* scratch, float* bias, int lane) {
+  const int row_base = row - lane;
+  if (row_base >= g.M) return;   // the same for the whole warp
+  if (g.bias != nullptr) {
+    const T* b = static_cast<const T*>(g.bias);
 #pragma unroll
-    for (int j = 0; j < NC; ++j)
-      if (col + j < g.N) acc[j] += to_float(__ldg(bias + col + j));
-  }
-  T* c = static_cast<T*>(g.c);
-  constexpr int kPer = 32 / static_cast<int>(sizeof(T));   // elements of a 32-byte store
-  if (col + NC <= g.N && ((reinterpret_cast<uintptr_t>(c) | (static_cast<uintptr_t>(g.ldc) * sizeof(T))) & 31u) == 0 && NC % kPer == 0) {
-    // whole 32-byte sectors of this lane's row (col is a multiple of 32 or 112 elements)
-    if ((static_cast<unsigned>(col) * sizeof(T)) % 32 == 0) {
-      if (row >= g.M) return;
-      T* dst = c + static_cast<size_t>(row) * g.ldc + col;
+    for (int j = 0; j < NC / 32; ++j) bias[j * 32 + lane] = to_float(__ldg(b + min(col + j * 32 + lane, g.N - 1)));
+    __syncwarp();
 #pragma unroll
-      for (int j = 0; j < NC / kPer; ++j) {
-        union { T x[kPer]; uint32_t w[8]; } u;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) u.x[k] = round_to<T>(acc[j * kPer + k]);
-        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + j * kPer), "r"(u.w[0]), "r"(u.w[1]), "r"(u.w[2]), "r"(u.w[3]), "r"(u.w[4]),
-                     "r"(u.w[5]), "r"(u.w[6]), "r"(u.w[7])
-                     : "memory");
-      }
-      return;
+    for (int j = 0; j < NC; j += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(bias + j);
+      acc[j] += v.x;
+      acc[j + 1] += v.y;
+      acc[j + 2] += v.z;
+      acc[j + 3] += v.w;
     }
+    __syncwarp();
+  }
+  if (mapped) {
+    constexpr int kPer = kOutRow / static_cast<int>(sizeof(T)), kChunk = 16 / static_cast<int>(sizeof(T));
+#pragma unroll
+    for (int p = 0; p < NC / kPer; ++p) {
+      if (col + p * kPer >= g.N) break;
+      uint8_t* piece = scratch + (p & 1) * kPieceBytes;
+      if (lane == 0) bulk_wait_read<1>();   // the piece before the last has been read
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        union { T x[kChunk]; uint4 w; } u;
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) u.x[k] = round_to<T>(acc[p * kPer + c * kChunk + k]);
+        *reinterpret_cast<uint4*>(piece + lane * kOutRow + ((c ^ (lane >> 1)) & 3) * 16) = u.w;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(map, smem_u32(piece), col + p * kPer, row_base);
+        bulk_commit();
+      }
+    }
+    return;
   }
   // Rows that start anywhere: 16 rows of 32 columns at a time through shared memory, a row per instruction.
-  const int row_base = row - lane;
+  T* c = static_cast<T*>(g.c);
+  float* rows = reinterpret_cast<float*>(scratch);
 #pragma unroll
-  for (int p = 0; p < (NC + 31) / 32; ++p) {
+  for (int p = 0; p < NC / 32; ++p) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if ((lane >> 4) == half) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (p * 32 + j < NC) scratch[(lane & 15) * kPitch + j] = acc[p * 32 + j];
+        for (int j = 0; j < 32; ++j) rows[(lane & 15) * kPitch + j] = acc[p * 32 + j];
       }
       __syncwarp();
       const int n = col + p * 32 + lane;
 #pragma unroll 4
       for (int r = 0; r < 16; ++r) {
         const int m = row_base + half * 16 + r;
-        if (m < g.M && n < g.N && p * 32 + lane < NC) c[static_cast<size_t>(m) * g.ldc + n] = round_to<T>(scratch[r * kPitch + lane]);
+        if (m < g.M && n < g.N) c[static_cast<size_t>(m) * g.ldc + n] = round_to<T>(rows[r * kPitch + lane]);
       }
       __syncwarp();
     }
@@ -131,14 +164,17 @@ __device__ __forceinline__ void store_row(const Args& g, int row, int col, float
 // B_ROWS: B has a scale for every row instead of for 128.
 template <int BN, bool B_ROWS>
 __global__ void __launch_bounds__(kPairThreads, 1)
-gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const __grid_constant__ Args g) {
+gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const __grid_constant__ CUtensorMap tma_c,
+                     const __grid_constant__ Args g, bool mapped) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int NS = kStages, NC = BN / 2;
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
-  PairCtl* ctl = reinterpret_cast<PairCtl*>(smem + NS * kPairStage<BN>);
-  uint8_t* scratch_all = reinterpret_cast<uint8_t*>(ctl + 1);
+  uint8_t* scratch_all = smem + NS * kPairStage<BN>;      // per promotion warp
+  PairCtl* ctl = reinterpret_cast<PairCtl*>(scratch_all + kPromoters * kScratchBytes);
+  float* slots = reinterpret_cast<float*>(ctl + 1);      // [2][kGroup][128 rows], then [kGroup][kCols], each
+  float* bias_all = slots + 2 * kSlot<BN, B_ROWS>;      // per promotion warp
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t cta = cluster_ctarank();   // 0: leader
@@ -150,11 +186,15 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(smem_u32(&ctl->full[s]), 2);
-      mbar_init(smem_u32(&ctl->empty[s]), 1);
+      mbar_init(smem_u32(&ctl->empty[s]), 2);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(smem_u32(&ctl->acc_full[b]), 1);
-      mbar_init(smem_u32(&ctl->acc_empty[b]), 2 * kPromoters);
+      mbar_init(smem_u32(&ctl->scales_full[b]), 32);
+      mbar_init(smem_u32(&ctl->scales_empty[b]), kPromoters);
+    }
+    for (int b = 0; b < 4; ++b) {
+      mbar_init(smem_u32(&ctl->acc_full[b >> 1][b & 1]), 1);
+      mbar_init(smem_u32(&ctl->acc_empty[b >> 1][b & 1]), kPromoters);
     }
     ctl->abort = 0;
     fence_barrier_init();
@@ -163,6 +203,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
   if (warp == 0 && lane == 0) {
     prefetch_tensormap(&tma_a);
     prefetch_tensormap(&tma_b);
+    if (mapped) prefetch_tensormap(&tma_c);
   }
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(&ctl->tmem_base), kTmemCols);
@@ -176,80 +217,114 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
   const uint64_t budget = g.wait_budget_ns;
   const bool leader = elect_one();   // the lane that issues for its warp
 
-  if (warp == 0) {
-    uint32_t it = 0, s = 0, ph = 1;   // ring position: count, stage, parity to wait for
-    bool ok = true;
-    const uint32_t leader_full = map_to_cta(smem_u32(&ctl->full[0]), 0);
-    for (int t = pair; t < num_tiles && ok; t += n_pairs) {
-      int tm, tn;
-      tiles.at(t, &tm, &tn);
-      const int row_a = tm * 256 + static_cast<int>(cta) * 128, row_b = tn * BN + static_cast<int>(cta) * (BN / 2);
-      for (int kb = 0; kb < num_kb; ++kb, ++it) {
-        if (!mbar_wait_warp(smem_u32(&ctl->empty[0]) + s * 8u, ph, &ctl->abort, budget)) { ok = false; break; }
-        if (leader) {
-          const uint32_t full = leader_full + s * 8u, dst = base + s * kPairStage<BN>;
-          mbar_arrive_expect_tx_cluster(full, kPairStage<BN>);
-          tma_load_2d_pair(dst, &tma_a, full, kb * kBlockK, row_a);
-          tma_load_2d_pair(dst + kTileBytes, &tma_b, full, kb * kBlockK, row_b);
-        }
-        if (++s == NS) { s = 0; ph ^= 1u; }
-      }
-    }
-    // Both CTAs' loads count on the leader's barriers, and its partner stays until the cluster barrier at the end.  Where
-    // this producer gave up, the partner may be up to a ring ahead.
-    if (cta == 0) {
-      loads_land(&ctl->full[0], NS, it, budget);
-      if (!ok) loads_land(&ctl->full[0], NS, it + NS, budget);
-    }
-  } else if (warp == 1) {
-    if (cta == 0) {
-      constexpr uint32_t idesc = make_idesc_e4m3(256, BN);
-      const uint64_t da0 = make_smem_desc_sw128(base), db0 = make_smem_desc_sw128(base + kTileBytes);
-      uint32_t s = 0, ph = 0, it = 0;
+  if (warp < kFirst) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+    if (warp == 0) {
+      uint32_t it = 0, s = 0, ph = 1;   // ring position: count, stage, parity to wait for
       bool ok = true;
+      const uint32_t leader_full = map_to_cta(smem_u32(&ctl->full[0]), 0);
       for (int t = pair; t < num_tiles && ok; t += n_pairs) {
+        int tm, tn;
+        tiles.at(t, &tm, &tn);
+        const int row_a = tm * 256 + static_cast<int>(cta) * 128, row_b = tn * BN + static_cast<int>(cta) * (BN / 4);
         for (int kb = 0; kb < num_kb; ++kb, ++it) {
-          const uint32_t buf = it & 1u, acc_ph = (it >> 1) & 1u;
-          ok = mbar_wait_warp(smem_u32(&ctl->acc_empty[0]) + buf * 8u, acc_ph ^ 1u, &ctl->abort, budget);
-          if (!ok) break;
-          ok = mbar_wait_warp(smem_u32(&ctl->full[0]) + s * 8u, ph, &ctl->abort, budget);
-          if (!ok) break;
-          tc_fence_after_sync();
-          const uint64_t da = da0 + static_cast<uint64_t>(s * (kPairStage<BN> >> 4)), db = db0 + static_cast<uint64_t>(s * (kPairStage<BN> >> 4));
+          if (!mbar_wait_warp(smem_u32(&ctl->empty[0]) + s * 8u, ph, &ctl->abort, budget)) { ok = false; break; }
           if (leader) {
-#pragma unroll
-            for (int k = 0; k < kBlockK / kMmaK; ++k)
-              umma_e4m3_pair(tmem_base + buf * 256u, da + static_cast<uint64_t>(k * 2), db + static_cast<uint64_t>(k * 2), idesc, k != 0 ? 1u : 0u);
-            umma_commit_pair(smem_u32(&ctl->empty[0]) + s * 8u, 3);      // the stage is free in both CTAs
-            umma_commit_pair(smem_u32(&ctl->acc_full[0]) + buf * 8u, 3);
+            const uint32_t full = leader_full + s * 8u, dst = base + s * kPairStage<BN>;
+            mbar_arrive_expect_tx_cluster(full, kPairStage<BN>);
+            tma_load_2d_pair(dst, &tma_a, full, kb * kBlockK, row_a);
+            tma_load_2d_pair(dst + kTileBytes, &tma_b, full, kb * kBlockK, row_b);   // a quarter of the tile's rows of B for each half
+            tma_load_2d_pair(dst + kTileBytes + BN / 4 * kBlockK, &tma_b, full, kb * kBlockK, row_b + NC);
           }
           if (++s == NS) { s = 0; ph ^= 1u; }
         }
       }
+      // Both CTAs' loads count on the leader's barriers, and its partner stays until the cluster barrier at the end.  Where
+      // this producer gave up, the partner may be up to a ring ahead.
+      if (cta == 0) {
+        loads_land(&ctl->full[0], NS, it, budget);
+        if (!ok) loads_land(&ctl->full[0], NS, it + NS, budget);
+      }
+    } else if (warp < 3) {
+      if (cta == 0) {
+        constexpr uint32_t idesc = make_idesc_e4m3(256, NC);
+        const uint32_t half = static_cast<uint32_t>(warp) - 1u;
+        const uint64_t da0 = make_smem_desc_sw128(base), db0 = make_smem_desc_sw128(base + kTileBytes + half * (BN / 4 * kBlockK));
+        const uint32_t full = smem_u32(&ctl->full[0]), empty = smem_u32(&ctl->empty[0]);
+        const uint32_t acc_full = smem_u32(&ctl->acc_full[0][half]), acc_empty = smem_u32(&ctl->acc_empty[0][half]);
+        uint32_t s = 0, ph = 0, it = 0;
+        bool ok = true;
+        for (int t = pair; t < num_tiles && ok; t += n_pairs) {
+          for (int kb = 0; kb < num_kb; ++kb, ++it) {
+            const uint32_t buf = it & 1u, acc_ph = (it >> 1) & 1u;
+            ok = mbar_wait_both(full + s * 8u, ph, acc_empty + buf * 16u, acc_ph ^ 1u, &ctl->abort, budget);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint64_t da = da0 + static_cast<uint64_t>(s * (kPairStage<BN> >> 4)), db = db0 + static_cast<uint64_t>(s * (kPairStage<BN> >> 4));
+            if (leader) {
+#pragma unroll
+              for (int k = 0; k < kBlockK / kMmaK; ++k)   // 32 bytes on inside a 128-byte swizzle row: +2 in the address field
+                umma_e4m3_pair(tmem_base + buf * 256u + half * NC, da + static_cast<uint64_t>(k * 2), db + static_cast<uint64_t>(k * 2), idesc, k != 0 ? 1u : 0u);
+              umma_commit_pair(acc_full + buf * 16u, 3);
+              umma_commit_pair(empty + s * 8u, 3);   // with the other half's: the stage is free in both CTAs
+            }
+            if (++s == NS) { s = 0; ph ^= 1u; }
+          }
+        }
+      }
+    } else {
+      // Scales: of this CTA's 128 rows, and of B the tile's columns or, for each half of them, the two blocks of 128 rows that it may touch.
+      uint32_t group = 0;
+      bool ok = true;
+      for (int t = pair; t < num_tiles && ok; t += n_pairs) {
+        int tm, tn;
+        tiles.at(t, &tm, &tn);
+        constexpr int kOwn = B_ROWS ? BN / 32 : 1;
+        const float *rows[4], *cols[kOwn];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) rows[j] = g.a.at(min(tm * 256 + static_cast<int>(cta) * 128 + lane + j * 32, g.M - 1));
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) {
+          const int n = B_ROWS ? tn * BN + lane + j * 32 : ((tn * BN + (lane >> 1 & 1) * NC) & ~127) + (lane & 1) * 128;
+          cols[j] = g.b.at(min(n, g.N - 1)) + (B_ROWS ? 0 : (lane >> 2) * g.b.blk);   // lanes 4i .. 4i + 3 fetch the group's i-th block
+        }
+        for (int kb = 0; kb < num_kb; kb += kGroup, ++group) {
+          ok = mbar_wait_warp(smem_u32(&ctl->scales_empty[group & 1u]), (group >> 1 & 1u) ^ 1u, &ctl->abort, budget);
+          if (!ok) break;
+          float* slot = slots + (group & 1u) * kSlot<BN, B_ROWS>;
+          for (int i = 0; i < kGroup && kb + i < num_kb; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              copy4_async(slot + i * 128 + lane + j * 32, rows[j]);
+              rows[j] += g.a.blk;
+            }
+            if constexpr (B_ROWS) {
+#pragma unroll
+              for (int j = 0; j < kOwn; ++j) {
+                copy4_async(slot + kGroup * 128 + i * BN + lane + j * 32, cols[j]);
+                cols[j] += g.b.blk;
+              }
+            }
+          }
+          if constexpr (!B_ROWS) {
+            if (lane < 4 * kGroup && kb + (lane >> 2) < num_kb) copy4_async(slot + kGroup * 128 + lane, cols[0]);
+            cols[0] += kGroup * g.b.blk;
+          }
+          copies_arrive(smem_u32(&ctl->scales_full[group & 1u]));
+        }
+      }
+      copies_wait();
     }
   } else {
-    const int q = warp & 3, first_col = ((warp - 2) >> 2) * NC;
-    float* scratch = reinterpret_cast<float*>(scratch_all + (warp - 2) * kScratchBytes);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromoterRegs));
+    const int q = warp & 3, half = (warp - kFirst) >> 2, first_col = half * NC;
+    uint8_t* scratch = scratch_all + (warp - kFirst) * kScratchBytes;
+    float* bias = bias_all + (warp - kFirst) * kBiasFloats;
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + first_col;
-    const uint32_t acc_empty = map_to_cta(smem_u32(&ctl->acc_empty[0]), 0);
-    // Scales of the block to come, fetched a block ahead (across tiles too): this lane's row; of B the two blocks of 128 rows that the warp's
-    // columns may touch, or a lane's share of the columns.
-    constexpr int kOwn = B_ROWS ? (NC + 31) / 32 : 2;
-    float rs = 0.0f, cs[kOwn];
-    const auto fetch = [&](int t, int kb) {
-      int tm, tn;
-      tiles.at(t, &tm, &tn);
-      rs = __ldg(g.a.at(min(tm * 256 + static_cast<int>(cta) * 128 + q * 32 + lane, g.M - 1)) + kb * g.a.blk);
-      const int col = tn * BN + first_col;
-#pragma unroll
-      for (int j = 0; j < kOwn; ++j) {
-        const int n = B_ROWS ? col + lane + j * 32 : (col & ~127) + j * 128;
-        cs[j] = __ldg(g.b.at(min(n, g.N - 1)) + kb * g.b.blk);
-      }
-    };
+    const uint32_t acc_full = smem_u32(&ctl->acc_full[0][half]), acc_empty = map_to_cta(smem_u32(&ctl->acc_empty[0][half]), 0);
+    uint32_t group = 0;
     uint32_t it = 0;
-    bool ok = true;
-    if (pair < num_tiles) fetch(pair, 0);
+    bool ok = true, ready = false;
     for (int t = pair; t < num_tiles && ok; t += n_pairs) {
       int tm, tn;
       tiles.at(t, &tm, &tn);
@@ -257,57 +332,76 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
       float acc[NC];
 #pragma unroll
       for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
-      for (int kb = 0; kb < num_kb; ++kb, ++it) {
-        const uint32_t buf = it & 1u, acc_ph = (it >> 1) & 1u;
-        const float r = rs;
-        float s[2];
-        if constexpr (B_ROWS) {
-#pragma unroll
-          for (int j = 0; j < kOwn; ++j) scratch[(it & 1u) * 128 + lane + j * 32] = cs[j];
-          __syncwarp();   // the scales of two blocks ago have been read, this block's are written
-        } else {
-          s[0] = r * cs[0];
-          s[1] = r * cs[1];
-        }
-        if (kb + 1 < num_kb) fetch(t, kb + 1);
-        else if (t + n_pairs < num_tiles) fetch(t + n_pairs, 0);
-        ok = mbar_wait_warp(smem_u32(&ctl->acc_full[0]) + buf * 8u, acc_ph, &ctl->abort, budget);
+      for (int kb = 0; kb < num_kb && ok; kb += kGroup, ++group) {
+        ok = mbar_wait_warp(smem_u32(&ctl->scales_full[group & 1u]), group >> 1 & 1u, &ctl->abort, budget);
         if (!ok) break;
-        tc_fence_after_sync();
-        promote<NC>(
-            taddr + buf * 256u,
-            [&](int c, const uint32_t (&v)[16]) {
-              if constexpr (B_ROWS) {
+        const float* rows = slots + (group & 1u) * kSlot<BN, B_ROWS> + q * 32 + lane;
+        const float* cols = slots + (group & 1u) * kSlot<BN, B_ROWS> + kGroup * 128 + (B_ROWS ? first_col : half * 2);
+        float x[kGroup][2];   // the row's scale, or its products with B's
 #pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                  const float4 b = *reinterpret_cast<const float4*>(scratch + (it & 1u) * 128 + c * 16 + j);
-                  acc[c * 16 + j] += __uint_as_float(v[j]) * r * b.x;
-                  acc[c * 16 + j + 1] += __uint_as_float(v[j + 1]) * r * b.y;
-                  acc[c * 16 + j + 2] += __uint_as_float(v[j + 2]) * r * b.z;
-                  acc[c * 16 + j + 3] += __uint_as_float(v[j + 3]) * r * b.w;
+        for (int i = 0; i < kGroup; ++i) {   // (blocks beyond the last one: not used)
+          x[i][0] = x[i][1] = rows[i * 128];
+          if constexpr (!B_ROWS) {
+            x[i][0] *= cols[i * 4];
+            x[i][1] *= cols[i * 4 + 1];
+          }
+        }
+        if constexpr (!B_ROWS) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&ctl->scales_empty[group & 1u]));
+        }
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          if (kb + i >= num_kb) break;
+          const uint32_t buf = it & 1u, acc_ph = (it >> 1) & 1u;
+          ++it;
+          ok = __all_sync(0xffffffffu, ready) || mbar_wait_warp(acc_full + buf * 16u, acc_ph, &ctl->abort, budget);
+          if (!ok) break;
+          tc_fence_after_sync();
+          promote<NC, B_ROWS ? 32 : 64>(
+              taddr + buf * 256u,
+              [&](int c, const auto& v) {
+                constexpr int kPiece = sizeof(v) / 4;
+                if constexpr (B_ROWS) {
+#pragma unroll
+                  for (int j = 0; j < kPiece; j += 4) {
+                    const float4 b = *reinterpret_cast<const float4*>(cols + i * BN + c + j);
+                    acc[c + j] += __uint_as_float(v[j]) * x[i][0] * b.x;
+                    acc[c + j + 1] += __uint_as_float(v[j + 1]) * x[i][0] * b.y;
+                    acc[c + j + 2] += __uint_as_float(v[j + 2]) * x[i][0] * b.z;
+                    acc[c + j + 3] += __uint_as_float(v[j + 3]) * x[i][0] * b.w;
+                  }
+                } else {
+#pragma unroll
+                  for (int h = 0; h < kPiece; h += 32) {
+                    const float y = BN != 192 || (col & 127) + c + h < 128 ? x[i][0] : x[i][1];   // 32 columns lie in one block: col is a multiple of 32
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) acc[c + h + j] += __uint_as_float(v[h + j]) * y;
+                  }
                 }
-              } else {
-                const float x = (col & 127) + c * 16 < 128 ? s[0] : s[1];   // a piece lies in one block: col is a multiple of 16
-#pragma unroll
-                for (int j = 0; j < 16; ++j) acc[c * 16 + j] += __uint_as_float(v[j]) * x;
-              }
-            },
-            [&] {
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_cluster(acc_empty + buf * 8u);
-            });
+              },
+              [&] {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(acc_empty + buf * 16u);
+                ready = mbar_test(acc_full + (buf ^ 1u) * 16u, (it >> 1) & 1u);   // the next block: its answer is there when the sums are done
+              });
+        }
+        if constexpr (B_ROWS) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&ctl->scales_empty[group & 1u]));
+        }
       }
       if (!ok) break;
-      if constexpr (B_ROWS) __syncwarp();   // the scratch holds scales up to here
       if (col < g.N) {
         switch (g.type) {
-          case 6: store_row<__half>(g, row, col, acc, scratch, lane); break;
-          case 7: store_row<float>(g, row, col, acc, scratch, lane); break;
-          default: store_row<__nv_bfloat16>(g, row, col, acc, scratch, lane);
+          case 6: store_rows<__half>(g, &tma_c, mapped, row, col, acc, scratch, bias, lane); break;
+          case 7: store_rows<float>(g, &tma_c, mapped, row, col, acc, scratch, bias, lane); break;
+          default: store_rows<__nv_bfloat16>(g, &tma_c, mapped, row, col, acc, scratch, bias, lane);
         }
       }
     }
+    if (lane == 0) bulk_wait_all();   // what is on its way out lies in this CTA's shared memory
   }
 
   tc_fence_before_sync();
@@ -321,11 +415,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
 }
 
 template <int BN, bool B_ROWS>
-cudaError_t fire(const CUtensorMap& ta, const CUtensorMap& tb, const Args& g, int tiles, cudaStream_t stream) {
+cudaError_t fire(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, bool mapped, const Args& g, int tiles, cudaStream_t stream) {
   auto kernel = gemm_fp8_pair_kernel<BN, B_ROWS>;
-  constexpr int smem_bytes = kStages * kPairStage<BN> + 1024 /*alignment slack*/ + static_cast<int>(sizeof(PairCtl)) + kPromoters * kScratchBytes;
+  constexpr int smem_bytes = kStages * kPairStage<BN> + 1024 /*alignment slack*/ + static_cast<int>(sizeof(PairCtl)) + 2 * kSlot<BN, B_ROWS> * 4 +
+                             kPromoters * (kScratchBytes + kBiasFloats * 4);
+  static_assert(kPairStage<BN> % 1024 == 0 && 16 * kPitch * 4 <= kScratchBytes, "layout of shared memory");
   static_assert(smem_bytes <= 227 * 1024, "shared memory");
-  static_assert(2 * 128 * 4 <= kScratchBytes, "two blocks' scales fit the scratch");
   static int most_dev[kMaxDevices] = {};   // pairs that the device holds at once, which a persistent kernel must not exceed
   int& most = most_dev[current_device_slot()];
   cudaLaunchConfig_t cfg = {};
@@ -352,14 +447,28 @@ cudaError_t fire(const CUtensorMap& ta, const CUtensorMap& tb, const Args& g, in
     most = n;
   }
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min(tiles, most)));
-  return cudaLaunchKernelEx(&cfg, kernel, ta, tb, g);
+  return cudaLaunchKernelEx(&cfg, kernel, ta, tb, tc, g, mapped);
+}
+
+// C for stores of 32 rows of 64 bytes; false where its rows do not start on 16 bytes.
+bool make_tensor_map_out(CUtensorMap* map, const Args& g) {
+  const CudaDriver* d = CudaDriver::get();
+  const cuuint64_t size = g.type == 7 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(g.c) & 15u) != 0 || g.ldc * size % 16 != 0 || g.ldc * size >= (1ull << 40)) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(g.N), static_cast<cuuint64_t>(g.M)};
+  cuuint64_t strides[1] = {g.ldc * size};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(kOutRow / size), 32};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = g.type == 7 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  return d->TensorMapEncodeTiled(map, type, 2, g.c, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // The tile width that needs the fewest waves times (columns + 256): a narrower tile pays where it saves a wave.
 int pick_width(int M, int N, int pairs, long* cost) {
   int best = 256;
   *cost = -1;
-  for (const int bn : {256, 224, 192, 128}) {
+  for (const int bn : {256, 192, 128}) {
     const long tiles = static_cast<long>((M + 255) / 256) * ((N + bn - 1) / bn), c = (tiles + pairs - 1) / pairs * (bn + 64);
     if (*cost < 0 || c < *cost) {
       *cost = c;
@@ -384,17 +493,18 @@ int run(const void* a, int64_t lda, const void* b, int64_t ldb, Args g, cudaStre
   } else {
     const long tiles = static_cast<long>((g.M + 255) / 256) * ((g.N + bn - 1) / bn);
     if (tiles > 0x7fffffff / 2) return -2;
-    CUtensorMap ta, tb;
-    if (!make_tensor_map_e4m3(&ta, a, g.M, g.K, lda, 128, &why) || !make_tensor_map_e4m3(&tb, b, g.N, g.K, ldb, bn / 2, &why)) {
+    CUtensorMap ta, tb, tc = {};
+    bool mapped = false;
+    if (!make_tensor_map_e4m3(&ta, a, g.M, g.K, lda, 128, &why) || !make_tensor_map_e4m3(&tb, b, g.N, g.K, ldb, bn / 4, &why)) {
       e = cudaErrorInvalidValue;
     } else {
+      mapped = make_tensor_map_out(&tc, g);
       const auto go = [&](auto rows) {
         constexpr bool R = decltype(rows)::value;
         switch (bn) {
-          case 256: return fire<256, R>(ta, tb, g, static_cast<int>(tiles), stream);
-          case 224: return fire<224, R>(ta, tb, g, static_cast<int>(tiles), stream);
-          case 192: return fire<192, R>(ta, tb, g, static_cast<int>(tiles), stream);
-          default: return fire<128, R>(ta, tb, g, static_cast<int>(tiles), stream);
+          case 256: return fire<256, R>(ta, tb, tc, mapped, g, static_cast<int>(tiles), stream);
+          case 192: return fire<192, R>(ta, tb, tc, mapped, g, static_cast<int>(tiles), stream);
+          default: return fire<128, R>(ta, tb, tc, mapped, g, static_cast<int>(tiles), stream);
         }
       };
       e = g.b.shift == 0 ? go(std::true_type{}) : go(std::false_type{});

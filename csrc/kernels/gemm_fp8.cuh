@@ -6,7 +6,9 @@
 // The tensor cores compute one block's P_b into an accumulator of its own (four tcgen05.mma of kind f8f6f4, K = 32 each);
 // "promotion" warps read it from tensor memory, multiply by the scales and add it to sums that they hold in registers.
 // So scales are any fp32 numbers, and between blocks everything is added in fp32.  Accumulators alternate: one block is
-// promoted while the next ones are multiplied.  The control flow (bounded waits, one elected lane that issues for its
+// promoted while the next ones are multiplied.
+//
+// The control flow (bounded waits, one elected lane that issues for its
 // warp, a producer that stays until its loads have landed) is that of the bf16 kernels.
 #pragma once
 #include <cuda_bf16.h>
@@ -24,6 +26,10 @@ namespace fp8 {
 constexpr int kBlockK = 128;                  // elements, and bytes: a 128-byte swizzle row
 constexpr int kTileBytes = 128 * kBlockK;     // 128 rows of an operand: 16 KB
 constexpr int kMmaK = 32;
+// A warp of its own brings the scales into shared memory, for this many blocks at a time and a group ahead: a promotion warp that fetched its
+// own spent more time on that than on its sums, and a plain load in flight holds up the thread's next arrival on a barrier (which
+// releases what came before it): with scales loaded a block ahead the persistent kernel took 1000 cycles a block.
+constexpr int kGroup = 4;
 
 // Scales of one operand: element (row >> shift, block) with strides.
 struct Scales {
@@ -69,30 +75,98 @@ __device__ __forceinline__ void umma_e4m3_pair(uint32_t tmem_d, uint64_t desc_a,
       : "memory");
 }
 
-// The wait for this thread's tensor-memory loads, tied to the registers they fill: no use of them can move above it.
-__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
-                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
+// 32 lanes x 16, 32 or 64 columns of tensor memory, read and waited for in one statement, so that no use of the registers can come before the
+// wait.  (A wait apart that names the registers it covers costs a move for each of them: half of the promotion warps' instructions.)
+__device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
 }
 
-// This lane's row of a block's accumulator, NC columns from `taddr` on, 16 at a time: use(c, values) for each piece while the next one
-// is on its way, released() once the last has been read.
-template <int NC, typename Use, typename Released>
+// This lane's row of a block's accumulator, NC columns from `taddr` on, at most MOST at a time: use(first column, values) for each piece,
+// released() once the last has been read.
+template <int NC, int MOST, int C = 0, typename Use, typename Released>
 __device__ __forceinline__ void promote(uint32_t taddr, Use use, Released released) {
-  static_assert(NC % 16 == 0, "whole pieces");
-  uint32_t r[2][16];
-  tmem_ld_32x16(taddr, r[0]);
-  tmem_ld_wait(r[0]);
-#pragma unroll
-  for (int c = 0; c < NC / 16; ++c) {
-    if (c + 1 < NC / 16) tmem_ld_32x16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
-    else released();
-    use(c, r[c & 1]);
-    if (c + 1 < NC / 16) tmem_ld_wait(r[(c + 1) & 1]);
-  }
+  constexpr int kPiece = MOST >= 64 && NC - C >= 64 ? 64 : NC - C >= 32 ? 32 : 16;
+  uint32_t r[kPiece];
+  tmem_read(taddr + C, r);
+  if constexpr (C + kPiece == NC) released();
+  use(C, r);
+  if constexpr (C + kPiece < NC) promote<NC, MOST, C + kPiece>(taddr, use, released);
+}
+
+// Whether a barrier's phase is over, without waiting.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// Four bytes, global -> shared, without the thread waiting for them; an arrival on `bar` (counted among those it expects) when all of this
+// thread's copies so far have landed.
+__device__ __forceinline__ void copy4_async(float* dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Two waits that take one trip where both phases are over already.
+__device__ __forceinline__ bool mbar_wait_both(uint32_t bar, uint32_t parity, uint32_t bar2, uint32_t parity2, volatile uint32_t* abort_flag, uint64_t budget_ns) {
+  const bool first = mbar_try_wait(bar, parity), second = mbar_try_wait(bar2, parity2);
+  if (__all_sync(0xffffffffu, first && second)) return true;
+  return mbar_wait_warp(bar, parity, abort_flag, budget_ns) && mbar_wait_warp(bar2, parity2, abort_flag, budget_ns);
+}
+
+// Tiled store shared -> global, tracked by bulk async-groups; what lies outside the tensor is not written.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t smem_src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_src), "r"(c0),
+               "r"(c1)
+               : "memory");
 }
 
 template <typename T>

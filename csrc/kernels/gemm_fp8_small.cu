@@ -21,6 +21,8 @@ template <int TN>
 constexpr int kCols = TN / (kWarps<TN> / 4);      // columns a promotion warp holds
 template <int TN>
 constexpr int kBuffers = TN >= 128 ? 2 : 4;       // accumulators
+template <int TN>
+constexpr int kSlot = kGroup * (32 + kCols<TN>);   // floats: a group's scales of a promotion warp
 constexpr int kMostStages = 12;
 
 struct __align__(16) Ctl {
@@ -74,7 +76,7 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
   Ctl* ctl = reinterpret_cast<Ctl*>(smem + NS * kStage<TN>);
-  float* col_scales = reinterpret_cast<float*>(ctl + 1);   // [promotion warp][2][NC]
+  float* scales = reinterpret_cast<float*>(ctl + 1);   // [promotion warp][2][kSlot]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slices = static_cast<int>(cluster_size());
@@ -161,50 +163,68 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
       if (++s == NS) { s = 0; ph ^= 1u; }
     }
   } else {
-    const float* row_scale = g.b.at(min(n, g.N - 1));
-    constexpr int kOwn = (NC + 31) / 32;   // column scales a lane fetches for its warp
+    // Brings the scales of the next group of blocks into slot `to`: this lane's row of B, the lane's share of the columns.
+    constexpr int kOwn = (NC + 31) / 32;
+    const float* row_scale = g.b.at(min(n, g.N - 1)) + kb0 * g.b.blk;
     const float* col_scale[kOwn];
 #pragma unroll
-    for (int j = 0; j < kOwn; ++j) col_scale[j] = g.a.at(min(m0 + first_col + (lane + j * 32) % NC, g.M - 1));
-    float* box = col_scales + (warp - 2) * 2 * NC;
-    float rs, cs[kOwn];
-    auto fetch = [&](int i) {
-      rs = __ldg(row_scale + (kb0 + i) * g.b.blk);
+    for (int j = 0; j < kOwn; ++j) col_scale[j] = g.a.at(min(m0 + first_col + lane + j * 32, g.M - 1)) + kb0 * g.a.blk;
+    float* slots = scales + (warp - 2) * 2 * kSlot<TN>;
+    int ahead = 0;
+    const auto fetch = [&](uint32_t to) {
+      float* slot = slots + to * kSlot<TN>;
 #pragma unroll
-      for (int j = 0; j < kOwn; ++j) cs[j] = __ldg(col_scale[j] + (kb0 + i) * g.a.blk);
+      for (int i = 0; i < kGroup; ++i) {
+        if (ahead + i >= nkb) break;
+        copy4_async(slot + i * 32 + lane, row_scale);
+        row_scale += g.b.blk;
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) {
+          if (lane + j * 32 < NC) copy4_async(slot + kGroup * 32 + i * NC + lane + j * 32, col_scale[j]);
+          col_scale[j] += g.a.blk;
+        }
+      }
+      ahead += kGroup;
     };
     fetch(0);
     const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + first_col;
-    for (int i = 0; i < nkb; ++i) {
-      float* mine = box + (i & 1) * NC;
+    uint32_t group = 0;
+    for (int i0 = 0; i0 < nkb && ok; i0 += kGroup, group ^= 1u) {
+      copies_wait();
+      __syncwarp();   // this group's scales are there, the other slot's have been read
+      const float* rows = slots + group * kSlot<TN>;
+      const float* cols = rows + kGroup * 32;
+      float x[kGroup];
 #pragma unroll
-      for (int j = 0; j < kOwn; ++j)
-        if (lane + j * 32 < NC) mine[lane + j * 32] = cs[j];
-      const float r = rs;
-      __syncwarp();   // the box of two blocks ago has been read, this one's is written
-      if (i + 1 < nkb) fetch(i + 1);
-      const uint32_t buf = static_cast<uint32_t>(i) % NB, acc_ph = (static_cast<uint32_t>(i) / NB) & 1u;
-      ok = mbar_wait_warp(smem_u32(&ctl->acc_full[0]) + buf * 8u, acc_ph, &ctl->abort, g.wait_budget_ns);
-      if (!ok) break;
-      tc_fence_after_sync();
-      promote<NC>(
-          taddr + buf * TN,
-          [&](int c, const uint32_t (&v)[16]) {
+      for (int i = 0; i < kGroup; ++i) x[i] = rows[i * 32 + lane];
+      fetch(group ^ 1u);
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const float4 s = *reinterpret_cast<const float4*>(mine + c * 16 + j);
-              acc[c * 16 + j] += __uint_as_float(v[j]) * r * s.x;
-              acc[c * 16 + j + 1] += __uint_as_float(v[j + 1]) * r * s.y;
-              acc[c * 16 + j + 2] += __uint_as_float(v[j + 2]) * r * s.z;
-              acc[c * 16 + j + 3] += __uint_as_float(v[j + 3]) * r * s.w;
-            }
-          },
-          [&] {
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&ctl->acc_empty[0]) + buf * 8u);
-          });
+      for (int i = 0; i < kGroup; ++i) {
+        if (i0 + i >= nkb) break;
+        const uint32_t buf = static_cast<uint32_t>(i0 + i) % NB, acc_ph = (static_cast<uint32_t>(i0 + i) / NB) & 1u;
+        ok = mbar_wait_warp(smem_u32(&ctl->acc_full[0]) + buf * 8u, acc_ph, &ctl->abort, g.wait_budget_ns);
+        if (!ok) break;
+        tc_fence_after_sync();
+        promote<NC, 32>(
+            taddr + buf * TN,
+            [&](int c, const auto& v) {
+#pragma unroll
+              for (int j = 0; j < static_cast<int>(sizeof(v) / 4); j += 4) {
+                const float4 s = *reinterpret_cast<const float4*>(cols + i * NC + c + j);
+                acc[c + j] += __uint_as_float(v[j]) * x[i] * s.x;
+                acc[c + j + 1] += __uint_as_float(v[j + 1]) * x[i] * s.y;
+                acc[c + j + 2] += __uint_as_float(v[j + 2]) * x[i] * s.z;
+                acc[c + j + 3] += __uint_as_float(v[j + 3]) * x[i] * s.w;
+              }
+            },
+            [&] {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(&ctl->acc_empty[0]) + buf * 8u);
+            });
+      }
     }
+    copies_wait();
   }
   __syncwarp();
 
@@ -251,7 +271,7 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
 template <int TN, int NS>
 cudaError_t fire(const CUtensorMap& tw, const CUtensorMap& tx, const SmallArgs& a, const SmallPlan& p, cudaStream_t stream) {
   auto kernel = gemm_fp8_small_kernel<TN, NS>;
-  constexpr int smem_bytes = NS * kStage<TN> + 1024 /*alignment slack*/ + static_cast<int>(sizeof(Ctl)) + kWarps<TN> * 2 * kCols<TN> * 4;
+  constexpr int smem_bytes = NS * kStage<TN> + 1024 /*alignment slack*/ + static_cast<int>(sizeof(Ctl)) + kWarps<TN> * 2 * kSlot<TN> * 4;
   static_assert(smem_bytes <= 227 * 1024, "shared memory");
   static_assert(TN * 128 * 4 <= NS * kStage<TN>, "the slices' partial sums fit the ring");
   static bool configured[kMaxDevices] = {};
