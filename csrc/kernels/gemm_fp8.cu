@@ -308,6 +308,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
           }
           if constexpr (!B_ROWS) {
             if (lane < 4 * kGroup && kb + (lane >> 2) < num_kb) copy4_async(slot + kGroup * 128 + lane, cols[0]);
+            static_assert(4 * kGroup <= 32, "a lane for each of a group's scales");
             cols[0] += kGroup * g.b.blk;
           }
           copies_arrive(smem_u32(&ctl->scales_full[group & 1u]));
@@ -332,64 +333,59 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
       float acc[NC];
 #pragma unroll
       for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
-      for (int kb = 0; kb < num_kb && ok; kb += kGroup, ++group) {
-        ok = mbar_wait_warp(smem_u32(&ctl->scales_full[group & 1u]), group >> 1 & 1u, &ctl->abort, budget);
-        if (!ok) break;
-        const float* rows = slots + (group & 1u) * kSlot<BN, B_ROWS> + q * 32 + lane;
-        const float* cols = slots + (group & 1u) * kSlot<BN, B_ROWS> + kGroup * 128 + (B_ROWS ? first_col : half * 2);
-        float x[kGroup][2];   // the row's scale, or its products with B's
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i) {   // (blocks beyond the last one: not used)
-          x[i][0] = x[i][1] = rows[i * 128];
-          if constexpr (!B_ROWS) {
-            x[i][0] *= cols[i * 4];
-            x[i][1] *= cols[i * 4 + 1];
-          }
-        }
-        if constexpr (!B_ROWS) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&ctl->scales_empty[group & 1u]));
-        }
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i) {
-          if (kb + i >= num_kb) break;
-          const uint32_t buf = it & 1u, acc_ph = (it >> 1) & 1u;
-          ++it;
-          ok = __all_sync(0xffffffffu, ready) || mbar_wait_warp(acc_full + buf * 16u, acc_ph, &ctl->abort, budget);
+      // One rolled loop: unrolled by groups, with their scales in registers, it ran into instruction-cache misses.
+#pragma unroll 1
+      for (int kb = 0; kb < num_kb; ++kb) {
+        const int i = kb % kGroup;
+        if (i == 0) {
+          ok = mbar_wait_warp(smem_u32(&ctl->scales_full[group & 1u]), group >> 1 & 1u, &ctl->abort, budget);
           if (!ok) break;
-          tc_fence_after_sync();
-          promote<NC, B_ROWS ? 32 : 64>(
-              taddr + buf * 256u,
-              [&](int c, const auto& v) {
-                constexpr int kPiece = sizeof(v) / 4;
-                if constexpr (B_ROWS) {
-#pragma unroll
-                  for (int j = 0; j < kPiece; j += 4) {
-                    const float4 b = *reinterpret_cast<const float4*>(cols + i * BN + c + j);
-                    acc[c + j] += __uint_as_float(v[j]) * x[i][0] * b.x;
-                    acc[c + j + 1] += __uint_as_float(v[j + 1]) * x[i][0] * b.y;
-                    acc[c + j + 2] += __uint_as_float(v[j + 2]) * x[i][0] * b.z;
-                    acc[c + j + 3] += __uint_as_float(v[j + 3]) * x[i][0] * b.w;
-                  }
-                } else {
-#pragma unroll
-                  for (int h = 0; h < kPiece; h += 32) {
-                    const float y = BN != 192 || (col & 127) + c + h < 128 ? x[i][0] : x[i][1];   // 32 columns lie in one block: col is a multiple of 32
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) acc[c + h + j] += __uint_as_float(v[h + j]) * y;
-                  }
-                }
-              },
-              [&] {
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(acc_empty + buf * 16u);
-                ready = mbar_test(acc_full + (buf ^ 1u) * 16u, (it >> 1) & 1u);   // the next block: its answer is there when the sums are done
-              });
         }
-        if constexpr (B_ROWS) {
+        const float* slot = slots + (group & 1u) * kSlot<BN, B_ROWS>;
+        const float* cols = slot + kGroup * 128 + (B_ROWS ? i * BN + first_col : i * 4 + half * 2);
+        const float r = slot[i * 128 + q * 32 + lane];
+        float x[2];   // the row's scale, or its products with B's
+        if constexpr (!B_ROWS) {
+          x[0] = r * cols[0];
+          x[1] = r * cols[1];
+        }
+        const uint32_t buf = it & 1u, acc_ph = (it >> 1) & 1u;
+        ++it;
+        ok = __all_sync(0xffffffffu, ready) || mbar_wait_warp(acc_full + buf * 16u, acc_ph, &ctl->abort, budget);
+        if (!ok) break;
+        tc_fence_after_sync();
+        promote<NC, B_ROWS ? 32 : 64>(
+            taddr + buf * 256u,
+            [&](int c, const auto& v) {
+              constexpr int kPiece = sizeof(v) / 4;
+              if constexpr (B_ROWS) {
+#pragma unroll
+                for (int j = 0; j < kPiece; j += 4) {
+                  const float4 b = *reinterpret_cast<const float4*>(cols + c + j);
+                  acc[c + j] += __uint_as_float(v[j]) * r * b.x;
+                  acc[c + j + 1] += __uint_as_float(v[j + 1]) * r * b.y;
+                  acc[c + j + 2] += __uint_as_float(v[j + 2]) * r * b.z;
+                  acc[c + j + 3] += __uint_as_float(v[j + 3]) * r * b.w;
+                }
+              } else {
+#pragma unroll
+                for (int h = 0; h < kPiece; h += 32) {
+                  const float y = BN != 192 || (col & 127) + c + h < 128 ? x[0] : x[1];   // 32 columns lie in one block: col is a multiple of 32
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) acc[c + h + j] += __uint_as_float(v[h + j]) * y;
+                }
+              }
+            },
+            [&] {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(acc_empty + buf * 16u);
+              ready = mbar_test(acc_full + (buf ^ 1u) * 16u, (it >> 1) & 1u);   // the next block: its answer is there when the sums are done
+            });
+        if (i == kGroup - 1 || kb + 1 == num_kb) {   // this group's scales have been read
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&ctl->scales_empty[group & 1u]));
+          ++group;
         }
       }
       if (!ok) break;

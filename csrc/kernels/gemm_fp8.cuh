@@ -29,7 +29,7 @@ constexpr int kMmaK = 32;
 // A warp of its own brings the scales into shared memory, for this many blocks at a time and a group ahead: a promotion warp that fetched its
 // own spent more time on that than on its sums, and a plain load in flight holds up the thread's next arrival on a barrier (which
 // releases what came before it): with scales loaded a block ahead the persistent kernel took 1000 cycles a block.
-constexpr int kGroup = 4;
+constexpr int kGroup = 8;
 
 // Scales of one operand: element (row >> shift, block) with strides.
 struct Scales {
@@ -190,6 +190,7 @@ struct SmallPlan {
   int slices = 1;        // CTAs of a cluster that share a tile's K
   int kb_per_slice = 0;
   int tiles = 0;
+  bool deep = true;      // one CTA per SM with the whole shared memory as its ring, or two
 };
 bool plan_small(int M, int N, int K, int sms, SmallPlan* p, long* ns);
 cudaError_t launch_small(const void* a, int64_t lda, const void* b, int64_t ldb, const Args& g, const SmallPlan& p, cudaStream_t stream, std::string* why);

@@ -3,6 +3,10 @@
 // Operands are swapped: the 128 rows of the MMA are rows of B (a weight), its TN columns rows of A, so a tile of 16 tokens costs 2 KB of
 // shared memory a block instead of 16, and a column of the result is 128 consecutive elements of a row of C.  K is split over the CTAs of a
 // cluster where the tiles alone leave SMs idle; the slices meet in distributed shared memory and are added in slice order.  One tile per CTA.
+//
+// What bounds it is bytes in flight and handshakes.  A hand-over between the MMA warp and the promotion warps costs both about 300 cycles,
+// as much as the MMAs of a block themselves, so accumulators are handed over in units of up to four blocks (each block has its own columns), and
+// ring stages hold two blocks where tiles are narrow.
 #include <algorithm>
 
 #include "kernels/gemm_fp8.cuh"
@@ -14,20 +18,27 @@ namespace fp8 {
 namespace {
 
 template <int TN>
-constexpr int kStage = kTileBytes + TN * kBlockK;
+constexpr int kPerStage = TN <= 32 ? 2 : 1;       // blocks of K a ring stage holds: 128-row tiles of B, then TN-row tiles of A
+template <int TN>
+constexpr int kStage = kPerStage<TN> * (kTileBytes + TN * kBlockK);
+template <int TN>
+constexpr int kUnit = TN <= 16 ? 4 : 2;           // blocks that are handed over together
 template <int TN>
 constexpr int kWarps = TN >= 64 ? 8 : 4;          // promotion warps: one or two for each quarter of tensor memory's lanes
 template <int TN>
 constexpr int kCols = TN / (kWarps<TN> / 4);      // columns a promotion warp holds
 template <int TN>
-constexpr int kBuffers = TN >= 128 ? 2 : 4;       // accumulators
+constexpr int kBuffers = 2;                       // units in tensor memory
 template <int TN>
-constexpr int kSlot = kGroup * (32 + kCols<TN>);   // floats: a group's scales of a promotion warp
-constexpr int kMostStages = 12;
+constexpr int kSlot = kGroup * (128 + TN);         // floats: a group's scales
+template <int TN>
+constexpr int kThreads = 32 * (3 + kWarps<TN>);    // a producer, an MMA issuer, the promotion warps, one that brings their scales
+constexpr int kMostStages = 8;
 
 struct __align__(16) Ctl {
   uint64_t full[kMostStages], empty[kMostStages];
-  uint64_t acc_full[4], acc_empty[4];
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t scales_full[2], scales_empty[2];
   uint32_t tmem_base;
   volatile uint32_t abort;
 };
@@ -65,18 +76,20 @@ __device__ __forceinline__ float bias_of(const Args& g, int n) {
 }
 
 template <int TN, int NS>
-__global__ void __launch_bounds__(32 * (2 + kWarps<TN>))
+__global__ void __launch_bounds__(kThreads<TN>)
 gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x, const __grid_constant__ SmallArgs args) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int NB = kBuffers<TN>, W = kWarps<TN>, NC = kCols<TN>;
-  constexpr uint32_t kTmem = NB * TN;   // 64, 128, 256, 256 columns
+  constexpr int KPS = kPerStage<TN>, U = kUnit<TN>;
+  constexpr uint32_t kTmem = NB * U * TN;   // 128, 128, 256, 512 columns
+  static_assert(U % KPS == 0 && kGroup % U == 0, "a unit is whole stages, a group of scales whole units");
   static_assert(NS <= kMostStages && (NB & (NB - 1)) == 0, "ring depth");
   const Args& g = args.g;
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
   Ctl* ctl = reinterpret_cast<Ctl*>(smem + NS * kStage<TN>);
-  float* scales = reinterpret_cast<float*>(ctl + 1);   // [promotion warp][2][kSlot]
+  float* slots = reinterpret_cast<float*>(ctl + 1);   // [2][kGroup][128 rows of B], then [kGroup][TN rows of A], each
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slices = static_cast<int>(cluster_size());
@@ -86,13 +99,18 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   const int num_kb = (g.K + kBlockK - 1) / kBlockK;
   const int kb0 = slice * args.kb_per_slice;
   const int nkb = min(num_kb, kb0 + args.kb_per_slice) - kb0;   // at least 1: the plan leaves no slice empty
+  const int stages = (nkb + KPS - 1) / KPS;
 
   const bool leader = elect_one();
   auto load = [&](int i, uint32_t s) {
     const uint32_t full = smem_u32(&ctl->full[0]) + s * 8u, dst = base + s * kStage<TN>;
     mbar_arrive_expect_tx(full, kStage<TN>);
-    tma_load_2d(dst, &tma_w, full, (kb0 + i) * kBlockK, n0);
-    tma_load_2d(dst + kTileBytes, &tma_x, full, (kb0 + i) * kBlockK, m0);
+#pragma unroll
+    for (int p = 0; p < KPS; ++p) {   // (what lies beyond K is loaded as zeros)
+      const int k = (kb0 + i * KPS + p) * kBlockK;
+      tma_load_2d(dst + p * kTileBytes, &tma_w, full, k, n0);
+      tma_load_2d(dst + KPS * kTileBytes + p * (TN * kBlockK), &tma_x, full, k, m0);
+    }
   };
   if (warp == 0) {
     if (leader) {
@@ -106,12 +124,16 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
         mbar_init(smem_u32(&ctl->acc_full[b]), 1);
         mbar_init(smem_u32(&ctl->acc_empty[b]), W);
       }
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(smem_u32(&ctl->scales_full[b]), 32);
+        mbar_init(smem_u32(&ctl->scales_empty[b]), W);
+      }
       ctl->abort = 0;
       fence_barrier_init();
       fence_proxy_async();
     }
     __syncwarp();
-    for (int i = 0; i < NS && i < nkb; ++i)
+    for (int i = 0; i < NS && i < stages; ++i)
       if (leader) load(i, i);
   }
   __syncwarp();
@@ -127,6 +149,7 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   // promotion warps: warp's quarter of the lanes, its columns of the tile, this lane's row of B
   const int q = warp & 3, first_col = ((warp - 2) >> 2) * NC;
   const int n = n0 + q * 32 + lane;
+  const bool promoter = warp >= 2 && warp < 2 + W;
   float acc[NC];
 #pragma unroll
   for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
@@ -135,101 +158,119 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   if (warp == 0) {
     uint32_t s = 0, ph = 0;
     int i = NS;
-    for (; i < nkb; ++i) {
+    for (; i < stages; ++i) {
       if (!mbar_wait_warp(smem_u32(&ctl->empty[0]) + s * 8u, ph, &ctl->abort, g.wait_budget_ns)) break;
       if (leader) load(i, s);
       if (++s == NS) { s = 0; ph ^= 1u; }
     }
-    loads_land(&ctl->full[0], NS, static_cast<uint32_t>(min(i, nkb)), g.wait_budget_ns);
+    loads_land(&ctl->full[0], NS, static_cast<uint32_t>(min(i, stages)), g.wait_budget_ns);
   } else if (warp == 1) {
     constexpr uint32_t idesc = make_idesc_e4m3(128, TN);
-    const uint64_t dw0 = make_smem_desc_sw128(base), dx0 = make_smem_desc_sw128(base + kTileBytes);
-    uint32_t s = 0, ph = 0;
-    for (int i = 0; i < nkb; ++i) {
-      const uint32_t buf = static_cast<uint32_t>(i) % NB, acc_ph = (static_cast<uint32_t>(i) / NB) & 1u;
-      ok = mbar_wait_warp(smem_u32(&ctl->acc_empty[0]) + buf * 8u, acc_ph ^ 1u, &ctl->abort, g.wait_budget_ns);
+    const uint64_t dw0 = make_smem_desc_sw128(base), dx0 = make_smem_desc_sw128(base + KPS * kTileBytes);
+    uint32_t s = 0, ph = 0, unit = 0;
+    for (int i0 = 0; i0 < nkb && ok; i0 += U, ++unit) {
+      const uint32_t buf = unit & 1u;
+      ok = mbar_wait_warp(smem_u32(&ctl->acc_empty[0]) + buf * 8u, (unit >> 1 & 1u) ^ 1u, &ctl->abort, g.wait_budget_ns);
       if (!ok) break;
-      ok = mbar_wait_warp(smem_u32(&ctl->full[0]) + s * 8u, ph, &ctl->abort, g.wait_budget_ns);
-      if (!ok) break;
-      tc_fence_after_sync();
-      const uint64_t dw = dw0 + static_cast<uint64_t>(s * (kStage<TN> >> 4)), dx = dx0 + static_cast<uint64_t>(s * (kStage<TN> >> 4));
-      if (leader) {
 #pragma unroll
-        for (int k = 0; k < kBlockK / kMmaK; ++k)   // 32 bytes on inside a 128-byte swizzle row: +2 in the address field
-          umma_e4m3(tmem + buf * TN, dw + static_cast<uint64_t>(k * 2), dx + static_cast<uint64_t>(k * 2), idesc, k != 0 ? 1u : 0u);
-        umma_commit(smem_u32(&ctl->empty[0]) + s * 8u);
-        umma_commit(smem_u32(&ctl->acc_full[0]) + buf * 8u);
-      }
-      if (++s == NS) { s = 0; ph ^= 1u; }
-    }
-  } else {
-    // Brings the scales of the next group of blocks into slot `to`: this lane's row of B, the lane's share of the columns.
-    constexpr int kOwn = (NC + 31) / 32;
-    const float* row_scale = g.b.at(min(n, g.N - 1)) + kb0 * g.b.blk;
-    const float* col_scale[kOwn];
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j) col_scale[j] = g.a.at(min(m0 + first_col + lane + j * 32, g.M - 1)) + kb0 * g.a.blk;
-    float* slots = scales + (warp - 2) * 2 * kSlot<TN>;
-    int ahead = 0;
-    const auto fetch = [&](uint32_t to) {
-      float* slot = slots + to * kSlot<TN>;
-#pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        if (ahead + i >= nkb) break;
-        copy4_async(slot + i * 32 + lane, row_scale);
-        row_scale += g.b.blk;
-#pragma unroll
-        for (int j = 0; j < kOwn; ++j) {
-          if (lane + j * 32 < NC) copy4_async(slot + kGroup * 32 + i * NC + lane + j * 32, col_scale[j]);
-          col_scale[j] += g.a.blk;
-        }
-      }
-      ahead += kGroup;
-    };
-    fetch(0);
-    const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + first_col;
-    uint32_t group = 0;
-    for (int i0 = 0; i0 < nkb && ok; i0 += kGroup, group ^= 1u) {
-      copies_wait();
-      __syncwarp();   // this group's scales are there, the other slot's have been read
-      const float* rows = slots + group * kSlot<TN>;
-      const float* cols = rows + kGroup * 32;
-      float x[kGroup];
-#pragma unroll
-      for (int i = 0; i < kGroup; ++i) x[i] = rows[i * 32 + lane];
-      fetch(group ^ 1u);
-#pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        if (i0 + i >= nkb) break;
-        const uint32_t buf = static_cast<uint32_t>(i0 + i) % NB, acc_ph = (static_cast<uint32_t>(i0 + i) / NB) & 1u;
-        ok = mbar_wait_warp(smem_u32(&ctl->acc_full[0]) + buf * 8u, acc_ph, &ctl->abort, g.wait_budget_ns);
+      for (int st = 0; st < U; st += KPS) {
+        if (i0 + st >= nkb) break;
+        ok = mbar_wait_warp(smem_u32(&ctl->full[0]) + s * 8u, ph, &ctl->abort, g.wait_budget_ns);
         if (!ok) break;
         tc_fence_after_sync();
-        promote<NC, 32>(
-            taddr + buf * TN,
-            [&](int c, const auto& v) {
+        const uint64_t dw = dw0 + static_cast<uint64_t>(s * (kStage<TN> >> 4)), dx = dx0 + static_cast<uint64_t>(s * (kStage<TN> >> 4));
+        if (leader) {
 #pragma unroll
-              for (int j = 0; j < static_cast<int>(sizeof(v) / 4); j += 4) {
-                const float4 s = *reinterpret_cast<const float4*>(cols + i * NC + c + j);
-                acc[c + j] += __uint_as_float(v[j]) * x[i] * s.x;
-                acc[c + j + 1] += __uint_as_float(v[j + 1]) * x[i] * s.y;
-                acc[c + j + 2] += __uint_as_float(v[j + 2]) * x[i] * s.z;
-                acc[c + j + 3] += __uint_as_float(v[j + 3]) * x[i] * s.w;
-              }
-            },
-            [&] {
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(smem_u32(&ctl->acc_empty[0]) + buf * 8u);
-            });
+          for (int p = 0; p < KPS; ++p) {
+            if (p != 0 && i0 + st + p >= nkb) break;
+#pragma unroll
+            for (int k = 0; k < kBlockK / kMmaK; ++k)   // 32 bytes on inside a 128-byte swizzle row: +2 in the address field
+              umma_e4m3(tmem + buf * (U * TN) + (st + p) * TN, dw + static_cast<uint64_t>(p * (kTileBytes >> 4) + k * 2),
+                        dx + static_cast<uint64_t>(p * (TN * kBlockK >> 4) + k * 2), idesc, k != 0 ? 1u : 0u);
+          }
+          umma_commit(smem_u32(&ctl->empty[0]) + s * 8u);
+        }
+        if (++s == NS) { s = 0; ph ^= 1u; }
       }
+      if (ok && leader) umma_commit(smem_u32(&ctl->acc_full[0]) + buf * 8u);
+    }
+  } else if (warp == 2 + W) {
+    const float *rows[4], *cols[(TN + 31) / 32];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) rows[j] = g.b.at(min(n0 + lane + j * 32, g.N - 1)) + kb0 * g.b.blk;
+#pragma unroll
+    for (int j = 0; j < (TN + 31) / 32; ++j) cols[j] = g.a.at(min(m0 + lane + j * 32, g.M - 1)) + kb0 * g.a.blk;
+    uint32_t group = 0;
+    for (int i0 = 0; i0 < nkb; i0 += kGroup, ++group) {
+      if (!mbar_wait_warp(smem_u32(&ctl->scales_empty[group & 1u]), (group >> 1 & 1u) ^ 1u, &ctl->abort, g.wait_budget_ns)) break;
+      float* slot = slots + (group & 1u) * kSlot<TN>;
+      for (int i = 0; i < kGroup && i0 + i < nkb; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          copy4_async(slot + i * 128 + lane + j * 32, rows[j]);
+          rows[j] += g.b.blk;
+        }
+#pragma unroll
+        for (int j = 0; j < (TN + 31) / 32; ++j) {
+          if (lane + j * 32 < TN) copy4_async(slot + kGroup * 128 + i * TN + lane + j * 32, cols[j]);
+          cols[j] += g.a.blk;
+        }
+      }
+      copies_arrive(smem_u32(&ctl->scales_full[group & 1u]));
     }
     copies_wait();
+  } else {
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + first_col;
+    const uint32_t acc_full = smem_u32(&ctl->acc_full[0]), acc_empty = smem_u32(&ctl->acc_empty[0]);
+    uint32_t group = 0;
+    uint32_t unit = 0;
+    bool ready = false;
+#pragma unroll 1
+    for (int i0 = 0; i0 < nkb; i0 += U, ++unit) {
+      if (i0 % kGroup == 0) {
+        ok = mbar_wait_warp(smem_u32(&ctl->scales_full[group & 1u]), group >> 1 & 1u, &ctl->abort, g.wait_budget_ns);
+        if (!ok) break;
+      }
+      const float* slot = slots + (group & 1u) * kSlot<TN>;
+      const uint32_t buf = unit & 1u;
+      ok = __all_sync(0xffffffffu, ready) || mbar_wait_warp(acc_full + buf * 8u, unit >> 1 & 1u, &ctl->abort, g.wait_budget_ns);
+      if (!ok) break;
+      tc_fence_after_sync();
+      const int blocks = min(U, nkb - i0);
+#pragma unroll
+      for (int p = 0; p < U; ++p) {
+        if (p >= blocks) break;
+        const int in = i0 % kGroup + p;
+        const float* cols = slot + kGroup * 128 + in * TN + first_col;
+        const float r = slot[in * 128 + q * 32 + lane];
+        uint32_t v[NC];
+        tmem_read(taddr + buf * (U * TN) + p * TN, v);
+        if (p == blocks - 1) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty + buf * 8u);
+          ready = mbar_test(acc_full + (buf ^ 1u) * 8u, (unit + 1u) >> 1 & 1u);   // the next unit: its answer is there when the sums are done
+        }
+#pragma unroll
+        for (int j = 0; j < NC; j += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(cols + j);
+          acc[j] += __uint_as_float(v[j]) * r * s.x;
+          acc[j + 1] += __uint_as_float(v[j + 1]) * r * s.y;
+          acc[j + 2] += __uint_as_float(v[j + 2]) * r * s.z;
+          acc[j + 3] += __uint_as_float(v[j + 3]) * r * s.w;
+        }
+      }
+      if ((i0 + U) % kGroup == 0 || i0 + U >= nkb) {   // this group's scales have been read
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl->scales_empty[group & 1u]));
+        ++group;
+      }
+    }
   }
   __syncwarp();
 
   if (slices == 1) {
-    if (warp >= 2 && ok) {
+    if (promoter && ok) {
       const float bias = bias_of(g, n);
 #pragma unroll
       for (int j = 0; j < NC; ++j) store(g, m0 + first_col + j, n, acc[j] + bias);
@@ -239,7 +280,7 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
     cluster_sync_all();
     const int own = TN / slices, own_log2 = 31 - __clz(own);   // columns this slice finishes (a power of two)
     float* recv = reinterpret_cast<float*>(smem);               // [source slice][own columns][128 rows]
-    if (warp >= 2 && ok) {
+    if (promoter && ok) {
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
         const int col = first_col + j;
@@ -248,7 +289,7 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
       }
     }
     cluster_sync_all();
-    if (warp >= 2 && ok) {
+    if (promoter && ok) {
       const float bias = bias_of(g, n);
       for (int c = (warp - 2) >> 2; c < own; c += W / 4) {
         const int m = m0 + slice * own + c;
@@ -271,7 +312,7 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
 template <int TN, int NS>
 cudaError_t fire(const CUtensorMap& tw, const CUtensorMap& tx, const SmallArgs& a, const SmallPlan& p, cudaStream_t stream) {
   auto kernel = gemm_fp8_small_kernel<TN, NS>;
-  constexpr int smem_bytes = NS * kStage<TN> + 1024 /*alignment slack*/ + static_cast<int>(sizeof(Ctl)) + kWarps<TN> * 2 * kSlot<TN> * 4;
+  constexpr int smem_bytes = NS * kStage<TN> + 1024 /*alignment slack*/ + static_cast<int>(sizeof(Ctl)) + 2 * kSlot<TN> * 4;
   static_assert(smem_bytes <= 227 * 1024, "shared memory");
   static_assert(TN * 128 * 4 <= NS * kStage<TN>, "the slices' partial sums fit the ring");
   static bool configured[kMaxDevices] = {};
@@ -283,7 +324,7 @@ cudaError_t fire(const CUtensorMap& tw, const CUtensorMap& tx, const SmallArgs& 
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.tiles) * p.slices);
-  cfg.blockDim = dim3(32 * (2 + kWarps<TN>));
+  cfg.blockDim = dim3(kThreads<TN>);
   cfg.dynamicSmemBytes = smem_bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -298,6 +339,12 @@ cudaError_t fire(const CUtensorMap& tw, const CUtensorMap& tx, const SmallArgs& 
 
 }  // namespace
 
+// Blocks of K a slice takes: whole ring stages.
+int per_slice(int num_kb, int slices, int tn) {
+  const int per_stage = tn <= 32 ? 2 : 1, stages = (num_kb + per_stage - 1) / per_stage;
+  return (stages + slices - 1) / slices * per_stage;
+}
+
 // Fewest CTAs' worth of K while SMs are idle: slices are doubled as long as all CTAs still run at once.
 bool plan_small(int M, int N, int K, int sms, SmallPlan* p, long* ns) {
   const int num_kb = (K + kBlockK - 1) / kBlockK;
@@ -308,10 +355,10 @@ bool plan_small(int M, int N, int K, int sms, SmallPlan* p, long* ns) {
   p->tiles = static_cast<int>(tiles);
   p->slices = 1;
   while (p->slices < 8 && tiles * p->slices * 2 <= sms && num_kb >= p->slices * 4) p->slices *= 2;
-  p->kb_per_slice = (num_kb + p->slices - 1) / p->slices;
+  p->kb_per_slice = per_slice(num_kb, p->slices, p->tn);
   while ((p->slices - 1) * p->kb_per_slice >= num_kb) {   // a slice would be empty
     p->slices /= 2;
-    p->kb_per_slice = (num_kb + p->slices - 1) / p->slices;
+    p->kb_per_slice = per_slice(num_kb, p->slices, p->tn);
   }
   *ns = 5000 + ((tiles * p->slices + sms - 1) / sms) * p->kb_per_slice * (p->tn == 128 ? 300 : 200);
   return true;
@@ -321,10 +368,11 @@ cudaError_t launch_small(const void* a, int64_t lda, const void* b, int64_t ldb,
   CUtensorMap tw, tx;
   if (!make_tensor_map_e4m3(&tw, b, g.N, g.K, ldb, 128, why) || !make_tensor_map_e4m3(&tx, a, g.M, g.K, lda, p.tn, why)) return cudaErrorInvalidValue;
   const SmallArgs s{g, (g.N + 127) / 128, p.kb_per_slice};
+  // ring depths: all of an SM's shared memory, or half of it
   switch (p.tn) {
-    case 16: return fire<16, 10>(tw, tx, s, p, stream);
-    case 32: return fire<32, 10>(tw, tx, s, p, stream);
-    case 64: return fire<64, 8>(tw, tx, s, p, stream);
+    case 16: return p.deep ? fire<16, 5>(tw, tx, s, p, stream) : fire<16, 2>(tw, tx, s, p, stream);
+    case 32: return p.deep ? fire<32, 5>(tw, tx, s, p, stream) : fire<32, 2>(tw, tx, s, p, stream);
+    case 64: return p.deep ? fire<64, 8>(tw, tx, s, p, stream) : fire<64, 4>(tw, tx, s, p, stream);
     case 128: return fire<128, 6>(tw, tx, s, p, stream);
   }
   return cudaErrorInvalidValue;
