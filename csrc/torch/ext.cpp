@@ -13,6 +13,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -20,7 +21,10 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <optional>
+
 #include "mini_nccl_api.h"
+#include "mini_nccl_ops.h"
 
 namespace {
 
@@ -32,6 +36,10 @@ struct Library {
                  const void*, size_t, cudaStream_t) = nullptr;
   int (*ag_gemm)(void* const*, const void*, void*, int, int, int, int, int, int, int, int, void* const*, void* const*, uint32_t*, int,
                  int, const void*, size_t, cudaStream_t) = nullptr;
+  decltype(&mncclQuantizeFp8) quantize_fp8 = nullptr;
+  decltype(&mncclGemmFp8) gemm_fp8 = nullptr;
+  decltype(&mncclDistillForward) distill_forward = nullptr;
+  decltype(&mncclDistillBackward) distill_backward = nullptr;
 } lib;
 
 // ncclDataType_t of a tensor's scalar type, -1 for a type the library does not have.
@@ -86,15 +94,19 @@ bool arg_count(Py_ssize_t n, Py_ssize_t want) {
   return n == want;
 }
 
-// bind(all_reduce_ex, async_error, gemm, gemm_rs, ag_gemm): addresses in the library that ctypes has loaded (the
-// last three may be 0)
+// bind(all_reduce_ex, async_error, gemm, gemm_rs, ag_gemm, quantize_fp8, gemm_fp8, distill_forward, distill_backward): addresses
+// in the library that ctypes has loaded (all but the first two may be 0)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (!arg_count(n, 5)) return nullptr;
+  if (!arg_count(n, 9)) return nullptr;
   lib.all_reduce_ex = reinterpret_cast<decltype(lib.all_reduce_ex)>(PyLong_AsVoidPtr(args[0]));
   lib.async_error = reinterpret_cast<decltype(lib.async_error)>(PyLong_AsVoidPtr(args[1]));
   lib.gemm = reinterpret_cast<decltype(lib.gemm)>(PyLong_AsVoidPtr(args[2]));
   lib.gemm_rs = reinterpret_cast<decltype(lib.gemm_rs)>(PyLong_AsVoidPtr(args[3]));
   lib.ag_gemm = reinterpret_cast<decltype(lib.ag_gemm)>(PyLong_AsVoidPtr(args[4]));
+  lib.quantize_fp8 = reinterpret_cast<decltype(lib.quantize_fp8)>(PyLong_AsVoidPtr(args[5]));
+  lib.gemm_fp8 = reinterpret_cast<decltype(lib.gemm_fp8)>(PyLong_AsVoidPtr(args[6]));
+  lib.distill_forward = reinterpret_cast<decltype(lib.distill_forward)>(PyLong_AsVoidPtr(args[7]));
+  lib.distill_backward = reinterpret_cast<decltype(lib.distill_backward)>(PyLong_AsVoidPtr(args[8]));
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -308,6 +320,254 @@ PyObject* ag_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- 8-bit operators and distillation (ops/fp8.py, ops/distill.py).  They run on their tensors' GPU, whichever is current, and on the given
+// stream or that GPU's current one; what they allocate belongs to that stream.
+
+constexpr int64_t kBlock = 128, kMost = 2147483647 - 65536;
+int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
+int64_t padded(int64_t n) { return (n + 15) / 16 * 16; }
+
+struct On {
+  c10::cuda::OptionalCUDAGuard device;
+  c10::cuda::OptionalCUDAStreamGuard stream;
+  cudaStream_t raw = nullptr;
+};
+bool on(const at::Tensor& t, PyObject* stream, On* o) {
+  if (stream == Py_None) {
+    o->device.set_index(t.get_device());
+    o->raw = c10::cuda::getCurrentCUDAStream().stream();
+    return true;
+  }
+  int64_t v[3];
+  const char* names[3] = {"stream_id", "device_index", "device_type"};
+  for (int i = 0; i < 3; ++i) {
+    PyObject* x = PyObject_GetAttrString(stream, names[i]);
+    if (!x) return false;
+    v[i] = PyLong_AsLongLong(x);
+    Py_DECREF(x);
+    if (PyErr_Occurred()) return false;
+  }
+  if (v[1] != t.get_device()) {
+    PyErr_Format(PyExc_ValueError, "the stream is on cuda:%lld, the tensors are on cuda:%d", static_cast<long long>(v[1]), static_cast<int>(t.get_device()));
+    return false;
+  }
+  o->stream.reset_stream(c10::Stream::unpack3(v[0], static_cast<c10::DeviceIndex>(v[1]), static_cast<c10::DeviceType>(v[2])));
+  o->raw = c10::cuda::getCurrentCUDAStream().stream();
+  return true;
+}
+
+// fp16, fp32 and bf16, by the library's codes; -1 for another type
+int float_code(const at::Tensor& t) {
+  const int c = type_code(t.scalar_type());
+  return c == ncclFloat16 || c == ncclFloat || c == ncclBfloat16 ? c : -1;
+}
+
+// Whether `t` is a matrix the kernels can read, and its row stride.
+bool matrix(const at::Tensor& t, const char* name, bool right_type, int64_t* ld) {
+  if (!t.is_cuda()) {
+    PyErr_Format(PyExc_TypeError, "%s must be a CUDA tensor", name);
+  } else if (!right_type) {
+    PyErr_Format(PyExc_TypeError, "%s is of a type that this call does not take: %s", name, c10::toString(t.scalar_type()));
+  } else if (t.dim() != 2 || t.size(0) > kMost || t.size(1) > kMost) {
+    PyErr_Format(PyExc_ValueError, "%s must be a matrix of at most %lld rows and columns", name, static_cast<long long>(kMost));
+  } else if (t.size(1) > 1 && t.stride(1) != 1) {
+    PyErr_Format(PyExc_ValueError, "%s needs a unit inner stride", name);
+  } else {
+    *ld = t.size(0) > 1 ? t.stride(0) : padded(t.size(1));
+    if (*ld >= t.size(1)) return true;
+    PyErr_Format(PyExc_ValueError, "%s's rows overlap", name);
+  }
+  return false;
+}
+
+PyObject* failed(const char* what, int rc) {
+  PyErr_Format(PyExc_RuntimeError, "%s failed with code %d", what, rc);
+  return nullptr;
+}
+PyObject* wrap(const at::Tensor& t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); }
+
+// quantize_fp8(x, block_rows, transposed, stream | None) -> (q, scale, qt | None, scale_t | None) as the kernels write them: rows padded
+// to 16 bytes, scales [K blocks, M] (block_rows 1) or [M blocks, K blocks]
+PyObject* quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 4)) return nullptr;
+  const at::Tensor* x = tensor_arg(args[0], "x");
+  if (!x) return nullptr;
+  const long block_rows = PyLong_AsLong(args[1]);
+  const int transposed = PyObject_IsTrue(args[2]);
+  if (transposed < 0 || PyErr_Occurred()) return nullptr;
+  const int code = float_code(*x);
+  int64_t ld = 0;
+  if (!matrix(*x, "x", code >= 0, &ld)) return nullptr;
+  if (block_rows != 1 && block_rows != kBlock) {
+    PyErr_SetString(PyExc_ValueError, "block_rows must be 1 or 128");
+    return nullptr;
+  }
+  On o;
+  if (!on(*x, args[3], &o)) return nullptr;
+  const int64_t M = x->size(0), K = x->size(1);
+  const auto e4m3 = x->options().dtype(at::kFloat8_e4m3fn).requires_grad(false), f32 = x->options().dtype(at::kFloat).requires_grad(false);
+  const bool row = block_rows == 1;
+  at::Tensor q = at::empty({M, padded(K)}, e4m3), scale = at::empty(row ? at::IntArrayRef{blocks(K), M} : at::IntArrayRef{blocks(M), blocks(K)}, f32), qt, scale_t;
+  if (transposed) {
+    qt = at::empty({K, padded(M)}, e4m3);
+    if (row) scale_t = at::empty({blocks(M), K}, f32);
+  }
+  int rc = 0;
+  if (M > 0 && K > 0) {
+    Py_BEGIN_ALLOW_THREADS
+    rc = lib.quantize_fp8(x->data_ptr(), code, ld, static_cast<int>(M), static_cast<int>(K), static_cast<int>(block_rows), q.data_ptr(), q.size(1),
+                          scale.data_ptr<float>(), transposed ? qt.data_ptr() : nullptr, transposed ? qt.size(1) : 0,
+                          scale_t.defined() ? scale_t.data_ptr<float>() : nullptr, o.raw);
+    Py_END_ALLOW_THREADS
+  }
+  if (rc != 0) return failed("mncclQuantizeFp8", rc);
+  return Py_BuildValue("(NNNN)", wrap(q), wrap(scale), wrap(qt), wrap(scale_t));
+  END_HANDLE_TH_ERRORS
+}
+
+bool operand(const at::Tensor& t, const char* name, int64_t* ld) {
+  if (!matrix(t, name, t.scalar_type() == at::kFloat8_e4m3fn, ld)) return false;
+  if (t.numel() == 0 || (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && *ld % 16 == 0)) return true;
+  PyErr_Format(PyExc_ValueError, "%s's rows must start on 16 bytes (quantize_fp8 lays them out so)", name);
+  return false;
+}
+// Whether `t` holds the scales of an operand [rows, K]; *per: rows of a scale.
+bool scales(const at::Tensor& t, const char* name, int64_t rows, int64_t K, const at::Tensor& like, int* per) {
+  if (t.scalar_type() != at::kFloat || t.device() != like.device()) {
+    PyErr_Format(PyExc_TypeError, "%s must be an fp32 tensor on the operands' GPU", name);
+    return false;
+  }
+  if (t.dim() != 2 || t.size(1) != blocks(K) || (t.size(0) != rows && t.size(0) != blocks(rows))) {
+    PyErr_Format(PyExc_ValueError, "%s must be [%lld or %lld, %lld]", name, static_cast<long long>(rows), static_cast<long long>(blocks(rows)),
+                 static_cast<long long>(blocks(K)));
+    return false;
+  }
+  *per = t.size(0) == rows ? 1 : static_cast<int>(kBlock);
+  return true;
+}
+
+// gemm_fp8(a, a_scale, b, b_scale, out | None, out_dtype | None, bias | None, stream | None) -> out; see ops/fp8.py
+PyObject* gemm_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 8)) return nullptr;
+  const at::Tensor *a = tensor_arg(args[0], "a"), *sa = a ? tensor_arg(args[1], "a_scale") : nullptr, *b = sa ? tensor_arg(args[2], "b") : nullptr,
+                   *sb = b ? tensor_arg(args[3], "b_scale") : nullptr;
+  if (!sb) return nullptr;
+  int64_t lda = 0, ldb = 0, ldc = 0;
+  if (!operand(*a, "a", &lda) || !operand(*b, "b", &ldb)) return nullptr;
+  const int64_t M = a->size(0), K = a->size(1), N = b->size(0);
+  if (b->size(1) != K || b->device() != a->device()) {
+    PyErr_SetString(PyExc_ValueError, "shapes: a [M, K], b [N, K], on one GPU");
+    return nullptr;
+  }
+  int pa = 1, pb = 1;
+  if (!scales(*sa, "a_scale", M, K, *a, &pa) || !scales(*sb, "b_scale", N, K, *a, &pb)) return nullptr;
+  std::optional<at::ScalarType> type;
+  if (args[5] != Py_None) {
+    if (!THPDtype_Check(args[5])) {
+      PyErr_SetString(PyExc_TypeError, "out_dtype must be a torch dtype");
+      return nullptr;
+    }
+    type = reinterpret_cast<THPDtype*>(args[5])->scalar_type;
+  }
+  On o;
+  if (!on(*a, args[7], &o)) return nullptr;
+  at::Tensor fresh;
+  const at::Tensor* out = nullptr;
+  if (args[4] != Py_None) {
+    out = tensor_arg(args[4], "out");
+    if (!out) return nullptr;
+    if (type && *type != out->scalar_type()) {
+      PyErr_SetString(PyExc_ValueError, "out has another type than out_dtype");
+      return nullptr;
+    }
+  } else {
+    fresh = at::empty({M, N}, a->options().dtype(type.value_or(at::kBFloat16)).requires_grad(false));
+    out = &fresh;
+  }
+  const int code = float_code(*out);
+  if (out->dim() != 2 || out->size(0) != M || out->size(1) != N || out->device() != a->device()) {
+    PyErr_SetString(PyExc_ValueError, "out must be [M, N] on the operands' GPU");
+    return nullptr;
+  }
+  if (!matrix(*out, "out", code >= 0, &ldc)) return nullptr;
+  const at::Tensor* bias = nullptr;
+  if (args[6] != Py_None) {
+    bias = tensor_arg(args[6], "bias");
+    if (!bias) return nullptr;
+    if (bias->scalar_type() != out->scalar_type() || bias->device() != a->device() || bias->dim() != 1 || bias->size(0) != N || (N > 1 && bias->stride(0) != 1)) {
+      PyErr_SetString(PyExc_ValueError, "bias must be [N], dense, of out's type and on its GPU");
+      return nullptr;
+    }
+  }
+  if (K == 0) {
+    c10::AutoGradMode no_grad(false);
+    if (bias) out->copy_(bias->expand({M, N}));
+    else out->zero_();
+  } else if (M > 0 && N > 0) {
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = lib.gemm_fp8(a->data_ptr(), lda, sa->data_ptr<float>(), sa->stride(0), sa->stride(1), pa, b->data_ptr(), ldb, sb->data_ptr<float>(), sb->stride(0),
+                      sb->stride(1), pb, out->data_ptr(), ldc, code, bias ? bias->data_ptr() : nullptr, static_cast<int>(M), static_cast<int>(N),
+                      static_cast<int>(K), o.raw);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return failed("mncclGemmFp8", rc);
+  }
+  return fresh.defined() ? THPVariable_Wrap(fresh) : Py_NewRef(args[4]);
+  END_HANDLE_TH_ERRORS
+}
+
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)); }
+
+// distill_forward(rows, ids, top, tau) -> (p, stats, counts, row_loss, mean); ops/distill.py has checked the arguments
+PyObject* distill_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 4)) return nullptr;
+  const at::Tensor *rows = tensor_arg(args[0], "rows"), *ids = rows ? tensor_arg(args[1], "ids") : nullptr, *top = ids ? tensor_arg(args[2], "top") : nullptr;
+  if (!top) return nullptr;
+  const double tau = PyFloat_AsDouble(args[3]);
+  if (PyErr_Occurred()) return nullptr;
+  On o;
+  if (!on(*rows, Py_None, &o)) return nullptr;
+  const int64_t T = rows->size(0), K = ids->size(1);
+  const auto f32 = rows->options().dtype(at::kFloat).requires_grad(false);
+  at::Tensor p = at::empty({T, K}, f32), stats = at::empty({T, 2}, f32), counts = at::empty({T}, f32.dtype(at::kInt)), row_loss = at::empty({T}, f32), mean = at::empty({3}, f32);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = lib.distill_forward(rows->data_ptr(), float_code(*rows), row_stride(*rows), static_cast<int>(T), static_cast<int>(rows->size(1)), ids->data_ptr<int64_t>(),
+                           top->data_ptr<float>(), static_cast<int>(K), static_cast<float>(tau), p.data_ptr<float>(), stats.data_ptr<float>(), row_loss.data_ptr<float>(),
+                           counts.data_ptr<int>(), mean.data_ptr<float>(), o.raw);
+  Py_END_ALLOW_THREADS
+  if (rc != 0) return failed("mncclDistillForward", rc);
+  return Py_BuildValue("(NNNNN)", wrap(p), wrap(stats), wrap(counts), wrap(row_loss), wrap(mean));
+  END_HANDLE_TH_ERRORS
+}
+
+// distill_backward(rows, ids, p, stats, counts, tokens | None, tau, grad, d); tokens: what the gradient is divided by
+PyObject* distill_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 9)) return nullptr;
+  const at::Tensor* t[9] = {};
+  for (int i = 0; i < 9; ++i) {
+    if (i == 6 || (i == 5 && args[i] == Py_None)) continue;
+    if (!(t[i] = tensor_arg(args[i], "argument"))) return nullptr;
+  }
+  const double tau = PyFloat_AsDouble(args[6]);
+  if (PyErr_Occurred()) return nullptr;
+  On o;
+  if (!on(*t[0], Py_None, &o)) return nullptr;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = lib.distill_backward(t[0]->data_ptr(), float_code(*t[0]), row_stride(*t[0]), static_cast<int>(t[0]->size(0)), static_cast<int>(t[0]->size(1)), t[1]->data_ptr<int64_t>(),
+                            t[2]->data_ptr<float>(), static_cast<int>(t[1]->size(1)), static_cast<float>(tau), t[3]->data_ptr<float>(), t[4]->data_ptr<int>(),
+                            t[7]->data_ptr<float>(), t[7]->dim() > 0 ? 1 : 0, t[5] ? t[5]->data_ptr<float>() : nullptr, t[8]->data_ptr(), row_stride(*t[8]), o.raw);
+  Py_END_ALLOW_THREADS
+  if (rc != 0) return failed("mncclDistillBackward", rc);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // async_error(comm) -> ncclResult_t
 PyObject* async_error(PyObject*, PyObject* comm) {
   const int e = comm_error(comm);
@@ -320,6 +580,10 @@ PyMethodDef methods[] = {
     {"gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gemm)), METH_FASTCALL, nullptr},
     {"gemm_rs", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gemm_rs)), METH_FASTCALL, nullptr},
     {"ag_gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(ag_gemm)), METH_FASTCALL, nullptr},
+    {"quantize_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(quantize_fp8)), METH_FASTCALL, nullptr},
+    {"gemm_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gemm_fp8)), METH_FASTCALL, nullptr},
+    {"distill_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(distill_forward)), METH_FASTCALL, nullptr},
+    {"distill_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(distill_backward)), METH_FASTCALL, nullptr},
     {"async_error", async_error, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

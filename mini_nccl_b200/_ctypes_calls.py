@@ -121,11 +121,150 @@ def ag_gemm(lib, comm, n_comm_ctas, b, out, stream, swiglu, workspace):
     return out
 
 
+# ---- 8-bit operators and distillation
+
+_BLOCK = 128
+_E4M3 = torch.float8_e4m3fn
+_FLOATS = {torch.float16: 6, torch.float32: 7, torch.bfloat16: 9}
+_MOST = 2**31 - 1 - 2**16   # rows and columns of a matrix: indices are 32-bit, elements are addressed with 64
+
+
+def _blocks(n):
+    return -(-n // _BLOCK)
+
+
+def _padded(n):
+    return -(-n // 16) * 16
+
+
+def _check(rc, what):
+    if rc != 0:
+        raise RuntimeError(f"{what} failed with code {rc}")
+
+
+class _on:
+    """The GPU and the stream that a call runs on: the tensors' GPU, and `stream` or that GPU's current one.  What is
+    allocated inside belongs to that stream."""
+
+    def __init__(self, device, stream):
+        if stream is not None and stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the tensors are on {device}")
+        self.with_ = [torch.cuda.device(device)] if stream is None else [torch.cuda.device(device), torch.cuda.stream(stream)]
+
+    def __enter__(self):
+        for w in self.with_:
+            w.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *what):
+        for w in reversed(self.with_):
+            w.__exit__(*what)
+
+
+def _matrix(t, name, dtypes):
+    """(rows, columns, row stride) of a matrix the kernels can read."""
+    if not _tensor(t, name).is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} is of a type that this call does not take: {t.dtype}")
+    if t.dim() != 2 or max(t.shape) > _MOST:
+        raise ValueError(f"{name} must be a matrix of at most {_MOST} rows and columns")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} needs a unit inner stride")
+    ld = t.stride(0) if rows > 1 else _padded(cols)
+    if ld < cols:
+        raise ValueError(f"{name}'s rows overlap")
+    return rows, cols, ld
+
+
+def quantize_fp8(lib, x, block_rows, transposed, stream):
+    M, K, ld = _matrix(x, "x", _FLOATS)
+    if block_rows not in (1, _BLOCK):
+        raise ValueError("block_rows must be 1 or 128")
+    with _on(x.device, stream) as s:
+        q = torch.empty((M, _padded(K)), dtype=_E4M3, device=x.device)
+        scale = torch.empty((_blocks(K), M) if block_rows == 1 else (_blocks(M), _blocks(K)), dtype=torch.float32, device=x.device)
+        qt = torch.empty((K, _padded(M)), dtype=_E4M3, device=x.device) if transposed else None
+        scale_t = torch.empty((_blocks(M), K), dtype=torch.float32, device=x.device) if transposed and block_rows == 1 else None
+        if M and K:
+            _check(lib.mncclQuantizeFp8(x.data_ptr(), _FLOATS[x.dtype], ld, M, K, block_rows, q.data_ptr(), q.shape[1], scale.data_ptr(),
+                                        qt.data_ptr() if transposed else None, qt.shape[1] if transposed else 0,
+                                        scale_t.data_ptr() if scale_t is not None else None, s), "mncclQuantizeFp8")
+    return q, scale, qt, scale_t
+
+
+def _operand(t, name):
+    rows, cols, ld = _matrix(t, name, (_E4M3,))
+    if t.numel() and (t.data_ptr() % 16 or ld % 16):
+        raise ValueError(f"{name}'s rows must start on 16 bytes (quantize_fp8 lays them out so)")
+    return rows, cols, ld
+
+
+def _scales(t, name, rows, K, device):
+    """(row stride, block stride, rows of a scale) of the scales of an operand [rows, K]."""
+    if _tensor(t, name).dtype != torch.float32 or t.device != device:
+        raise TypeError(f"{name} must be an fp32 tensor on the operands' GPU")
+    if t.dim() != 2 or t.shape[1] != _blocks(K) or t.shape[0] not in (rows, _blocks(rows)):
+        raise ValueError(f"{name} must be [{rows} or {_blocks(rows)}, {_blocks(K)}]")
+    return t.stride(0), t.stride(1), 1 if t.shape[0] == rows else _BLOCK
+
+
+def gemm_fp8(lib, a, a_scale, b, b_scale, out, out_dtype, bias, stream):
+    M, K, lda = _operand(a, "a")
+    N, Kb, ldb = _operand(b, "b")
+    if K != Kb or b.device != a.device:
+        raise ValueError("shapes: a [M, K], b [N, K], on one GPU")
+    sa = _scales(a_scale, "a_scale", M, K, a.device)
+    sb = _scales(b_scale, "b_scale", N, K, a.device)
+    if out_dtype is not None and not isinstance(out_dtype, torch.dtype):
+        raise TypeError("out_dtype must be a torch dtype")
+    with _on(a.device, stream) as s:
+        if out is None:
+            out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=a.device)
+        elif out_dtype not in (None, _tensor(out, "out").dtype):
+            raise ValueError("out has another type than out_dtype")
+        if tuple(out.shape) != (M, N) or out.device != a.device:
+            raise ValueError("out must be [M, N] on the operands' GPU")
+        ldc = _matrix(out, "out", _FLOATS)[2]
+        if bias is not None and (_tensor(bias, "bias").dtype != out.dtype or bias.device != a.device or tuple(bias.shape) != (N,)
+                                 or (N > 1 and bias.stride(0) != 1)):
+            raise ValueError("bias must be [N], dense, of out's type and on its GPU")
+        if K == 0:
+            with torch.no_grad():
+                return out.zero_() if bias is None else out.copy_(bias.expand(M, N))
+        if M and N:
+            _check(lib.mncclGemmFp8(a.data_ptr(), lda, a_scale.data_ptr(), *sa, b.data_ptr(), ldb, b_scale.data_ptr(), *sb, out.data_ptr(), ldc,
+                                    _FLOATS[out.dtype], bias.data_ptr() if bias is not None else None, M, N, K, s), "mncclGemmFp8")
+    return out
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def distill_forward(lib, rows, ids, top, tau):
+    (T, V), K = rows.shape, ids.shape[1]
+    with _on(rows.device, None) as s:
+        empty = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=rows.device)  # noqa: E731
+        p, stats, counts, row_loss, mean = empty(T, K), empty(T, 2), empty(T, dtype=torch.int32), empty(T), empty(3)
+        _check(lib.mncclDistillForward(rows.data_ptr(), _FLOATS[rows.dtype], _row_stride(rows), T, V, ids.data_ptr(), top.data_ptr(), K, tau, p.data_ptr(),
+                                       stats.data_ptr(), row_loss.data_ptr(), counts.data_ptr(), mean.data_ptr(), s), "mncclDistillForward")
+    return p, stats, counts, row_loss, mean
+
+
+def distill_backward(lib, rows, ids, p, stats, counts, tokens, tau, grad, d):
+    with _on(rows.device, None) as s:
+        _check(lib.mncclDistillBackward(rows.data_ptr(), _FLOATS[rows.dtype], _row_stride(rows), *rows.shape, ids.data_ptr(), p.data_ptr(), ids.shape[1], tau,
+                                        stats.data_ptr(), counts.data_ptr(), grad.data_ptr(), 1 if grad.dim() else 0,
+                                        tokens.data_ptr() if tokens is not None else None, d.data_ptr(), _row_stride(d), s), "mncclDistillBackward")
+
+
 class Calls:
     """The extension's functions, bound to a loaded library."""
 
     def __init__(self, lib):
         from functools import partial
 
-        for f in (all_reduce, gemm, gemm_rs, ag_gemm):
+        for f in (all_reduce, gemm, gemm_rs, ag_gemm, quantize_fp8, gemm_fp8, distill_forward, distill_backward):
             setattr(self, f.__name__, partial(f, lib))

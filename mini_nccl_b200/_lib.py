@@ -235,7 +235,8 @@ def ext():
 
     address = lambda name: C.cast(getattr(L, name), C.c_void_p).value if hasattr(L, name) else 0
     _torch_ext.bind(address("mncclAllReduceEx"), address("mncclCommGetAsyncError"), address("mncclGemmBf16"),
-                    address("mncclGemmReduceScatterBf16Comm"), address("mncclAllGatherGemmBf16Comm"))
+                    address("mncclGemmReduceScatterBf16Comm"), address("mncclAllGatherGemmBf16Comm"), address("mncclQuantizeFp8"),
+                    address("mncclGemmFp8"), address("mncclDistillForward"), address("mncclDistillBackward"))
     _EXT = _torch_ext
     return _EXT
 

@@ -10,8 +10,7 @@ import math
 import torch
 import torch.nn.functional as F
 
-from .._lib import lib
-from .fp8 import _CODES, _check, _on
+from .fp8 import _FLOATS, _call
 from .gemm import gemm_bf16
 from .lm_loss import _MAX_ROWS, _eight, _pays, _plain, _transposed
 from .lm_loss import _rows as _dense_rows
@@ -39,30 +38,14 @@ def _reference(logits, ids, top, tau, reduction):
     return rows.sum() if reduction == "sum" else rows.sum() / counts.sum()
 
 
-class _Teacher:
-    """What the kernels keep of a call for its backward pass, and the two calls."""
-
-    @staticmethod
-    def forward(rows, ids, top, tau, stream):
-        (T, V), K = rows.shape, ids.shape[-1]
-        p, row_loss = torch.empty((T, K), dtype=torch.float32, device=rows.device), torch.empty(T, dtype=torch.float32, device=rows.device)
-        stats, mean = torch.empty((T, 2), dtype=torch.float32, device=rows.device), torch.empty(3, dtype=torch.float32, device=rows.device)
-        counts = torch.empty(T, dtype=torch.int32, device=rows.device)
-        _check(lib().mncclDistillForward(rows.data_ptr(), _CODES[rows.dtype], _stride(rows), T, V, ids.data_ptr(), top.data_ptr(), K, tau, p.data_ptr(),
-                                         stats.data_ptr(), row_loss.data_ptr(), counts.data_ptr(), mean.data_ptr(), stream), "mncclDistillForward")
-        return p, stats, counts, row_loss, mean
-
-    @staticmethod
-    def backward(rows, ids, p, stats, counts, mean, tau, reduction, grad, d, stream):
-        T, V = rows.shape
-        _check(lib().mncclDistillBackward(rows.data_ptr(), _CODES[rows.dtype], _stride(rows), T, V, ids.data_ptr(), p.data_ptr(), ids.shape[-1], tau,
-                                          stats.data_ptr(), counts.data_ptr(), grad.data_ptr(), 1 if reduction == "none" else 0,
-                                          mean.data_ptr() + 8 if reduction == "mean" else None, d.data_ptr(), _stride(d), stream),
-               "mncclDistillBackward")
+def _forward(rows, ids, top, tau):
+    """(p, stats, counts, loss of each row, {sum, mean, tokens that count}): the first three for the backward pass."""
+    return _call("distill_forward", "mncclDistillForward", "csrc/kernels/distill.cu")(rows, ids, top, tau)
 
 
-def _stride(rows):
-    return rows.stride(0) if rows.shape[0] > 1 else max(rows.stride(0), rows.shape[1])
+def _backward(rows, ids, p, stats, counts, mean, tau, reduction, grad, d):
+    _call("distill_backward", "mncclDistillBackward", "csrc/kernels/distill.cu")(rows, ids, p, stats, counts, mean[2:] if reduction == "mean" else None,
+                                                                                 tau, (grad.reshape(-1) if reduction == "none" else grad).contiguous(), d)
 
 
 def _logit_rows(logits):
@@ -89,8 +72,7 @@ class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, top, tau, reduction):
         rows = _logit_rows(logits)
-        with _on(logits.device, None) as stream:
-            p, stats, counts, row_loss, mean = _Teacher.forward(rows, ids, top, tau, stream)
+        p, stats, counts, row_loss, mean = _forward(rows, ids, top, tau)
         ctx.save_for_backward(logits, ids, top, p, stats, counts, mean)
         ctx.tau, ctx.reduction = tau, reduction
         return _reduced(row_loss, mean, reduction, logits.shape[:-1])
@@ -108,9 +90,8 @@ class _Distillation(torch.autograd.Function):
         if rows.shape[0] > 1 and rows.stride(0) != V:
             per = 16 // rows.element_size()
             wide = -(-V // per) * per
-        with _on(logits.device, None) as stream:
-            d = torch.empty((rows.shape[0], wide), dtype=rows.dtype, device=rows.device)[:, :V]
-            _Teacher.backward(rows, ids, p, stats, counts, mean, ctx.tau, ctx.reduction, grad.contiguous(), d, stream)
+        d = torch.empty((rows.shape[0], wide), dtype=rows.dtype, device=rows.device)[:, :V]
+        _backward(rows, ids, p, stats, counts, mean, ctx.tau, ctx.reduction, grad, d)
         return (d.view(logits.shape), *none)
 
 
@@ -121,7 +102,7 @@ class _LmHeadDistillation(torch.autograd.Function):
         rows, w = _dense_rows(x.detach()).view(-1, x.shape[-1]), _dense_rows(weight.detach())
         logits = torch.empty((rows.shape[0], _eight(V)), dtype=x.dtype, device=x.device)
         gemm_bf16(rows, w, out=logits[:, :V])
-        p, stats, counts, row_loss, mean = _Teacher.forward(logits[:, :V], ids, top, tau, torch.cuda.current_stream().cuda_stream)
+        p, stats, counts, row_loss, mean = _forward(logits[:, :V], ids, top, tau)
         ctx.save_for_backward(x, weight, ids, top, logits, p, stats, counts, mean)
         ctx.tau = tau
         return mean[1].clone()
@@ -137,7 +118,7 @@ class _LmHeadDistillation(torch.autograd.Function):
         V = weight.shape[0]
         rows, logits = _dense_rows(x).view(-1, x.shape[-1]), _dense_rows(logits)
         d = torch.empty((rows.shape[0], _eight(V)), dtype=x.dtype, device=x.device)[:, :V]
-        _Teacher.backward(logits[:, :V], ids, p, stats, counts, mean, ctx.tau, "mean", grad.contiguous(), d, stream)
+        _backward(logits[:, :V], ids, p, stats, counts, mean, ctx.tau, "mean", grad, d)
         dx = dw = None
         if want_x and V % 8 == 0:
             dx = gemm_bf16(d, _transposed(_dense_rows(weight), stream)).view(x.shape)
@@ -156,7 +137,7 @@ def _plain_call():
 
 def _native(logits, ids, top):
     """Whether the kernels take the call; the plain operators take the others."""
-    if not (logits.is_cuda and _plain(logits) and _plain(ids) and _plain(top) and logits.dtype in _CODES):
+    if not (logits.is_cuda and _plain(logits) and _plain(ids) and _plain(top) and logits.dtype in _FLOATS):
         return False
     if not (0 < ids.shape[-1] <= _MAX_ENTRIES and 0 < ids[..., 0].numel() < 2**31 and 0 < logits.shape[-1] < 2**31 - 2**12) or not _plain_call():
         return False

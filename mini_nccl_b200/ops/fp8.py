@@ -9,88 +9,24 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from .._lib import lib
+from .._lib import ext, lib
 
 BLOCK = 128
-E4M3 = torch.float8_e4m3fn
-_CODES = {torch.float16: 6, torch.float32: 7, torch.bfloat16: 9}
-_MOST = 2**31 - 2**16   # rows and columns of a matrix: indices are 32-bit, elements are addressed with 64
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_calls = {}   # the extension's entry points, looked up on the first call
 
 
-def _blocks(n):
-    return -(-n // BLOCK)
-
-
-def _padded(n):
-    return -(-n // 16) * 16
-
-
-def _check(rc, what):
-    if rc != 0:
-        raise RuntimeError(f"{what} failed with code {rc}")
-
-
-class _on:
-    """The GPU and the stream that a call runs on: the tensors' GPU, and `stream` or that GPU's current one.  What is
-    allocated inside belongs to that stream."""
-
-    def __init__(self, device, stream):
-        if stream is not None and stream.device != device:
-            raise ValueError(f"the stream is on {stream.device}, the tensors are on {device}")
-        self.with_ = []
-        if device.index != torch.cuda.current_device():
-            self.with_.append(torch.cuda.device(device))
-        if stream is not None:
-            self.with_.append(torch.cuda.stream(stream))
-
-    def __enter__(self):
-        for w in self.with_:
-            w.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *what):
-        for w in reversed(self.with_):
-            w.__exit__(*what)
-
-
-def _matrix(t, name, dtypes):
-    """(rows, columns, row stride) of a matrix the kernels can read."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{name} must be a CUDA tensor")
-    if t.dtype not in dtypes:
-        raise TypeError(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, not {t.dtype}")
-    if t.dim() != 2 or max(t.shape) > _MOST:
-        raise ValueError(f"{name} must be a matrix of at most {_MOST} rows and columns")
-    rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name} needs a unit inner stride")
-    ld = t.stride(0) if rows > 1 else _padded(cols)
-    if ld < cols:
-        raise ValueError(f"{name}'s rows overlap")
-    return rows, cols, ld
+def _call(name, symbol, source):
+    if name not in _calls:
+        if not hasattr(lib(), symbol):
+            raise RuntimeError(f"libmini_nccl.so was built without {source}")
+        _calls[name] = getattr(ext(), name)
+    return _calls[name]
 
 
 def _quantize(x, block_rows, transposed, stream=None):
     """Buffers with padded rows, [M, padded K] and [K, padded M], and scales as the kernels write them."""
-    M, K, ld = _matrix(x, "x", _CODES)
-    if block_rows not in (1, BLOCK):
-        raise ValueError("block_rows must be 1 or 128")
-    L = lib()
-    if not hasattr(L, "mncclQuantizeFp8"):
-        raise RuntimeError("libmini_nccl.so was built without csrc/kernels/fp8_quantize.cu")
-    with _on(x.device, stream) as s:
-        q = torch.empty((M, _padded(K)), dtype=E4M3, device=x.device)
-        scale = torch.empty((_blocks(K), M) if block_rows == 1 else (_blocks(M), _blocks(K)), dtype=torch.float32, device=x.device)
-        qt = scale_t = None
-        if transposed:
-            qt = torch.empty((K, _padded(M)), dtype=E4M3, device=x.device)
-            if block_rows == 1:
-                scale_t = torch.empty((_blocks(M), K), dtype=torch.float32, device=x.device)
-        if M and K:
-            _check(L.mncclQuantizeFp8(x.data_ptr(), _CODES[x.dtype], ld, M, K, block_rows, q.data_ptr(), q.shape[1], scale.data_ptr(),
-                                      qt.data_ptr() if transposed else None, qt.shape[1] if transposed else 0,
-                                      scale_t.data_ptr() if scale_t is not None else None, s), "mncclQuantizeFp8")
-    return q, scale, qt, scale_t
+    return _call("quantize_fp8", "mncclQuantizeFp8", "csrc/kernels/fp8_quantize.cu")(x, block_rows, transposed, stream)
 
 
 def quantize_fp8(x, block_rows=1, transposed=False, stream=None):
@@ -109,53 +45,13 @@ def quantize_fp8(x, block_rows=1, transposed=False, stream=None):
     return out if not transposed else (*out, qt[:, :M], scale_t.t() if block_rows == 1 else scale.t())
 
 
-def _scale(t, name, rows, K, device):
-    """(row stride, block stride, rows of a scale) of the scales of an operand [rows, K]."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device:
-        raise TypeError(f"{name} must be an fp32 tensor on {device}")
-    if t.dim() != 2 or t.shape[1] != _blocks(K) or t.shape[0] not in (rows, _blocks(rows)):
-        raise ValueError(f"{name} must be [{rows} or {_blocks(rows)}, {_blocks(K)}], not {list(t.shape)}")
-    return t.stride(0), t.stride(1), 1 if t.shape[0] == rows else BLOCK
-
-
-def _operand(t, name):
-    rows, cols, ld = _matrix(t, name, (E4M3,))
-    if t.numel() and (t.data_ptr() % 16 or ld % 16):
-        raise ValueError(f"{name}'s rows must start on 16 bytes (quantize_fp8 lays them out so)")
-    return rows, cols, ld
-
-
 def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=None, bias=None, stream=None):
     """``out[M, N] = a[M, K] @ b[N, K].T (+ bias[N])`` of e4m3 operands with a scale for each block of 128 along K; a scale covers one
     row or 128 rows: ``a_scale [M or ceil(M / 128), ceil(K / 128)]``, ``b_scale`` likewise, any fp32 values and strides.
 
     A block's products are summed in fp32, scaled and added up in fp32; with the bias added, one rounding to ``out``'s type (bf16 by
     default, fp16 or fp32).  ``bias`` has that type.  Operands have rows that start on 16 bytes.  Not differentiable."""
-    M, K, lda = _operand(a, "a")
-    N, Kb, ldb = _operand(b, "b")
-    if K != Kb or b.device != a.device:
-        raise ValueError("shapes: a [M, K], b [N, K], on one GPU")
-    sa = _scale(a_scale, "a_scale", M, K, a.device)
-    sb = _scale(b_scale, "b_scale", N, K, a.device)
-    L = lib()
-    if not hasattr(L, "mncclGemmFp8"):
-        raise RuntimeError("libmini_nccl.so was built without csrc/kernels/gemm_fp8.cu")
-    if out is not None and out_dtype not in (None, out.dtype):
-        raise ValueError("out has another type than out_dtype")
-    with _on(a.device, stream) as s:
-        if out is None:
-            out = torch.empty((M, N), dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=a.device)
-        if tuple(out.shape) != (M, N) or out.device != a.device:
-            raise ValueError("out must be [M, N] on the operands' GPU")
-        ldc = _matrix(out, "out", _CODES)[2]
-        if bias is not None and (bias.dtype != out.dtype or bias.device != a.device or tuple(bias.shape) != (N,) or (N > 1 and bias.stride(0) != 1)):
-            raise ValueError("bias must be [N], dense, of out's type and on its GPU")
-        if K == 0:
-            return out.zero_() if bias is None else out.copy_(bias.detach().expand(M, N))
-        if M and N:
-            _check(L.mncclGemmFp8(a.data_ptr(), lda, a_scale.data_ptr(), *sa, b.data_ptr(), ldb, b_scale.data_ptr(), *sb, out.data_ptr(), ldc,
-                                  _CODES[out.dtype], bias.data_ptr() if bias is not None else None, M, N, K, s), "mncclGemmFp8")
-    return out
+    return _call("gemm_fp8", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")(a, a_scale, b, b_scale, out, out_dtype, bias, stream)
 
 
 def _rows(t, cols):
@@ -208,7 +104,7 @@ def linear_fp8(x, weight, bias=None):
     for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
         if t is None and name == "bias":
             continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _CODES:
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _FLOATS:
             raise TypeError(f"{name} must be a CUDA tensor in bf16, fp16 or fp32")
         if t.dtype != x.dtype or t.device != x.device:
             raise TypeError(f"{name} must have x's type and be on its GPU")

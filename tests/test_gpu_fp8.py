@@ -329,6 +329,44 @@ def test_linear_strides_hooks_autocast_and_nothing():
         d.float().sum().backward()
 
 
+# ---- the binding
+
+
+@pytest.mark.gpu
+def test_calls_through_ctypes_do_the_same():
+    """What stands in for the extension where that cannot be built."""
+    import mini_nccl_b200 as mn
+    from mini_nccl_b200 import _lib
+    from mini_nccl_b200._ctypes_calls import Calls
+
+    ext, plain = _lib.ext(), Calls(mn.lib())
+    x, w = _input(70, 300, torch.bfloat16).cuda(), _input(140, 300, torch.float32, 1).cuda()
+    bias = torch.randn(140, device="cuda").half()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for rows, both, stream in ((1, True, None), (128, True, None), (1, False, side)):
+        got, want = ([c.quantize_fp8(x, rows, both, stream) for c in (plain, ext)])
+        torch.cuda.synchronize()
+        for p, q in zip(got, want):
+            assert (p is None) == (q is None) and (p is None or (p.shape == q.shape and torch.equal(p[:, :64].float(), q[:, :64].float())))
+    args = (*quantize_fp8(x), *quantize_fp8(w, block_rows=128))
+    assert torch.equal(plain.gemm_fp8(*args, None, torch.float16, bias, None), ext.gemm_fp8(*args, None, torch.float16, bias, None))
+    rows, ids, top = torch.randn(5, 1000, device="cuda"), torch.randint(-1, 1000, (5, 7), device="cuda"), torch.randn(5, 7, device="cuda")
+    grads = []
+    for c in (plain, ext):
+        p, stats, counts, row_loss, mean = c.distill_forward(rows, ids, top, 2.0)
+        d = torch.zeros_like(rows)
+        c.distill_backward(rows, ids, p, stats, counts, mean[2:], 2.0, torch.ones((), device="cuda"), d)
+        grads.append((row_loss, mean, d))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    for bad, error in ((lambda c: c.quantize_fp8(x.double(), 1, False, None), TypeError), (lambda c: c.quantize_fp8([1], 1, False, None), TypeError),
+                       (lambda c: c.quantize_fp8(x, 2, False, None), ValueError), (lambda c: c.gemm_fp8(*args, None, torch.int8, None, None), TypeError),
+                       (lambda c: c.gemm_fp8(*args, None, None, bias[:3], None), ValueError), (lambda c: c.gemm_fp8(args[0], args[0], *args[2:], None, None, None, None), TypeError)):
+        for c in (plain, ext):
+            with pytest.raises(error):
+                bad(c)
+
+
 # ---- refusals
 
 
