@@ -21,9 +21,7 @@ namespace {
 constexpr int kBlock = 128;
 constexpr int kThreads = 256;
 
-// Bits of |x| as an fp32 number: their order is that of the magnitudes, with infinity and NaN above all else.
-__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
+// The scale of a block whose largest magnitude has these fp32 bits, and its inverse.
 struct Scale {
   float scale, inverse;
 };
@@ -37,118 +35,159 @@ __device__ __forceinline__ Scale scale_of(uint32_t top) {
   return {__uint_as_float(static_cast<uint32_t>(biased) << 23), __uint_as_float(static_cast<uint32_t>(254 - biased) << 23)};
 }
 
+// Eight elements of a row as they lie in memory, and what is asked of them.
 template <typename T>
-__device__ __forceinline__ float as_float(T x) {
-  if constexpr (sizeof(T) == 4) return x;
-  else if constexpr (std::is_same_v<T, __half>) return __half2float(x);
-  else return __bfloat162float(x);
-}
+struct Eight {
+  static constexpr int kWords = 2 * sizeof(T);   // 32-bit
+  uint32_t w[kWords];
 
-// Elements [c, c + 8) of a row of K, zeros beyond its end.
-template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int c, int K, bool vec, float (&f)[8]) {
-  if (vec && c + 8 <= K) {
-    T v[8];
+  // Elements [c, c + 8) of a row of K, zeros beyond its end.
+  __device__ __forceinline__ void load(const T* __restrict__ row, int c, int K, bool vec) {
+    if (vec && c + 8 <= K) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-      reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+        w[4 * i] = v.x;
+        w[4 * i + 1] = v.y;
+        w[4 * i + 2] = v.z;
+        w[4 * i + 3] = v.w;
+      }
+    } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = as_float(v[j]);
-  } else {
+      for (int j = 0; j < 8; ++j) w[j] = c + j < K ? __float_as_uint(row[c + j]) : 0u;
+    } else {
+      const uint16_t* bits = reinterpret_cast<const uint16_t*>(row);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = c + j < K ? as_float(row[c + j]) : 0.0f;
+      for (int j = 0; j < 4; ++j)
+        w[j] = (c + 2 * j < K ? bits[c + 2 * j] : 0u) | (c + 2 * j + 1 < K ? static_cast<uint32_t>(bits[c + 2 * j + 1]) << 16 : 0u);
+    }
   }
-}
-
-__device__ __forceinline__ uint2 quantise8(const float (&f)[8], float inverse) {
-  uint32_t w[2];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i] * inverse, f[4 * i + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i + 2] * inverse, f[4 * i + 3] * inverse), __NV_SATFINITE, __NV_E4M3);
-    w[i] = lo | (hi << 16);
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
   }
-  return make_uint2(w[0], w[1]);
+  __device__ __forceinline__ float operator[](int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+    else if constexpr (std::is_same_v<T, __half>) return __half2float(__ushort_as_half(static_cast<uint16_t>(w[j / 2] >> (j % 2 * 16))));
+    else return __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+  }
+};
+
+// Magnitudes as bits, whose order is that of the numbers, with infinity and NaN above all else: one fp32 a word, or two 16-bit numbers.
+template <typename T>
+struct Bits {
+  static __device__ __forceinline__ uint32_t of(uint32_t w) { return w & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu); }
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) return max(a, b);
+    else return __vmaxu2(a, b);
+  }
+  // the larger of a word's two numbers (or its one), as the bits of an fp32 number
+  static __device__ __forceinline__ uint32_t as_fp32(uint32_t w) {
+    if constexpr (sizeof(T) == 4) {
+      return w;
+    } else {
+      const uint32_t top = max(w & 0xffffu, w >> 16);
+      if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top))));
+      else return top << 16;
+    }
+  }
+};
+template <typename T>
+__device__ __forceinline__ uint32_t largest(const Eight<T>& v) {
+  uint32_t top = Bits<T>::of(v.w[0]);
+#pragma unroll
+  for (int i = 1; i < Eight<T>::kWords; ++i) top = Bits<T>::most(top, Bits<T>::of(v.w[i]));
+  return top;
 }
 
-// 1 x 128 blocks.  16 lanes hold a block, 8 elements each; a thread block takes one block of 16 neighbouring rows, whose
-// scales are 64 contiguous bytes: scales are stored [K blocks][M].
+__device__ __forceinline__ uint32_t quantise4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
 template <typename T>
+__device__ __forceinline__ uint2 quantise8(const Eight<T>& v, float inverse) {
+  return make_uint2(quantise4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse),
+                    quantise4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
+}
+
+// 1 x 128 blocks.  16 lanes hold a block, 8 elements each; a thread block takes N blocks of 16 neighbouring rows, all loaded before the first is
+// looked at, and a block's scales of 16 rows are 64 contiguous bytes: scales are stored [K blocks][M].
+template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)
 quantise_rows_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t* __restrict__ q, size_t ldq, float* __restrict__ scale, bool vec) {
   const int m = static_cast<int>(blockIdx.x) * 16 + static_cast<int>(threadIdx.x >> 4);
-  const int c = static_cast<int>(blockIdx.y) * kBlock + static_cast<int>(threadIdx.x & 15) * 8;
+  const int first = static_cast<int>(blockIdx.y) * N, c = first * kBlock + static_cast<int>(threadIdx.x & 15) * 8;
   if (m >= M) return;   // all 16 lanes of a block
-  float f[8];
-  load8(x + m * ldx, c, K, vec, f);
-  uint32_t top = 0;
+  Eight<T> v[N];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, magnitude(f[j]));
+  for (int i = 0; i < N; ++i) v[i].load(x + m * ldx, c + i * kBlock, K, vec);
   const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
 #pragma unroll
-  for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(lanes, top, d));
-  const Scale s = scale_of(top);
-  // (q's rows are padded to 16 bytes)
-  if (c < K) *reinterpret_cast<uint2*>(q + m * ldq + c) = quantise8(f, s.inverse);
-  if ((threadIdx.x & 15) == 0) scale[static_cast<size_t>(blockIdx.y) * M + m] = s.scale;
+  for (int i = 0; i < N; ++i) {
+    if ((first + i) * kBlock >= K) break;
+    uint32_t top = largest(v[i]);
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) top = Bits<T>::most(top, __shfl_xor_sync(lanes, top, d));
+    const Scale s = scale_of(Bits<T>::as_fp32(top));
+    // (q's rows are padded to 16 bytes)
+    if (c + i * kBlock < K) *reinterpret_cast<uint2*>(q + m * ldq + c + i * kBlock) = quantise8(v[i], s.inverse);
+    if ((threadIdx.x & 15) == 0) scale[static_cast<size_t>(first + i) * M + m] = s.scale;
+  }
 }
 
-// A tile of 128 x 128 elements, which holds whole blocks of either kind along both dimensions: x is read once for q and
-// the transpose qt.  A thread holds 4 neighbouring rows of 2 x 8 columns, so that 4 elements of a column are one word of
-// the transposed tile in shared memory, [column][32 words + 1].
+// A tile of 128 x 128 elements, which holds whole blocks of either kind along both dimensions: x is read once for q, the transpose qt and the sums
+// of the tile's columns.  A thread holds 4 neighbouring rows of 2 x 8 columns, as they lie in memory (as fp32 numbers 16-bit types took 128
+// registers, and half of the memory's rate: 64 us for 8192 x 4096), so that 4 elements of a column are one word of the transposed tile in shared
+// memory, [column][32 words + 1].
 constexpr int kPitch = 33;
 
 template <typename T, bool SQUARE>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
 quantise_tile_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t* __restrict__ q, size_t ldq, float* __restrict__ scale,
-                     uint8_t* __restrict__ qt, size_t ldt, float* __restrict__ scale_t, bool vec) {
+                     uint8_t* __restrict__ qt, size_t ldt, float* __restrict__ scale_t, float* __restrict__ sums, bool vec) {
   __shared__ uint32_t tile[kBlock * kPitch];
-  __shared__ uint32_t part[8][kBlock];   // a warp's largest magnitude of each column
+  __shared__ uint32_t part[8][kBlock];   // a warp's largest magnitude of each column, then its sum
   __shared__ float inverse[kBlock];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m0 = static_cast<int>(blockIdx.x) * kBlock, k0 = static_cast<int>(blockIdx.y) * kBlock;
   const int r0 = warp * 16 + (lane >> 3) * 4, c0 = (lane & 7) * 8;   // columns c0 .. and c0 + 64 ..
-  float f[4][2][8];
-  uint32_t all = 0;
+  Eight<T> v[4][2];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int m = m0 + r0 + i;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if (m < M) load8(x + m * ldx, k0 + c0 + h * 64, K, vec, f[i][h]);
-      else
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[i][h][j] = 0.0f;
+      if (m < M) v[i][h].load(x + m * ldx, k0 + c0 + h * 64, K, vec);
+      else v[i][h].clear();
     }
   }
-  Scale s[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, magnitude(f[i][h][j]));
-    if constexpr (SQUARE) {
-      all = max(all, top);
-    } else {
-#pragma unroll
-      for (int d = 4; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-      s[i] = scale_of(top);
-      if ((lane & 7) == 0 && m0 + r0 + i < M) scale[static_cast<size_t>(blockIdx.y) * M + m0 + r0 + i] = s[i].scale;
-    }
-  }
+  float row_inverse[4];
   if constexpr (SQUARE) {
+    uint32_t all = 0;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) all = max(all, __shfl_xor_sync(0xffffffffu, all, d));
+    for (int i = 0; i < 4; ++i) all = Bits<T>::most(all, Bits<T>::most(largest(v[i][0]), largest(v[i][1])));
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) all = Bits<T>::most(all, __shfl_xor_sync(0xffffffffu, all, d));
     if (lane == 0) part[0][warp] = all;
     __syncthreads();
     all = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) all = max(all, part[0][w]);
+    for (int w = 0; w < 8; ++w) all = Bits<T>::most(all, part[0][w]);
+    const Scale s = scale_of(Bits<T>::as_fp32(all));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = scale_of(all);
-    if (threadIdx.x == 0) scale[static_cast<size_t>(blockIdx.x) * gridDim.y + blockIdx.y] = s[0].scale;
+    for (int i = 0; i < 4; ++i) row_inverse[i] = s.inverse;
+    if (threadIdx.x == 0) scale[static_cast<size_t>(blockIdx.x) * gridDim.y + blockIdx.y] = s.scale;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t top = Bits<T>::most(largest(v[i][0]), largest(v[i][1]));
+#pragma unroll
+      for (int d = 4; d > 0; d >>= 1) top = Bits<T>::most(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const Scale s = scale_of(Bits<T>::as_fp32(top));
+      row_inverse[i] = s.inverse;
+      if ((lane & 7) == 0 && m0 + r0 + i < M) scale[static_cast<size_t>(blockIdx.y) * M + m0 + r0 + i] = s.scale;
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -156,63 +195,109 @@ quantise_tile_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t*
     for (int h = 0; h < 2; ++h) {
       const int c = k0 + c0 + h * 64;
       if (m0 + r0 + i < M && c < K)
-        *reinterpret_cast<uint2*>(q + static_cast<size_t>(m0 + r0 + i) * ldq + c) = quantise8(f[i][h], s[i].inverse);
+        *reinterpret_cast<uint2*>(q + static_cast<size_t>(m0 + r0 + i) * ldq + c) = quantise8(v[i][h], row_inverse[i]);
     }
   if (qt == nullptr) return;
   if constexpr (!SQUARE) {
+    // Largest magnitude of each column: of the thread's four rows, of the warp's 16, of the tile.  A word holds the columns that lie next to one
+    // another in memory.
+    constexpr int kPer = 4 / static_cast<int>(sizeof(T));   // columns a word holds
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < Eight<T>::kWords; ++j) {
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, magnitude(f[i][h][j]));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        if (lane < 8) part[warp][c0 + h * 64 + j] = top;
+        for (int i = 0; i < 4; ++i) top = Bits<T>::most(top, Bits<T>::of(v[i][h].w[j]));
+        top = Bits<T>::most(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = Bits<T>::most(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        if (lane < 8) part[warp][(c0 + h * 64) / kPer + j] = top;
       }
     __syncthreads();
     if (threadIdx.x < kBlock) {
       uint32_t top = 0;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) top = max(top, part[w][threadIdx.x]);
-      const Scale t = scale_of(top);
+      for (int w = 0; w < 8; ++w) top = Bits<T>::most(top, part[w][threadIdx.x / kPer]);
+      if constexpr (kPer == 2) top = threadIdx.x & 1 ? top >> 16 : top & 0xffffu;
+      const Scale t = scale_of(Bits<T>::as_fp32(top));
       inverse[threadIdx.x] = t.inverse;
       if (k0 + static_cast<int>(threadIdx.x) < K) scale_t[static_cast<size_t>(blockIdx.x) * K + k0 + threadIdx.x] = t.scale;
     }
     __syncthreads();
+    if (sums != nullptr) {   // in a fixed order: rows of a thread, of a warp, warps; the caller's blocks of rows
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float s = (v[0][h][j] + v[1][h][j]) + (v[2][h][j] + v[3][h][j]);
+          s += __shfl_xor_sync(0xffffffffu, s, 8);
+          s += __shfl_xor_sync(0xffffffffu, s, 16);
+          if (lane < 8) part[warp][c0 + h * 64 + j] = __float_as_uint(s);
+        }
+    }
   }
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int c = c0 + h * 64 + j;
-      const float v = SQUARE ? s[0].inverse : inverse[c];
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0][h][j] * v, f[1][h][j] * v), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2][h][j] * v, f[3][h][j] * v), __NV_SATFINITE, __NV_E4M3);
-      tile[c * kPitch + r0 / 4] = lo | (hi << 16);
+      const float s = SQUARE ? row_inverse[0] : inverse[c];
+      tile[c * kPitch + r0 / 4] = quantise4(v[0][h][j] * s, v[1][h][j] * s, v[2][h][j] * s, v[3][h][j] * s);
     }
   __syncthreads();
 #pragma unroll 4
   for (int c = warp; c < kBlock; c += 8)   // a column leaves as 128 bytes; rows of qt are padded to 16
     if (k0 + c < K && m0 + lane * 4 < static_cast<int>(ldt))
       *reinterpret_cast<uint32_t*>(qt + static_cast<size_t>(k0 + c) * ldt + m0 + lane * 4) = tile[c * kPitch + lane];
+  if (!SQUARE && sums != nullptr && threadIdx.x < kBlock && k0 + static_cast<int>(threadIdx.x) < K) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += __uint_as_float(part[w][threadIdx.x]);
+    sums[static_cast<size_t>(blockIdx.x) * K + k0 + threadIdx.x] = s;
+  }
+}
+
+// out[k] = the sum over the tiles' sums [tiles][K], in their order.  32 columns a block, eight threads a column.
+template <typename T>
+__global__ void __launch_bounds__(256) sum_tiles_kernel(const float* __restrict__ sums, int tiles, int K, T* __restrict__ out) {
+  __shared__ float part[8][32];
+  const int k = static_cast<int>(blockIdx.x) * 32 + static_cast<int>(threadIdx.x & 31), y = threadIdx.x >> 5;
+  const int per = (tiles + 7) / 8;
+  float s = 0.0f;
+  if (k < K)
+    for (int t = y * per; t < min(tiles, (y + 1) * per); ++t) s += sums[static_cast<size_t>(t) * K + k];
+  part[y][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (y != 0 || k >= K) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x];
+  if constexpr (sizeof(T) == 4) out[k] = s;
+  else if constexpr (std::is_same_v<T, __half>) out[k] = __float2half_rn(s);
+  else out[k] = __float2bfloat16_rn(s);
+}
+
+int status() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : static_cast<int>(e) + 1000;
 }
 
 template <typename T>
 int quantise(const T* x, int64_t ldx, int M, int K, int block_rows, uint8_t* q, int64_t ldq, float* scale, uint8_t* qt, int64_t ldt, float* scale_t,
-             cudaStream_t stream) {
+             float* sums, cudaStream_t stream) {
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (ldx * static_cast<int64_t>(sizeof(T))) % 16 == 0;
-  const int blocks_k = (K + kBlock - 1) / kBlock;
-  if (block_rows == 1 && qt == nullptr) {
-    quantise_rows_kernel<T><<<dim3((M + 15) / 16, blocks_k), kThreads, 0, stream>>>(x, ldx, M, K, q, ldq, scale, vec);
+  const int blocks_k = (K + kBlock - 1) / kBlock, rows16 = (M + 15) / 16;
+  const dim3 grid((M + kBlock - 1) / kBlock, blocks_k);
+  if (block_rows == 128) {
+    quantise_tile_kernel<T, true><<<grid, kThreads, 0, stream>>>(x, ldx, M, K, q, ldq, scale, qt, ldt, scale_t, nullptr, vec);
+  } else if (qt != nullptr) {
+    quantise_tile_kernel<T, false><<<grid, kThreads, 0, stream>>>(x, ldx, M, K, q, ldq, scale, qt, ldt, scale_t, sums, vec);
+  } else if (static_cast<int64_t>(rows16) * blocks_k >= 4 * 2048) {
+    // Enough for every SM several times over: four blocks a thread in flight (8192 x 4096 bf16: 24.7 us with one).
+    quantise_rows_kernel<T, 4><<<dim3(rows16, (blocks_k + 3) / 4), kThreads, 0, stream>>>(x, ldx, M, K, q, ldq, scale, vec);
   } else {
-    const dim3 grid((M + kBlock - 1) / kBlock, blocks_k);
-    if (block_rows == 1) quantise_tile_kernel<T, false><<<grid, kThreads, 0, stream>>>(x, ldx, M, K, q, ldq, scale, qt, ldt, scale_t, vec);
-    else quantise_tile_kernel<T, true><<<grid, kThreads, 0, stream>>>(x, ldx, M, K, q, ldq, scale, qt, ldt, scale_t, vec);
+    quantise_rows_kernel<T, 1><<<dim3(rows16, blocks_k), kThreads, 0, stream>>>(x, ldx, M, K, q, ldq, scale, vec);
   }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : static_cast<int>(e) + 1000;
+  return status();
 }
 
 constexpr int kMaxK = 65535 * kBlock;   // gridDim.y
@@ -225,23 +310,38 @@ extern "C" {
 // x [M, K] (type 6 fp16, 7 fp32, 9 bf16; row stride ldx elements) -> q [M, K] e4m3 (row stride ldq, a multiple of 16 that holds K
 // rounded up to one; 16-byte aligned; the padding is written) and its scales: block_rows 1: scale[K blocks][M]; block_rows 128:
 // scale[M blocks][K blocks].  qt, if not null: the transpose [K, M] (ldt like ldq), for block_rows 1 quantised anew in blocks along M
-// with scale_t[M blocks][K].  Returns 0, -1 null or empty, -2 shape or alignment, or a cudaError_t + 1000.
+// with scale_t[M blocks][K].  sums, if not null (only with qt and block_rows 1): [M blocks][K], the columns' sums over each 128 rows.
+// Returns 0, -1 null or empty, -2 shape or alignment, or a cudaError_t + 1000.
 MNCCL_EXPORT int mncclQuantizeFp8(const void* x, int type, int64_t ldx, int M, int K, int block_rows, void* q, int64_t ldq, float* scale,
-                                  void* qt, int64_t ldt, float* scale_t, cudaStream_t stream) {
+                                  void* qt, int64_t ldt, float* scale_t, float* sums, cudaStream_t stream) {
   if (!x || !q || !scale || M <= 0 || K <= 0 || (qt && block_rows == 1 && !scale_t)) return -1;
   const auto padded = [](const void* p, int64_t ld, int64_t n) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 16 == 0 && ld >= (n + 15) / 16 * 16;
   };
-  if ((block_rows != 1 && block_rows != kBlock) || ldx < K || K > kMaxK || M > 0x7fffff00 || !padded(q, ldq, K) || (qt && !padded(qt, ldt, M)))
+  if ((block_rows != 1 && block_rows != kBlock) || ldx < K || K > kMaxK || M > 0x7fffff00 || !padded(q, ldq, K) || (qt && !padded(qt, ldt, M)) ||
+      (sums && (!qt || block_rows != 1)))
     return -2;
   uint8_t* qb = static_cast<uint8_t*>(q);
   uint8_t* tb = static_cast<uint8_t*>(qt);
   switch (type) {
-    case 6: return quantise(static_cast<const __half*>(x), ldx, M, K, block_rows, qb, ldq, scale, tb, ldt, scale_t, stream);
-    case 7: return quantise(static_cast<const float*>(x), ldx, M, K, block_rows, qb, ldq, scale, tb, ldt, scale_t, stream);
-    case 9: return quantise(static_cast<const __nv_bfloat16*>(x), ldx, M, K, block_rows, qb, ldq, scale, tb, ldt, scale_t, stream);
+    case 6: return quantise(static_cast<const __half*>(x), ldx, M, K, block_rows, qb, ldq, scale, tb, ldt, scale_t, sums, stream);
+    case 7: return quantise(static_cast<const float*>(x), ldx, M, K, block_rows, qb, ldq, scale, tb, ldt, scale_t, sums, stream);
+    case 9: return quantise(static_cast<const __nv_bfloat16*>(x), ldx, M, K, block_rows, qb, ldq, scale, tb, ldt, scale_t, sums, stream);
   }
   return -2;
+}
+
+// out[K] (type as above) = the columns' sums of mncclQuantizeFp8 over all `blocks` blocks of rows.  Returns as that.
+MNCCL_EXPORT int mncclSumBlocks(const float* sums, int blocks, int K, void* out, int type, cudaStream_t stream) {
+  if (!sums || !out || blocks <= 0 || K <= 0) return -1;
+  const unsigned grid = static_cast<unsigned>((K + 31) / 32);
+  switch (type) {
+    case 6: sum_tiles_kernel<<<grid, 256, 0, stream>>>(sums, blocks, K, static_cast<__half*>(out)); break;
+    case 7: sum_tiles_kernel<<<grid, 256, 0, stream>>>(sums, blocks, K, static_cast<float*>(out)); break;
+    case 9: sum_tiles_kernel<<<grid, 256, 0, stream>>>(sums, blocks, K, static_cast<__nv_bfloat16*>(out)); break;
+    default: return -2;
+  }
+  return status();
 }
 
 }  // extern "C"

@@ -37,6 +37,7 @@ struct Library {
   int (*ag_gemm)(void* const*, const void*, void*, int, int, int, int, int, int, int, int, void* const*, void* const*, uint32_t*, int,
                  int, const void*, size_t, cudaStream_t) = nullptr;
   decltype(&mncclQuantizeFp8) quantize_fp8 = nullptr;
+  decltype(&mncclSumBlocks) sum_blocks = nullptr;
   decltype(&mncclGemmFp8) gemm_fp8 = nullptr;
   decltype(&mncclDistillForward) distill_forward = nullptr;
   decltype(&mncclDistillBackward) distill_backward = nullptr;
@@ -94,19 +95,20 @@ bool arg_count(Py_ssize_t n, Py_ssize_t want) {
   return n == want;
 }
 
-// bind(all_reduce_ex, async_error, gemm, gemm_rs, ag_gemm, quantize_fp8, gemm_fp8, distill_forward, distill_backward): addresses
-// in the library that ctypes has loaded (all but the first two may be 0)
+// bind(all_reduce_ex, async_error, gemm, gemm_rs, ag_gemm, quantize_fp8, sum_blocks, gemm_fp8, distill_forward,
+// distill_backward): addresses in the library that ctypes has loaded (all but the first two may be 0)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (!arg_count(n, 9)) return nullptr;
+  if (!arg_count(n, 10)) return nullptr;
   lib.all_reduce_ex = reinterpret_cast<decltype(lib.all_reduce_ex)>(PyLong_AsVoidPtr(args[0]));
   lib.async_error = reinterpret_cast<decltype(lib.async_error)>(PyLong_AsVoidPtr(args[1]));
   lib.gemm = reinterpret_cast<decltype(lib.gemm)>(PyLong_AsVoidPtr(args[2]));
   lib.gemm_rs = reinterpret_cast<decltype(lib.gemm_rs)>(PyLong_AsVoidPtr(args[3]));
   lib.ag_gemm = reinterpret_cast<decltype(lib.ag_gemm)>(PyLong_AsVoidPtr(args[4]));
   lib.quantize_fp8 = reinterpret_cast<decltype(lib.quantize_fp8)>(PyLong_AsVoidPtr(args[5]));
-  lib.gemm_fp8 = reinterpret_cast<decltype(lib.gemm_fp8)>(PyLong_AsVoidPtr(args[6]));
-  lib.distill_forward = reinterpret_cast<decltype(lib.distill_forward)>(PyLong_AsVoidPtr(args[7]));
-  lib.distill_backward = reinterpret_cast<decltype(lib.distill_backward)>(PyLong_AsVoidPtr(args[8]));
+  lib.sum_blocks = reinterpret_cast<decltype(lib.sum_blocks)>(PyLong_AsVoidPtr(args[6]));
+  lib.gemm_fp8 = reinterpret_cast<decltype(lib.gemm_fp8)>(PyLong_AsVoidPtr(args[7]));
+  lib.distill_forward = reinterpret_cast<decltype(lib.distill_forward)>(PyLong_AsVoidPtr(args[8]));
+  lib.distill_backward = reinterpret_cast<decltype(lib.distill_backward)>(PyLong_AsVoidPtr(args[9]));
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -386,8 +388,33 @@ PyObject* failed(const char* what, int rc) {
 }
 PyObject* wrap(const at::Tensor& t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); }
 
-// quantize_fp8(x, block_rows, transposed, stream | None) -> (q, scale, qt | None, scale_t | None) as the kernels write them: rows padded
-// to 16 bytes, scales [K blocks, M] (block_rows 1) or [M blocks, K blocks]
+// A matrix in 8 bits as the kernels write it: rows padded to 16 bytes, scales [K blocks, M] (block_rows 1) or [M blocks, K blocks]; the
+// transpose and the sums of the columns over blocks of rows where they are asked for.
+struct Quantized {
+  at::Tensor q, scale, qt, scale_t, sums;
+};
+int quantize(const at::Tensor& x, int64_t ld, bool row, bool transposed, bool sums, cudaStream_t stream, Quantized* out) {
+  const int64_t M = x.size(0), K = x.size(1);
+  const auto e4m3 = x.options().dtype(at::kFloat8_e4m3fn).requires_grad(false), f32 = x.options().dtype(at::kFloat).requires_grad(false);
+  out->q = at::empty({M, padded(K)}, e4m3);
+  out->scale = row ? at::empty({blocks(K), M}, f32) : at::empty({blocks(M), blocks(K)}, f32);
+  if (transposed) {
+    out->qt = at::empty({K, padded(M)}, e4m3);
+    if (row) out->scale_t = at::empty({blocks(M), K}, f32);
+    if (sums) out->sums = at::empty({blocks(M), K}, f32);
+  }
+  if (M == 0 || K == 0) return 0;
+  const auto floats = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = lib.quantize_fp8(x.data_ptr(), float_code(x), ld, static_cast<int>(M), static_cast<int>(K), row ? 1 : static_cast<int>(kBlock), out->q.data_ptr(),
+                        out->q.size(1), floats(out->scale), transposed ? out->qt.data_ptr() : nullptr, transposed ? out->qt.size(1) : 0, floats(out->scale_t),
+                        floats(out->sums), stream);
+  Py_END_ALLOW_THREADS
+  return rc;
+}
+
+// quantize_fp8(x, block_rows, transposed, stream | None) -> (q, scale, qt | None, scale_t | None), see Quantized
 PyObject* quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arg_count(n, 4)) return nullptr;
@@ -396,33 +423,17 @@ PyObject* quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const long block_rows = PyLong_AsLong(args[1]);
   const int transposed = PyObject_IsTrue(args[2]);
   if (transposed < 0 || PyErr_Occurred()) return nullptr;
-  const int code = float_code(*x);
   int64_t ld = 0;
-  if (!matrix(*x, "x", code >= 0, &ld)) return nullptr;
+  if (!matrix(*x, "x", float_code(*x) >= 0, &ld)) return nullptr;
   if (block_rows != 1 && block_rows != kBlock) {
     PyErr_SetString(PyExc_ValueError, "block_rows must be 1 or 128");
     return nullptr;
   }
   On o;
   if (!on(*x, args[3], &o)) return nullptr;
-  const int64_t M = x->size(0), K = x->size(1);
-  const auto e4m3 = x->options().dtype(at::kFloat8_e4m3fn).requires_grad(false), f32 = x->options().dtype(at::kFloat).requires_grad(false);
-  const bool row = block_rows == 1;
-  at::Tensor q = at::empty({M, padded(K)}, e4m3), scale = at::empty(row ? at::IntArrayRef{blocks(K), M} : at::IntArrayRef{blocks(M), blocks(K)}, f32), qt, scale_t;
-  if (transposed) {
-    qt = at::empty({K, padded(M)}, e4m3);
-    if (row) scale_t = at::empty({blocks(M), K}, f32);
-  }
-  int rc = 0;
-  if (M > 0 && K > 0) {
-    Py_BEGIN_ALLOW_THREADS
-    rc = lib.quantize_fp8(x->data_ptr(), code, ld, static_cast<int>(M), static_cast<int>(K), static_cast<int>(block_rows), q.data_ptr(), q.size(1),
-                          scale.data_ptr<float>(), transposed ? qt.data_ptr() : nullptr, transposed ? qt.size(1) : 0,
-                          scale_t.defined() ? scale_t.data_ptr<float>() : nullptr, o.raw);
-    Py_END_ALLOW_THREADS
-  }
-  if (rc != 0) return failed("mncclQuantizeFp8", rc);
-  return Py_BuildValue("(NNNN)", wrap(q), wrap(scale), wrap(qt), wrap(scale_t));
+  Quantized q;
+  if (const int rc = quantize(*x, ld, block_rows == 1, transposed != 0, false, o.raw, &q)) return failed("mncclQuantizeFp8", rc);
+  return Py_BuildValue("(NNNN)", wrap(q.q), wrap(q.scale), wrap(q.qt), wrap(q.scale_t));
   END_HANDLE_TH_ERRORS
 }
 
@@ -518,38 +529,140 @@ PyObject* gemm_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)); }
+// `t [..., cols]` as a matrix that the kernels can read (a copy only where the strides need one), and its row stride.
+at::Tensor rows_of(const at::Tensor& t, int64_t cols, int64_t* ld) {
+  c10::AutoGradMode no_grad(false);
+  at::Tensor r = t.dim() == 2 ? t : t.reshape({cols > 0 ? t.numel() / cols : 0, cols});
+  if ((cols > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < cols)) r = r.contiguous();
+  *ld = r.size(0) > 1 ? r.stride(0) : padded(cols);
+  return r;
+}
 
-// distill_forward(rows, ids, top, tau) -> (p, stats, counts, row_loss, mean); ops/distill.py has checked the arguments
-PyObject* distill_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  if (!arg_count(n, 4)) return nullptr;
-  const at::Tensor *rows = tensor_arg(args[0], "rows"), *ids = rows ? tensor_arg(args[1], "ids") : nullptr, *top = ids ? tensor_arg(args[2], "top") : nullptr;
-  if (!top) return nullptr;
-  const double tau = PyFloat_AsDouble(args[3]);
-  if (PyErr_Occurred()) return nullptr;
-  On o;
-  if (!on(*rows, Py_None, &o)) return nullptr;
-  const int64_t T = rows->size(0), K = ids->size(1);
-  const auto f32 = rows->options().dtype(at::kFloat).requires_grad(false);
-  at::Tensor p = at::empty({T, K}, f32), stats = at::empty({T, 2}, f32), counts = at::empty({T}, f32.dtype(at::kInt)), row_loss = at::empty({T}, f32), mean = at::empty({3}, f32);
+// out [M, N] = a * b^T (+ bias) of padded buffers: a [M, padded K] with scales [K blocks, M], b [N, padded K] with scales that have these strides.
+int product(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb, int64_t sb_row, int64_t sb_blk, int sb_rows, int64_t M, int64_t N,
+            int64_t K, const at::Tensor& out, const at::Tensor* bias, cudaStream_t stream) {
+  if (M == 0 || N == 0) return 0;
+  if (K == 0) {
+    c10::AutoGradMode no_grad(false);
+    out.zero_();
+    return 0;
+  }
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = lib.distill_forward(rows->data_ptr(), float_code(*rows), row_stride(*rows), static_cast<int>(T), static_cast<int>(rows->size(1)), ids->data_ptr<int64_t>(),
-                           top->data_ptr<float>(), static_cast<int>(K), static_cast<float>(tau), p.data_ptr<float>(), stats.data_ptr<float>(), row_loss.data_ptr<float>(),
-                           counts.data_ptr<int>(), mean.data_ptr<float>(), o.raw);
+  rc = lib.gemm_fp8(a.data_ptr(), a.size(1), sa.data_ptr<float>(), 1, M, 1, b.data_ptr(), b.size(1), sb.data_ptr<float>(), sb_row, sb_blk, sb_rows, out.data_ptr(),
+                    N, float_code(out), bias ? bias->data_ptr() : nullptr, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), stream);
   Py_END_ALLOW_THREADS
-  if (rc != 0) return failed("mncclDistillForward", rc);
-  return Py_BuildValue("(NNNNN)", wrap(p), wrap(stats), wrap(counts), wrap(row_loss), wrap(mean));
+  return rc;
+}
+
+// linear_fp8_forward(x [..., K], weight [N, K], bias [N] | None, want_x, want_w) -> (y [..., N], and for the backward pass x^T and its scales,
+// weight^T and the weight's scales, each None where it is not wanted); ops/fp8.py has checked the arguments
+PyObject* linear_fp8_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 5)) return nullptr;
+  const at::Tensor *x = tensor_arg(args[0], "x"), *weight = x ? tensor_arg(args[1], "weight") : nullptr, *bias = nullptr;
+  if (!weight || (args[2] != Py_None && !(bias = tensor_arg(args[2], "bias")))) return nullptr;
+  const bool want_x = args[3] == Py_True, want_w = args[4] == Py_True;
+  On o;
+  if (!on(*x, Py_None, &o)) return nullptr;
+  const int64_t N = weight->size(0), K = weight->size(1);
+  int64_t ldx = 0, ldw = 0;
+  const at::Tensor rows = rows_of(*x, K, &ldx), w = rows_of(*weight, K, &ldw), dense = bias ? bias->contiguous() : at::Tensor();
+  Quantized qx, qw;
+  if (const int rc = quantize(rows, ldx, true, want_w, false, o.raw, &qx)) return failed("mncclQuantizeFp8", rc);
+  if (const int rc = quantize(w, ldw, false, want_x, false, o.raw, &qw)) return failed("mncclQuantizeFp8", rc);
+  auto shape = x->sizes().vec();
+  shape.back() = N;
+  at::Tensor y = at::empty(shape, x->options().requires_grad(false));
+  if (const int rc = product(qx.q, qx.scale, qw.q, qw.scale, qw.scale.size(1), 1, static_cast<int>(kBlock), rows.size(0), N, K, y, bias ? &dense : nullptr, o.raw))
+    return failed("mncclGemmFp8", rc);
+  return Py_BuildValue("(NNNNN)", wrap(y), wrap(qx.qt), wrap(qx.scale_t), wrap(qw.qt), wrap(want_x ? qw.scale : at::Tensor()));
   END_HANDLE_TH_ERRORS
 }
 
-// distill_backward(rows, ids, p, stats, counts, tokens | None, tau, grad, d); tokens: what the gradient is divided by
+// linear_fp8_backward(grad [..., N], xt | None, xt_scale | None, wt | None, w_scale | None, K, want_bias) -> (dx [tokens, K] | None, dweight [N, K] | None,
+// dbias [N] | None); xt .. w_scale as the forward call gave them
+PyObject* linear_fp8_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 7)) return nullptr;
+  const at::Tensor *grad = tensor_arg(args[0], "grad"), *t[4] = {};
+  if (!grad) return nullptr;
+  for (int i = 0; i < 4; ++i)
+    if (args[i + 1] != Py_None && !(t[i] = tensor_arg(args[i + 1], "argument"))) return nullptr;
+  const int64_t K = PyLong_AsLongLong(args[5]);
+  if (PyErr_Occurred()) return nullptr;
+  const bool want_bias = args[6] == Py_True;
+  On o;
+  if (!on(*grad, Py_None, &o)) return nullptr;
+  const int64_t N = grad->size(-1);
+  int64_t ld = 0;
+  const at::Tensor g = rows_of(*grad, N, &ld);
+  const int64_t T = g.size(0);
+  const auto like = g.options().requires_grad(false);
+  Quantized q;
+  if (const int rc = quantize(g, ld, true, t[0] || want_bias, want_bias, o.raw, &q)) return failed("mncclQuantizeFp8", rc);
+  at::Tensor dx, dw, db;
+  if (t[2]) {
+    dx = at::empty({T, K}, like);
+    const at::Tensor &wt = *t[2], &ws = *t[3];   // rows of weight^T are columns of the weight
+    if (const int rc = product(q.q, q.scale, wt, ws, 1, ws.size(1), static_cast<int>(kBlock), T, K, N, dx, nullptr, o.raw)) return failed("mncclGemmFp8", rc);
+  }
+  if (t[0]) {
+    dw = at::empty({N, K}, like);
+    if (const int rc = product(q.qt, q.scale_t, *t[0], *t[1], 1, K, 1, N, K, T, dw, nullptr, o.raw)) return failed("mncclGemmFp8", rc);
+  }
+  if (want_bias) {
+    db = T > 0 ? at::empty({N}, like) : at::zeros({N}, like);
+    if (T > 0 && N > 0) {
+      int rc;
+      Py_BEGIN_ALLOW_THREADS
+      rc = lib.sum_blocks(q.sums.data_ptr<float>(), static_cast<int>(q.sums.size(0)), static_cast<int>(N), db.data_ptr(), float_code(db), o.raw);
+      Py_END_ALLOW_THREADS
+      if (rc != 0) return failed("mncclSumBlocks", rc);
+    }
+  }
+  return Py_BuildValue("(NNN)", wrap(dx), wrap(dw), wrap(db));
+  END_HANDLE_TH_ERRORS
+}
+
+// distill_forward(logits [..., V], ids [T, K], top [T, K], tau, reduction) -> (loss, p, stats, counts, tokens); reduction: 0 a loss for each row, 1 their
+// sum, 2 their mean.  ops/distill.py has checked the arguments
+PyObject* distill_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 5)) return nullptr;
+  const at::Tensor *logits = tensor_arg(args[0], "logits"), *ids = logits ? tensor_arg(args[1], "ids") : nullptr, *top = ids ? tensor_arg(args[2], "top") : nullptr;
+  if (!top) return nullptr;
+  const double tau = PyFloat_AsDouble(args[3]);
+  const long reduction = PyLong_AsLong(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  On o;
+  if (!on(*logits, Py_None, &o)) return nullptr;
+  const int64_t V = logits->size(-1);
+  int64_t ld = 0;
+  const at::Tensor rows = rows_of(*logits, V, &ld);
+  const int64_t T = rows.size(0), K = ids->size(1);
+  const auto f32 = rows.options().dtype(at::kFloat).requires_grad(false);
+  at::Tensor p = at::empty({T, K}, f32), stats = at::empty({T, 2}, f32), counts = at::empty({T}, f32.dtype(at::kInt)), tokens = at::empty({}, f32),
+             row_loss = at::empty(logits->sizes().slice(0, logits->dim() - 1), f32), loss = at::empty({}, f32);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = lib.distill_forward(rows.data_ptr(), float_code(rows), ld, static_cast<int>(T), static_cast<int>(V), ids->data_ptr<int64_t>(), top->data_ptr<float>(),
+                           static_cast<int>(K), static_cast<float>(tau), p.data_ptr<float>(), stats.data_ptr<float>(), row_loss.data_ptr<float>(),
+                           counts.data_ptr<int>(), reduction == 1 ? loss.data_ptr<float>() : nullptr, reduction == 2 ? loss.data_ptr<float>() : nullptr,
+                           tokens.data_ptr<float>(), o.raw);
+  Py_END_ALLOW_THREADS
+  if (rc != 0) return failed("mncclDistillForward", rc);
+  return Py_BuildValue("(NNNNN)", wrap(reduction == 0 ? row_loss : loss), wrap(p), wrap(stats), wrap(counts), wrap(tokens));
+  END_HANDLE_TH_ERRORS
+}
+
+// distill_backward(logits [..., V], ids, p, stats, counts, tokens | None, tau, grad) -> gradient of the logits, for a gradient of each row's loss or of
+// their sum; tokens: what it is divided by
 PyObject* distill_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arg_count(n, 9)) return nullptr;
-  const at::Tensor* t[9] = {};
-  for (int i = 0; i < 9; ++i) {
+  if (!arg_count(n, 8)) return nullptr;
+  const at::Tensor* t[8] = {};
+  for (int i = 0; i < 8; ++i) {
     if (i == 6 || (i == 5 && args[i] == Py_None)) continue;
     if (!(t[i] = tensor_arg(args[i], "argument"))) return nullptr;
   }
@@ -557,14 +670,21 @@ PyObject* distill_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   On o;
   if (!on(*t[0], Py_None, &o)) return nullptr;
+  const int64_t V = t[0]->size(-1);
+  int64_t ld = 0;
+  const at::Tensor rows = rows_of(*t[0], V, &ld), grad = t[7]->contiguous();
+  // the gradient's rows lie to 16 bytes as the logits' do: padded where those are
+  const int64_t T = rows.size(0), per = 16 / rows.element_size(), ldd = rows.stride(0) != V ? (V + per - 1) / per * per : V;
+  at::Tensor d = at::empty({T, ldd}, rows.options().requires_grad(false));
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = lib.distill_backward(t[0]->data_ptr(), float_code(*t[0]), row_stride(*t[0]), static_cast<int>(t[0]->size(0)), static_cast<int>(t[0]->size(1)), t[1]->data_ptr<int64_t>(),
-                            t[2]->data_ptr<float>(), static_cast<int>(t[1]->size(1)), static_cast<float>(tau), t[3]->data_ptr<float>(), t[4]->data_ptr<int>(),
-                            t[7]->data_ptr<float>(), t[7]->dim() > 0 ? 1 : 0, t[5] ? t[5]->data_ptr<float>() : nullptr, t[8]->data_ptr(), row_stride(*t[8]), o.raw);
+  rc = lib.distill_backward(rows.data_ptr(), float_code(rows), ld, static_cast<int>(T), static_cast<int>(V), t[1]->data_ptr<int64_t>(), t[2]->data_ptr<float>(),
+                            static_cast<int>(t[1]->size(1)), static_cast<float>(tau), t[3]->data_ptr<float>(), t[4]->data_ptr<int>(), grad.data_ptr<float>(),
+                            grad.dim() > 0 ? 1 : 0, t[5] ? t[5]->data_ptr<float>() : nullptr, d.data_ptr(), ldd, o.raw);
   Py_END_ALLOW_THREADS
   if (rc != 0) return failed("mncclDistillBackward", rc);
-  Py_RETURN_NONE;
+  if (ldd != V) d = d.slice(1, 0, V);
+  return wrap(t[0]->dim() == 2 ? d : d.view(t[0]->sizes()));
   END_HANDLE_TH_ERRORS
 }
 
@@ -582,6 +702,8 @@ PyMethodDef methods[] = {
     {"ag_gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(ag_gemm)), METH_FASTCALL, nullptr},
     {"quantize_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(quantize_fp8)), METH_FASTCALL, nullptr},
     {"gemm_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gemm_fp8)), METH_FASTCALL, nullptr},
+    {"linear_fp8_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear_fp8_forward)), METH_FASTCALL, nullptr},
+    {"linear_fp8_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear_fp8_backward)), METH_FASTCALL, nullptr},
     {"distill_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(distill_forward)), METH_FASTCALL, nullptr},
     {"distill_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(distill_backward)), METH_FASTCALL, nullptr},
     {"async_error", async_error, METH_O, nullptr},

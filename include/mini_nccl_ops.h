@@ -109,9 +109,11 @@ int mncclTransposeBf16(const void* src, int64_t lds, int rows, int cols, void* d
  * smallest with e >= -126 and 448 * 2^e >= its largest magnitude; q = x / scale, rounded to nearest even.  A block with an
  * infinity or a NaN becomes NaN.  Rows of q hold K rounded up to 16; the padding is written.  block_rows 1:
  * scale[K blocks][M]; 128: scale[M blocks][K blocks].  qt (may be null): the transpose [K, M], for block_rows 1 quantised
- * along M with scale_t[M blocks][K]; for 128 with the same scales (scale_t unused). */
+ * along M with scale_t[M blocks][K]; for 128 with the same scales (scale_t unused).  sums (may be null; only with qt and
+ * block_rows 1): [M blocks][K], the columns' sums over each 128 rows, which mncclSumBlocks adds up to out[K]. */
 int mncclQuantizeFp8(const void* x, int type, int64_t ldx, int M, int K, int block_rows, void* q, int64_t ldq, float* scale, void* qt,
-                     int64_t ldt, float* scale_t, cudaStream_t stream);
+                     int64_t ldt, float* scale_t, float* sums, cudaStream_t stream);
+int mncclSumBlocks(const float* sums, int blocks, int K, void* out, int type, cudaStream_t stream);
 /* C[M, N] = A[M, K] * B[N, K]^T (+ bias[N]) of e4m3 operands: the fp32 sum of each block of 128 along K times
  * sa[(m / sa_rows) * sa_row + block * sa_blk] and sb likewise (any fp32 scales), added in fp32 and rounded once.  C and
  * bias (null: none) are of `type`. */
@@ -123,11 +125,11 @@ int mncclGemmFp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, in
  * Student logits [T, V] of `type` (6, 7 or 9), row stride ld; ids and top [T, K], K <= 1024, tau in [1e-3, 1e3].  With
  * p = softmax(top / tau) over the entries whose id is not negative and whose logit is above -infinity, a token's loss is
  * tau^2 * sum p (log p - log softmax(logits / tau)[id]); tokens without entries count for nothing; an id of V or more makes
- * its token NaN.  Forward writes p [T, K], stats [T, 2] (8-byte aligned), counts [T] for the backward pass, row_loss [T] and
- * mean[3] = {sum, mean, tokens that count}.  Backward: d [T, V], the gradient of every token's loss times grad[t]
+ * its token NaN.  Forward writes p [T, K], stats [T, 2] (8-byte aligned), counts [T] and tokens[1] (how many count) for the
+ * backward pass, row_loss [T], sum and mean (either may be null).  Backward: d [T, V], the gradient of every token's loss times grad[t]
  * (grad_per_row) or grad[0], over tokens[0] if not null. */
 int mncclDistillForward(const void* logits, int type, int64_t ld, int T, int V, const int64_t* ids, const float* top, int K, float tau,
-                        float* p, float* stats, float* row_loss, int* counts, float* mean, cudaStream_t stream);
+                        float* p, float* stats, float* row_loss, int* counts, float* sum, float* mean, float* tokens, cudaStream_t stream);
 int mncclDistillBackward(const void* logits, int type, int64_t ld, int T, int V, const int64_t* ids, const float* p, int K, float tau,
                          const float* stats, const int* counts, const float* grad, int grad_per_row, const float* tokens, void* d,
                          int64_t ldd, cudaStream_t stream);

@@ -178,20 +178,26 @@ def _matrix(t, name, dtypes):
     return rows, cols, ld
 
 
-def quantize_fp8(lib, x, block_rows, transposed, stream):
+def _quantize(lib, x, block_rows, transposed, sums, s):
     M, K, ld = _matrix(x, "x", _FLOATS)
+    q = torch.empty((M, _padded(K)), dtype=_E4M3, device=x.device)
+    scale = torch.empty((_blocks(K), M) if block_rows == 1 else (_blocks(M), _blocks(K)), dtype=torch.float32, device=x.device)
+    qt = torch.empty((K, _padded(M)), dtype=_E4M3, device=x.device) if transposed else None
+    scale_t, sums = (torch.empty((_blocks(M), K), dtype=torch.float32, device=x.device) if want else None
+                     for want in (transposed and block_rows == 1, transposed and sums))
+    if M and K:
+        _check(lib.mncclQuantizeFp8(x.data_ptr(), _FLOATS[x.dtype], ld, M, K, block_rows, q.data_ptr(), q.shape[1], scale.data_ptr(),
+                                    qt.data_ptr() if transposed else None, qt.shape[1] if transposed else 0,
+                                    *(t.data_ptr() if t is not None else None for t in (scale_t, sums)), s), "mncclQuantizeFp8")
+    return q, scale, qt, scale_t, sums
+
+
+def quantize_fp8(lib, x, block_rows, transposed, stream):
+    _matrix(x, "x", _FLOATS)
     if block_rows not in (1, _BLOCK):
         raise ValueError("block_rows must be 1 or 128")
     with _on(x.device, stream) as s:
-        q = torch.empty((M, _padded(K)), dtype=_E4M3, device=x.device)
-        scale = torch.empty((_blocks(K), M) if block_rows == 1 else (_blocks(M), _blocks(K)), dtype=torch.float32, device=x.device)
-        qt = torch.empty((K, _padded(M)), dtype=_E4M3, device=x.device) if transposed else None
-        scale_t = torch.empty((_blocks(M), K), dtype=torch.float32, device=x.device) if transposed and block_rows == 1 else None
-        if M and K:
-            _check(lib.mncclQuantizeFp8(x.data_ptr(), _FLOATS[x.dtype], ld, M, K, block_rows, q.data_ptr(), q.shape[1], scale.data_ptr(),
-                                        qt.data_ptr() if transposed else None, qt.shape[1] if transposed else 0,
-                                        scale_t.data_ptr() if scale_t is not None else None, s), "mncclQuantizeFp8")
-    return q, scale, qt, scale_t
+        return _quantize(lib, x, block_rows, transposed, False, s)[:4]
 
 
 def _operand(t, name):
@@ -239,25 +245,63 @@ def gemm_fp8(lib, a, a_scale, b, b_scale, out, out_dtype, bias, stream):
     return out
 
 
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _rows(t, cols):
+    """``t [..., cols]`` as a matrix that the kernels can read (a copy only where the strides need one)."""
+    t = t.detach()
+    t = t if t.dim() == 2 else t.reshape(t.numel() // cols if cols else 0, cols)
+    return t if (cols <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= cols) else t.contiguous()
 
 
-def distill_forward(lib, rows, ids, top, tau):
+def linear_fp8_forward(lib, x, weight, bias, want_x, want_w):
+    N, K = weight.shape
+    rows, w = _rows(x, K), _rows(weight, K)
+    with _on(x.device, None) as s:
+        q, scale, qt, scale_t, _ = _quantize(lib, rows, 1, want_w, False, s)
+        wq, w_scale, wt, _, _ = _quantize(lib, w, _BLOCK, want_x, False, s)
+    y = gemm_fp8(lib, q[:, :K], scale.t(), wq[:, :K], w_scale, None, x.dtype, None if bias is None else bias.detach().contiguous(), None)
+    return y.view(*x.shape[:-1], N), qt, scale_t, wt, w_scale if want_x else None
+
+
+def linear_fp8_backward(lib, grad, xt, xt_scale, wt, w_scale, K, want_bias):
+    N = grad.shape[-1]
+    g = _rows(grad, N)
+    T = g.shape[0]
+    dx = dw = db = None
+    with _on(g.device, None) as s:
+        q, scale, qt, scale_t, sums = _quantize(lib, g, 1, xt is not None or want_bias, want_bias, s)
+        if want_bias:
+            db = torch.zeros(N, dtype=g.dtype, device=g.device)
+            if T and N:
+                _check(lib.mncclSumBlocks(sums.data_ptr(), sums.shape[0], N, db.data_ptr(), _FLOATS[db.dtype], s), "mncclSumBlocks")
+    if wt is not None:
+        dx = gemm_fp8(lib, q[:, :N], scale.t(), wt[:, :N], w_scale.t(), None, g.dtype, None, None)
+    if xt is not None:
+        dw = gemm_fp8(lib, qt[:, :T], scale_t.t(), xt[:, :T], xt_scale.t(), None, g.dtype, None, None)
+    return dx, dw, db
+
+
+def distill_forward(lib, logits, ids, top, tau, reduction):
+    rows = _rows(logits, logits.shape[-1])
     (T, V), K = rows.shape, ids.shape[1]
     with _on(rows.device, None) as s:
         empty = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=rows.device)  # noqa: E731
-        p, stats, counts, row_loss, mean = empty(T, K), empty(T, 2), empty(T, dtype=torch.int32), empty(T), empty(3)
-        _check(lib.mncclDistillForward(rows.data_ptr(), _FLOATS[rows.dtype], _row_stride(rows), T, V, ids.data_ptr(), top.data_ptr(), K, tau, p.data_ptr(),
-                                       stats.data_ptr(), row_loss.data_ptr(), counts.data_ptr(), mean.data_ptr(), s), "mncclDistillForward")
-    return p, stats, counts, row_loss, mean
+        p, stats, counts, row_loss, loss, tokens = empty(T, K), empty(T, 2), empty(T, dtype=torch.int32), empty(*logits.shape[:-1]), empty(), empty()
+        _check(lib.mncclDistillForward(rows.data_ptr(), _FLOATS[rows.dtype], rows.stride(0) if T > 1 else _padded(V), T, V, ids.data_ptr(), top.data_ptr(), K, tau,
+                                       p.data_ptr(), stats.data_ptr(), row_loss.data_ptr(), counts.data_ptr(), *(loss.data_ptr() if reduction == r else None for r in (1, 2)), tokens.data_ptr(), s),
+               "mncclDistillForward")
+    return row_loss if reduction == 0 else loss, p, stats, counts, tokens
 
 
-def distill_backward(lib, rows, ids, p, stats, counts, tokens, tau, grad, d):
+def distill_backward(lib, logits, ids, p, stats, counts, tokens, tau, grad):
+    rows, grad = _rows(logits, logits.shape[-1]), grad.contiguous()
+    T, V = rows.shape
+    per = 16 // rows.element_size()
     with _on(rows.device, None) as s:
-        _check(lib.mncclDistillBackward(rows.data_ptr(), _FLOATS[rows.dtype], _row_stride(rows), *rows.shape, ids.data_ptr(), p.data_ptr(), ids.shape[1], tau,
-                                        stats.data_ptr(), counts.data_ptr(), grad.data_ptr(), 1 if grad.dim() else 0,
-                                        tokens.data_ptr() if tokens is not None else None, d.data_ptr(), _row_stride(d), s), "mncclDistillBackward")
+        d = torch.empty((T, -(-V // per) * per if rows.stride(0) != V else V), dtype=rows.dtype, device=rows.device)
+        _check(lib.mncclDistillBackward(rows.data_ptr(), _FLOATS[rows.dtype], rows.stride(0) if T > 1 else _padded(V), T, V, ids.data_ptr(), p.data_ptr(), ids.shape[1],
+                                        tau, stats.data_ptr(), counts.data_ptr(), grad.data_ptr(), 1 if grad.dim() else 0,
+                                        tokens.data_ptr() if tokens is not None else None, d.data_ptr(), d.shape[1], s), "mncclDistillBackward")
+    return d[:, :V].view(logits.shape)
 
 
 class Calls:
@@ -266,5 +310,6 @@ class Calls:
     def __init__(self, lib):
         from functools import partial
 
-        for f in (all_reduce, gemm, gemm_rs, ag_gemm, quantize_fp8, gemm_fp8, distill_forward, distill_backward):
+        for f in (all_reduce, gemm, gemm_rs, ag_gemm, quantize_fp8, gemm_fp8, linear_fp8_forward, linear_fp8_backward,
+                  distill_forward, distill_backward):
             setattr(self, f.__name__, partial(f, lib))

@@ -111,12 +111,13 @@ def lib() -> C.CDLL:
         sig("mncclLmLossBackward", i32, vp, C.c_int64, i32, i32, vp, vp, vp, vp, vp, C.c_int64, vp, C.c_int64, vp)
         sig("mncclTransposeBf16", i32, vp, C.c_int64, i32, i32, vp, C.c_int64, vp)
     if hasattr(L, "mncclQuantizeFp8"):
-        sig("mncclQuantizeFp8", i32, vp, i32, C.c_int64, i32, i32, i32, vp, C.c_int64, vp, vp, C.c_int64, vp, vp)
+        sig("mncclQuantizeFp8", i32, vp, i32, C.c_int64, i32, i32, i32, vp, C.c_int64, vp, vp, C.c_int64, vp, vp, vp)
+        sig("mncclSumBlocks", i32, vp, i32, i32, vp, i32, vp)
     if hasattr(L, "mncclGemmFp8"):
         sig("mncclGemmFp8", i32, vp, C.c_int64, vp, C.c_int64, C.c_int64, i32, vp, C.c_int64, vp, C.c_int64, C.c_int64, i32, vp, C.c_int64, i32,
             vp, i32, i32, i32, vp)
     if hasattr(L, "mncclDistillForward"):
-        sig("mncclDistillForward", i32, vp, i32, C.c_int64, i32, i32, vp, vp, i32, C.c_float, vp, vp, vp, vp, vp, vp)
+        sig("mncclDistillForward", i32, vp, i32, C.c_int64, i32, i32, vp, vp, i32, C.c_float, vp, vp, vp, vp, vp, vp, vp, vp)
         sig("mncclDistillBackward", i32, vp, i32, C.c_int64, i32, i32, vp, vp, i32, C.c_float, vp, vp, vp, i32, vp, vp, C.c_int64, vp)
     if hasattr(L, "mncclGemmReduceScatterBf16"):
         sig("mncclGemmRsStageBytes", sz, i32, i32, i32)
@@ -236,7 +237,7 @@ def ext():
     address = lambda name: C.cast(getattr(L, name), C.c_void_p).value if hasattr(L, name) else 0
     _torch_ext.bind(address("mncclAllReduceEx"), address("mncclCommGetAsyncError"), address("mncclGemmBf16"),
                     address("mncclGemmReduceScatterBf16Comm"), address("mncclAllGatherGemmBf16Comm"), address("mncclQuantizeFp8"),
-                    address("mncclGemmFp8"), address("mncclDistillForward"), address("mncclDistillBackward"))
+                    address("mncclSumBlocks"), address("mncclGemmFp8"), address("mncclDistillForward"), address("mncclDistillBackward"))
     _EXT = _torch_ext
     return _EXT
 

@@ -16,7 +16,7 @@ from .lm_loss import _MAX_ROWS, _eight, _pays, _plain, _transposed
 from .lm_loss import _rows as _dense_rows
 
 _MAX_ENTRIES = 1024   # mncclDistillForward
-_REDUCTIONS = ("mean", "sum", "none")
+_REDUCTIONS = ("none", "sum", "mean")
 
 
 def _reference(logits, ids, top, tau, reduction):
@@ -38,25 +38,14 @@ def _reference(logits, ids, top, tau, reduction):
     return rows.sum() if reduction == "sum" else rows.sum() / counts.sum()
 
 
-def _forward(rows, ids, top, tau):
-    """(p, stats, counts, loss of each row, {sum, mean, tokens that count}): the first three for the backward pass."""
-    return _call("distill_forward", "mncclDistillForward", "csrc/kernels/distill.cu")(rows, ids, top, tau)
+def _forward(logits, ids, top, tau, reduction):
+    """(loss, p, stats, counts, tokens): all but the first for the backward pass."""
+    return _call("distill_forward", "mncclDistillForward", "csrc/kernels/distill.cu")(logits, ids, top, tau, _REDUCTIONS.index(reduction))
 
 
-def _backward(rows, ids, p, stats, counts, mean, tau, reduction, grad, d):
-    _call("distill_backward", "mncclDistillBackward", "csrc/kernels/distill.cu")(rows, ids, p, stats, counts, mean[2:] if reduction == "mean" else None,
-                                                                                 tau, (grad.reshape(-1) if reduction == "none" else grad).contiguous(), d)
-
-
-def _logit_rows(logits):
-    """``logits [..., V]`` as a matrix with a unit inner stride (a copy only where the strides need one)."""
-    V = logits.shape[-1]
-    rows = logits.detach().reshape(-1, V)
-    return rows if (V == 1 or rows.stride(1) == 1) and (rows.shape[0] == 1 or rows.stride(0) >= V) else rows.contiguous()
-
-
-def _reduced(row_loss, mean, reduction, shape):
-    return row_loss.view(shape) if reduction == "none" else mean[0 if reduction == "sum" else 1].clone()
+def _backward(logits, ids, p, stats, counts, tokens, tau, reduction, grad):
+    return _call("distill_backward", "mncclDistillBackward", "csrc/kernels/distill.cu")(logits, ids, p, stats, counts, tokens if reduction == "mean" else None,
+                                                                                        tau, grad)
 
 
 def _again(ctx, inputs, f, grad):
@@ -71,28 +60,19 @@ def _again(ctx, inputs, f, grad):
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, top, tau, reduction):
-        rows = _logit_rows(logits)
-        p, stats, counts, row_loss, mean = _forward(rows, ids, top, tau)
-        ctx.save_for_backward(logits, ids, top, p, stats, counts, mean)
+        loss, *kept = _forward(logits, ids, top, tau, reduction)
+        ctx.save_for_backward(logits, ids, top, *kept)
         ctx.tau, ctx.reduction = tau, reduction
-        return _reduced(row_loss, mean, reduction, logits.shape[:-1])
+        return loss
 
     @staticmethod
     def backward(ctx, grad):
-        logits, ids, top, p, stats, counts, mean = ctx.saved_tensors
+        logits, ids, top, *kept = ctx.saved_tensors
         none = (None,) * 4
         if torch.is_grad_enabled():
             at = ids.view(*logits.shape[:-1], -1), top.view(*logits.shape[:-1], -1)
             return (*_again(ctx, [logits], lambda z: _reference(z, *at, ctx.tau, ctx.reduction), grad), *none)
-        rows, V = _logit_rows(logits), logits.shape[-1]
-        # rows of the gradient lie to 16 bytes as the logits' do: padded where those are
-        wide = V
-        if rows.shape[0] > 1 and rows.stride(0) != V:
-            per = 16 // rows.element_size()
-            wide = -(-V // per) * per
-        d = torch.empty((rows.shape[0], wide), dtype=rows.dtype, device=rows.device)[:, :V]
-        _backward(rows, ids, p, stats, counts, mean, ctx.tau, ctx.reduction, grad, d)
-        return (d.view(logits.shape), *none)
+        return (_backward(logits, ids, *kept, ctx.tau, ctx.reduction, grad), *none)
 
 
 class _LmHeadDistillation(torch.autograd.Function):
@@ -102,14 +82,14 @@ class _LmHeadDistillation(torch.autograd.Function):
         rows, w = _dense_rows(x.detach()).view(-1, x.shape[-1]), _dense_rows(weight.detach())
         logits = torch.empty((rows.shape[0], _eight(V)), dtype=x.dtype, device=x.device)
         gemm_bf16(rows, w, out=logits[:, :V])
-        p, stats, counts, row_loss, mean = _forward(logits[:, :V], ids, top, tau)
-        ctx.save_for_backward(x, weight, ids, top, logits, p, stats, counts, mean)
+        loss, *kept = _forward(logits[:, :V], ids, top, tau, "mean")
+        ctx.save_for_backward(x, weight, ids, top, logits, *kept)
         ctx.tau = tau
-        return mean[1].clone()
+        return loss
 
     @staticmethod
     def backward(ctx, grad):
-        x, weight, ids, top, logits, p, stats, counts, mean = ctx.saved_tensors
+        x, weight, ids, top, logits, *kept = ctx.saved_tensors
         want_x, want_w = ctx.needs_input_grad[:2]
         if torch.is_grad_enabled():
             at = ids.view(*x.shape[:-1], -1), top.view(*x.shape[:-1], -1)
@@ -117,8 +97,7 @@ class _LmHeadDistillation(torch.autograd.Function):
         stream = torch.cuda.current_stream().cuda_stream
         V = weight.shape[0]
         rows, logits = _dense_rows(x).view(-1, x.shape[-1]), _dense_rows(logits)
-        d = torch.empty((rows.shape[0], _eight(V)), dtype=x.dtype, device=x.device)[:, :V]
-        _backward(logits[:, :V], ids, p, stats, counts, mean, ctx.tau, "mean", grad, d)
+        d = _backward(logits[:, :V], ids, *kept, ctx.tau, "mean", grad)   # in padded rows, as the logits
         dx = dw = None
         if want_x and V % 8 == 0:
             dx = gemm_bf16(d, _transposed(_dense_rows(weight), stream)).view(x.shape)
@@ -141,7 +120,11 @@ def _native(logits, ids, top):
         return False
     if not (0 < ids.shape[-1] <= _MAX_ENTRIES and 0 < ids[..., 0].numel() < 2**31 and 0 < logits.shape[-1] < 2**31 - 2**12) or not _plain_call():
         return False
-    return torch.autograd.forward_ad.unpack_dual(logits).tangent is None
+    return _no_tangent(logits)
+
+
+def _no_tangent(t):
+    return torch.autograd.forward_ad._current_level < 0 or torch.autograd.forward_ad.unpack_dual(t).tangent is None
 
 
 def _arguments(shape, device, ids, top, temperature, reduction="mean"):
@@ -193,7 +176,7 @@ def lm_head_distillation(x, weight, top_ids, top_logits, temperature=1.0):
     native = (x.dim() >= 2 and x.dtype == weight.dtype == torch.bfloat16 and x.device == weight.device and _plain(x) and _plain(weight)
               and x.is_cuda and x.device.index == torch.cuda.current_device() and V >= 8 and d >= 8 and d % 8 == 0 and 0 < T
               and max(T, V) <= _MAX_ROWS and not torch.is_autocast_enabled() and _native(x, ids, top)
-              and torch.autograd.forward_ad.unpack_dual(weight).tangent is None)
+              and _no_tangent(weight))
     if not native or not _pays(T, V, d):
         return distillation_loss(F.linear(x, weight), ids, top, tau)
     K = ids.shape[-1]

@@ -54,41 +54,20 @@ def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=None, bias=None, stream
     return _call("gemm_fp8", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")(a, a_scale, b, b_scale, out, out_dtype, bias, stream)
 
 
-def _rows(t, cols):
-    """``t [..., cols]`` as a matrix that the quantisation reads (a copy only where the strides need one)."""
-    t = t.detach().reshape(-1, cols)
-    return t if (cols <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= cols) else t.contiguous()
-
-
 class _LinearFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        N, K = weight.shape
         want_x, want_w = ctx.needs_input_grad[:2]
-        rows = _rows(x, K)
-        q, scale, qt, scale_t = _quantize(rows, 1, want_w)
-        w, w_scale, wt, _ = _quantize(_rows(weight, K), BLOCK, want_x)
-        y = gemm_fp8(q[:, :K], scale.t(), w[:, :K], w_scale, out_dtype=x.dtype, bias=None if bias is None else bias.detach().contiguous())
-        # the padded buffers: a saved-tensor hook may hand back a dense copy of what it is given
-        ctx.save_for_backward(qt, scale_t, wt, w_scale if want_x else None)
-        ctx.shape, ctx.sizes = x.shape, (rows.shape[0], N, K)
-        return y.view(*x.shape[:-1], N)
+        y, *kept = _call("linear_fp8_forward", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")(x, weight, bias, want_x, want_w)
+        ctx.save_for_backward(*kept)
+        ctx.shape = x.shape
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        xt, xt_scale, wt, w_scale = ctx.saved_tensors
-        want_x, want_w, want_b = ctx.needs_input_grad
-        T, N, K = ctx.sizes
-        g = _rows(grad, N)
-        dx = dw = None
-        if want_x or want_w:
-            q, scale, qt, scale_t = _quantize(g, 1, want_w)
-        if want_x:
-            dx = gemm_fp8(q[:, :N], scale.t(), wt[:, :N], w_scale.t(), out_dtype=grad.dtype).view(ctx.shape)
-        if want_w:
-            dw = gemm_fp8(qt[:, :T], scale_t.t(), xt[:, :T], xt_scale.t(), out_dtype=grad.dtype)
-        return dx, dw, g.float().sum(0).to(grad.dtype) if want_b else None
+        dx, dw, db = _calls["linear_fp8_backward"](grad, *ctx.saved_tensors, ctx.shape[-1], ctx.needs_input_grad[2])
+        return None if dx is None else dx.view(ctx.shape), dw, db
 
 
 def linear_fp8(x, weight, bias=None):
@@ -112,4 +91,5 @@ def linear_fp8(x, weight, bias=None):
         raise ValueError("shapes: x [..., K], weight [N, K], bias [N]")
     if weight.shape[1] == 0:
         raise ValueError("a layer without input features")
+    _call("linear_fp8_backward", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")
     return _LinearFp8.apply(x, weight, bias)

@@ -351,14 +351,30 @@ def test_calls_through_ctypes_do_the_same():
             assert (p is None) == (q is None) and (p is None or (p.shape == q.shape and torch.equal(p[:, :64].float(), q[:, :64].float())))
     args = (*quantize_fp8(x), *quantize_fp8(w, block_rows=128))
     assert torch.equal(plain.gemm_fp8(*args, None, torch.float16, bias, None), ext.gemm_fp8(*args, None, torch.float16, bias, None))
-    rows, ids, top = torch.randn(5, 1000, device="cuda"), torch.randint(-1, 1000, (5, 7), device="cuda"), torch.randn(5, 7, device="cuda")
-    grads = []
-    for c in (plain, ext):
-        p, stats, counts, row_loss, mean = c.distill_forward(rows, ids, top, 2.0)
-        d = torch.zeros_like(rows)
-        c.distill_backward(rows, ids, p, stats, counts, mean[2:], 2.0, torch.ones((), device="cuda"), d)
-        grads.append((row_loss, mean, d))
-    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    for lead in ((), (5,), (2, 3)):
+        for wide in (1000, 1008):
+            logits = torch.randn(*lead, wide, device="cuda")[..., :1000]
+            n = logits.numel() // 1000
+            ids, top = torch.randint(-1, 1000, (n, 7), device="cuda"), torch.randn(n, 7, device="cuda")
+            ids[0, 0] = 3
+            for reduction in (0, 1, 2):
+                results = []
+                for c in (plain, ext):
+                    loss, p, stats, counts, tokens = c.distill_forward(logits, ids, top, 2.0, reduction)
+                    results.append((loss, p, tokens, c.distill_backward(logits, ids, p, stats, counts, tokens if reduction == 2 else None, 2.0, torch.ones_like(loss))))
+                assert all(torch.equal(a, b) and a.shape == b.shape and a.stride() == b.stride() for a, b in zip(*results))
+                assert results[0][0].shape == (lead if reduction == 0 else ()) and results[0][3].shape == logits.shape
+    for dtype in TYPES:
+        x, w, b = _input(30, 200, dtype, 3).view(3, 10, 200).cuda(), _input(130, 200, dtype, 4).cuda(), _input(1, 130, dtype, 5)[0].cuda()
+        grad = _input(30, 130, dtype, 6).view(3, 10, 130).cuda()
+        for want_x, want_w, bias in ((True, True, b), (True, False, None), (False, True, b), (False, False, b)):
+            results = []
+            for c in (plain, ext):
+                y, *kept = c.linear_fp8_forward(x, w, bias, want_x, want_w)
+                results.append((y, *c.linear_fp8_backward(grad, *kept, 200, bias is not None)))
+            assert all((a is None) == (q is None) and (a is None or torch.equal(a, q)) for a, q in zip(*results))
+            assert [r is not None for r in results[0][1:]] == [want_x, want_w, bias is not None]
+    x = _input(70, 300, torch.bfloat16).cuda()
     for bad, error in ((lambda c: c.quantize_fp8(x.double(), 1, False, None), TypeError), (lambda c: c.quantize_fp8([1], 1, False, None), TypeError),
                        (lambda c: c.quantize_fp8(x, 2, False, None), ValueError), (lambda c: c.gemm_fp8(*args, None, torch.int8, None, None), TypeError),
                        (lambda c: c.gemm_fp8(*args, None, None, bias[:3], None), ValueError), (lambda c: c.gemm_fp8(args[0], args[0], *args[2:], None, None, None, None), TypeError)):
@@ -375,13 +391,14 @@ def test_entry_points_refuse_bad_arguments():
 
     L = mn.lib()
     p = C.c_void_p(4096)   # never looked at: every call below is refused before anything is launched
-    q = [p, 9, 128, 4, 128, 1, p, 128, p, None, 0, None, None]
+    q = [p, 9, 128, 4, 128, 1, p, 128, p, None, 0, None, None, None]
     for at, value, code in ((0, None, -1), (6, None, -1), (8, None, -1), (3, 0, -1), (4, -1, -1), (1, 3, -2), (2, 64, -2), (5, 2, -2), (6, C.c_void_p(4097), -2), (7, 120, -2),
-                            (7, 112, -2), (4, 65536 * 128, -2)):
+                            (7, 112, -2), (4, 65536 * 128, -2), (12, p, -2)):
         bad = list(q)
         bad[at] = value
         assert L.mncclQuantizeFp8(*bad) == code, (at, value)
-    assert L.mncclQuantizeFp8(*q[:9], p, 16, None, None) == -1 and L.mncclQuantizeFp8(*q[:9], p, 8, p, None) == -2
+    assert L.mncclQuantizeFp8(*q[:9], p, 16, None, None, None) == -1 and L.mncclQuantizeFp8(*q[:9], p, 8, p, None, None) == -2
+    assert L.mncclSumBlocks(None, 1, 8, p, 9, None) == -1 and L.mncclSumBlocks(p, 0, 8, p, 9, None) == -1 and L.mncclSumBlocks(p, 1, 8, p, 8, None) == -2
     g = [p, 128, p, 1, 4, 1, p, 128, p, 1, 1, 128, p, 64, 9, None, 4, 64, 128, None]
     for at, value, code in ((0, None, -1), (2, None, -1), (6, None, -1), (8, None, -1), (12, None, -1), (16, 0, -1), (17, 0, -1), (18, -5, -1), (0, C.c_void_p(4100), -2), (1, 120, -2),
                             (7, 112, -2), (5, 64, -2), (11, 0, -2), (13, 63, -2), (14, 8, -2)):
