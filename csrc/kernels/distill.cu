@@ -75,6 +75,23 @@ struct Running {
   }
 };
 
+// The largest of N elements and `highest`; 16-bit types two at a time.
+template <typename T, int N>
+__device__ __forceinline__ float highest_of(const T (&x)[N], float highest) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) highest = fmaxf(highest, x[j]);
+    return highest;
+  } else {
+    using Two = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const Two* two = reinterpret_cast<const Two*>(x);
+    Two top = two[0];
+#pragma unroll
+    for (int j = 1; j < N / 2; ++j) top = __hmax2(top, two[j]);
+    return fmaxf(highest, fmaxf(as_float(top.x), as_float(top.y)));
+  }
+}
+
 __device__ __forceinline__ float warp_max(float x) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
@@ -111,7 +128,7 @@ __device__ __forceinline__ float block_sum(float x, float* box) {
 // {max, sum}, row_loss[t] and counts[t].  PER: teacher's entries a thread holds.  They and the student's logits at their ids are fetched before
 // the row is read, so that the end of a block does not wait for memory again.
 template <typename T, int PER>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, PER == 1 ? 5 : 3)
 distill_rows_kernel(const T* __restrict__ logits, size_t ld, int V, const int64_t* __restrict__ ids, const float* __restrict__ top, int K,
                     float tau, int parts, float* __restrict__ p, float2* __restrict__ stats, float* __restrict__ row_loss, int* __restrict__ counts) {
   __shared__ float box[2][kThreads / 32];
@@ -128,7 +145,8 @@ distill_rows_kernel(const T* __restrict__ logits, size_t ld, int V, const int64_
   for (int i = 0; i < PER; ++i) {
     const int k = static_cast<int>(threadIdx.x) + i * kThreads;
     const int64_t id = k < K ? ids[t * K + k] : -1;
-    teacher[i] = id >= 0 ? top[t * K + k] : -INFINITY;
+    const float logit = k < K ? top[t * K + k] : -INFINITY;
+    teacher[i] = id >= 0 ? logit : -INFINITY;
     const bool there = teacher[i] != -INFINITY;
     any = any || there;
     bad = bad || (there && id >= V);
@@ -159,9 +177,7 @@ distill_rows_kernel(const T* __restrict__ logits, size_t ld, int V, const int64_
     for (int b = 0; b < kBatch; ++b) u[b].raw = __ldg(body + v + b * kThreads);
     float highest = r.m;
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) highest = fmaxf(highest, as_float(u[b].x[j]));
+    for (int b = 0; b < kBatch; ++b) highest = highest_of(u[b].x, highest);
     r.raise(highest, c);
     const float base = Running::base(r.m);
 #pragma unroll
@@ -172,10 +188,7 @@ distill_rows_kernel(const T* __restrict__ logits, size_t ld, int V, const int64_
   for (; v < last; v += kThreads) {
     union { uint4 raw; T x[kVec]; } u;
     u.raw = __ldg(body + v);
-    float highest = r.m;
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) highest = fmaxf(highest, as_float(u.x[j]));
-    r.raise(highest, c);
+    r.raise(highest_of(u.x, r.m), c);
     const float base = Running::base(r.m);
 #pragma unroll
     for (int j = 0; j < kVec; ++j) r.s += exp2_fast((as_float(u.x[j]) - base) * c);
