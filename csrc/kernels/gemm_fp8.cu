@@ -460,32 +460,51 @@ bool make_tensor_map_out(CUtensorMap* map, const Args& g) {
                                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The tile width that needs the fewest waves times (columns + 256): a narrower tile pays where it saves a wave.
-int pick_width(int M, int N, int pairs, long* cost) {
+// The tile width with the least estimated time (ns): a wave of tiles takes about a microsecond and so much a block of K (measured: 8192 x 4096 x 1024, seven
+// waves of 256, 41 us; 512 x 4096 x 4096, one wave of 128, 15.8 us; 4096 x 4096 x 4096, four of 256, 67 us, and 101 with a scale for every row of
+// B).  A narrower tile pays where it saves a wave or leaves fewer SMs idle.
+int pick_width(int M, int N, int K, bool b_rows, int pairs, long* ns) {
+  struct Width {
+    int bn;
+    long per_block, per_block_rows;
+  };
+  constexpr Width kWidths[] = {{256, 480, 740}, {192, 400, 580}, {128, 310, 420}};
+  const long num_kb = (K + kBlockK - 1) / kBlockK;
   int best = 256;
-  *cost = -1;
-  for (const int bn : {256, 192, 128}) {
-    const long tiles = static_cast<long>((M + 255) / 256) * ((N + bn - 1) / bn), c = (tiles + pairs - 1) / pairs * (bn + 64);
-    if (*cost < 0 || c < *cost) {
-      *cost = c;
-      best = bn;
+  *ns = -1;
+  for (const Width& w : kWidths) {
+    const long tiles = static_cast<long>((M + 255) / 256) * ((N + w.bn - 1) / w.bn), waves = (tiles + pairs - 1) / pairs;
+    const long t = 5000 + waves * (1000 + num_kb * (b_rows ? w.per_block_rows : w.per_block));
+    if (*ns < 0 || t < *ns) {
+      *ns = t;
+      best = w.bn;
     }
   }
   return best;
+}
+
+struct Plan {
+  bool small;
+  SmallPlan p;
+  int bn;   // pairs: tile width
+};
+Plan make_plan(int M, int N, int K, bool b_rows, int sms) {
+  Plan plan{};
+  long pair_ns = 0, small_ns = 0;
+  plan.bn = pick_width(M, N, K, b_rows, sms / 2, &pair_ns);
+  plan.small = plan_small(M, N, K, sms, &plan.p, &small_ns) && small_ns < pair_ns;
+  return plan;
 }
 
 int run(const void* a, int64_t lda, const void* b, int64_t ldb, Args g, cudaStream_t stream) {
   std::string why;
   g.err = error_word();
   g.wait_budget_ns = 2000000000ull;
-  const int sms = sm_count();
-  long cost = 0, small_ns = 0;
-  const int bn = pick_width(g.M, g.N, sms / 2, &cost);
-  const long num_kb = (g.K + kBlockK - 1) / kBlockK, pair_ns = 6000 + cost * num_kb * 300 / 320;
-  SmallPlan p;
+  const Plan plan = make_plan(g.M, g.N, g.K, g.b.shift == 0, sm_count());
+  const int bn = plan.bn;
   cudaError_t e;
-  if (plan_small(g.M, g.N, g.K, sms, &p, &small_ns) && small_ns < pair_ns) {
-    e = launch_small(a, lda, b, ldb, g, p, stream, &why);
+  if (plan.small) {
+    e = launch_small(a, lda, b, ldb, g, plan.p, stream, &why);
   } else {
     const long tiles = static_cast<long>((g.M + 255) / 256) * ((g.N + bn - 1) / bn);
     if (tiles > 0x7fffffff / 2) return -2;
@@ -547,6 +566,17 @@ MNCCL_EXPORT int mncclGemmFp8(const void* a, int64_t lda, const float* sa, int64
   } catch (...) {   // out of host memory for a message
     return -3;
   }
+}
+
+// The kernel that an M x N x K product takes on `sms` SMs: returns 1 for the one for few rows or tiles (tile = rows of A per tile, slices = CTAs that
+// share a tile's K), 0 for CTA pairs (tile = columns, slices = 1).  b_rows: rows of a scale of B.  Host arithmetic only (needs no GPU).
+MNCCL_EXPORT int mncclGemmFp8Plan(int M, int N, int K, int b_rows, int sms, int* tile, int* slices) {
+  using namespace mnccl::gemm::fp8;
+  if (M <= 0 || N <= 0 || K <= 0 || sms < 2 || (b_rows != 1 && b_rows != 128)) return -1;
+  const Plan plan = make_plan(M, N, K, b_rows == 1, sms);
+  if (tile) *tile = plan.small ? plan.p.tn : plan.bn;
+  if (slices) *slices = plan.small ? plan.p.slices : 1;
+  return plan.small ? 1 : 0;
 }
 
 }  // extern "C"

@@ -186,11 +186,11 @@ __device__ __forceinline__ T round_to(float x) {
 bool make_tensor_map_e4m3(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t row_stride, uint32_t box_rows, std::string* why);
 
 struct SmallPlan {
-  int tn = 0;            // rows of A per tile: 16, 32, 64 or 128
+  int tn = 0;            // rows of A per tile: 16, 32 or 64
   int slices = 1;        // CTAs of a cluster that share a tile's K
   int kb_per_slice = 0;
   int tiles = 0;
-  bool deep = true;      // one CTA per SM with the whole shared memory as its ring, or two
+  bool deep = false;     // one CTA per SM with the whole shared memory as its ring, or two
 };
 bool plan_small(int M, int N, int K, int sms, SmallPlan* p, long* ns);
 cudaError_t launch_small(const void* a, int64_t lda, const void* b, int64_t ldb, const Args& g, const SmallPlan& p, cudaStream_t stream, std::string* why);

@@ -81,7 +81,7 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   extern __shared__ uint8_t smem_raw[];
   constexpr int NB = kBuffers<TN>, W = kWarps<TN>, NC = kCols<TN>;
   constexpr int KPS = kPerStage<TN>, U = kUnit<TN>;
-  constexpr uint32_t kTmem = NB * U * TN;   // 128, 128, 256, 512 columns
+  constexpr uint32_t kTmem = NB * U * TN;   // 128, 128, 256 columns
   static_assert(U % KPS == 0 && kGroup % U == 0, "a unit is whole stages, a group of scales whole units");
   static_assert(NS <= kMostStages && (NB & (NB - 1)) == 0, "ring depth");
   const Args& g = args.g;
@@ -345,23 +345,39 @@ int per_slice(int num_kb, int slices, int tn) {
   return (stages + slices - 1) / slices * per_stage;
 }
 
-// Fewest CTAs' worth of K while SMs are idle: slices are doubled as long as all CTAs still run at once.
+// The plan with the least estimated time (ns).  Measured on 148 SMs, operands not in L2 (M x N x K, tile's rows of A / slices):
+//   1 x 4096 x 4096      16 / 4: 8.2 us, 16 / 8: 8.6, 16 / 2: 9.6          64 x 14336 x 4096   64 / 1: 20.2 us, 32 / 1: 23.1, pairs: 21.2
+//   16 x 4096 x 14336    16 / 8: 14.7 us, 16 / 4: 15.3, 16 / 2: 19.5       128 x 4096 x 4096   64 / 2: 15.1 us, 32 / 1: 16.8, pairs: 16.8
+//   256 x 1024 x 1024    16 / 1: 6.9 us, 64 / 4: 7.7, pairs: 7.8           256 x 4096 x 4096   64 / 1: 18.9 us, pairs: 16.4
+// So a tile takes a fixed time and one per block of K that grows with its width; a second CTA on an SM takes as long again, except where
+// memory is what all wait for; and nothing is faster than the operands come from memory.  Tiles of 128 rows of A never won (128 x 4096 x
+// 4096: 16.4 us).  A tile that has its K and its SM to itself takes all of the shared memory as its ring (16 x 14336 x 4096: 16.9 -> 15.5 us);
+// slices do better with half, which lets the next wave's CTAs in early (1 x 4096 x 4096: 9.0 -> 8.2 us).
 bool plan_small(int M, int N, int K, int sms, SmallPlan* p, long* ns) {
+  struct Cost {
+    int tn;
+    long fixed, per_block, split;   // a tile; a block of K; the meeting of the slices
+  };
+  constexpr Cost kCost[] = {{16, 4500, 270, 1300}, {32, 4700, 360, 1800}, {64, 5200, 490, 2200}};
   const int num_kb = (K + kBlockK - 1) / kBlockK;
-  const long tiles_n = (N + 127) / 128;
-  p->tn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  const long tiles = tiles_n * ((M + p->tn - 1) / p->tn);
-  if (tiles > (1 << 24)) return false;
-  p->tiles = static_cast<int>(tiles);
-  p->slices = 1;
-  while (p->slices < 8 && tiles * p->slices * 2 <= sms && num_kb >= p->slices * 4) p->slices *= 2;
-  p->kb_per_slice = per_slice(num_kb, p->slices, p->tn);
-  while ((p->slices - 1) * p->kb_per_slice >= num_kb) {   // a slice would be empty
-    p->slices /= 2;
-    p->kb_per_slice = per_slice(num_kb, p->slices, p->tn);
+  const long tiles_n = (N + 127) / 128, floor_ns = 4500 + static_cast<long>((static_cast<double>(K) * (static_cast<double>(M) + N) + 2.0 * M * N) / 5800.0);
+  *ns = -1;
+  for (const Cost& c : kCost) {
+    const long tiles = tiles_n * ((M + c.tn - 1) / c.tn);
+    if (tiles > (1 << 20)) continue;
+    for (int slices = 1; slices <= 8; slices *= 2) {
+      const int per = per_slice(num_kb, slices, c.tn);
+      const long items = tiles * slices;
+      if ((slices - 1) * per >= num_kb || (slices > 1 && items > 2L * sms)) break;   // a slice would be empty, or CTAs wait for others
+      const long rounds = (items + sms - 1) / sms, fixed = c.fixed + (slices > 1 ? c.split : 0) + (slices > 4 ? 1500 : 0);
+      const long t = std::max(fixed + rounds * std::min(per, num_kb) * c.per_block, floor_ns + (items > sms ? 300 : 0));
+      if (*ns < 0 || t < *ns) {
+        *ns = t;
+        *p = SmallPlan{c.tn, slices, per, static_cast<int>(tiles), slices == 1 && items <= sms};
+      }
+    }
   }
-  *ns = 5000 + ((tiles * p->slices + sms - 1) / sms) * p->kb_per_slice * (p->tn == 128 ? 300 : 200);
-  return true;
+  return *ns > 0;
 }
 
 cudaError_t launch_small(const void* a, int64_t lda, const void* b, int64_t ldb, const Args& g, const SmallPlan& p, cudaStream_t stream, std::string* why) {
@@ -373,7 +389,6 @@ cudaError_t launch_small(const void* a, int64_t lda, const void* b, int64_t ldb,
     case 16: return p.deep ? fire<16, 5>(tw, tx, s, p, stream) : fire<16, 2>(tw, tx, s, p, stream);
     case 32: return p.deep ? fire<32, 5>(tw, tx, s, p, stream) : fire<32, 2>(tw, tx, s, p, stream);
     case 64: return p.deep ? fire<64, 8>(tw, tx, s, p, stream) : fire<64, 4>(tw, tx, s, p, stream);
-    case 128: return fire<128, 6>(tw, tx, s, p, stream);
   }
   return cudaErrorInvalidValue;
 }
