@@ -91,19 +91,25 @@ struct Tiles {
   }
 };
 
+// The bias of a warp's NC columns, into its shared memory before a tile's first block is there.
+template <typename T, int NC>
+__device__ __forceinline__ void load_bias(const Args& g, int col, float* bias, int lane) {
+  const T* b = static_cast<const T*>(g.bias);
+  __syncwarp();   // the tile before has been stored
+#pragma unroll
+  for (int j = 0; j < NC / 32; ++j) bias[j * 32 + lane] = to_float(__ldg(b + min(col + j * 32 + lane, g.N - 1)));
+  __syncwarp();
+}
+
 // A lane's NC sums of row `row`, columns [col, col + NC): bias, one rounding, out.  With a tensor map of C a warp's 32 rows leave as pieces of 64
 // bytes a row that it lays out in shared memory (64-byte swizzle: no bank conflicts) and the TMA unit writes while the next tile is
 // begun.  (Each lane storing its own row, 32 bytes at a time, held the tensor cores up for a fifth of the time at K = 4096 and for two fifths
 // at K = 1024.)
 template <typename T, int NC>
-__device__ __forceinline__ void store_rows(const Args& g, const CUtensorMap* map, bool mapped, int row, int col, float (&acc)[NC], uint8_t* scratch, float* bias, int lane) {
+__device__ __forceinline__ void store_rows(const Args& g, const CUtensorMap* map, bool mapped, int row, int col, float (&acc)[NC], uint8_t* scratch, const float* bias, int lane) {
   const int row_base = row - lane;
   if (row_base >= g.M) return;   // the same for the whole warp
   if (g.bias != nullptr) {
-    const T* b = static_cast<const T*>(g.bias);
-#pragma unroll
-    for (int j = 0; j < NC / 32; ++j) bias[j * 32 + lane] = to_float(__ldg(b + min(col + j * 32 + lane, g.N - 1)));
-    __syncwarp();
 #pragma unroll
     for (int j = 0; j < NC; j += 4) {
       const float4 v = *reinterpret_cast<const float4*>(bias + j);
@@ -112,7 +118,6 @@ __device__ __forceinline__ void store_rows(const Args& g, const CUtensorMap* map
       acc[j + 2] += v.z;
       acc[j + 3] += v.w;
     }
-    __syncwarp();
   }
   if (mapped) {
     constexpr int kPer = kOutRow / static_cast<int>(sizeof(T)), kChunk = 16 / static_cast<int>(sizeof(T));
@@ -330,6 +335,13 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
       int tm, tn;
       tiles.at(t, &tm, &tn);
       const int row = tm * 256 + static_cast<int>(cta) * 128 + q * 32 + lane, col = tn * BN + first_col;
+      if (g.bias != nullptr) {
+        switch (g.type) {
+          case 6: load_bias<__half, NC>(g, col, bias, lane); break;
+          case 7: load_bias<float, NC>(g, col, bias, lane); break;
+          default: load_bias<__nv_bfloat16, NC>(g, col, bias, lane);
+        }
+      }
       float acc[NC];
 #pragma unroll
       for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
@@ -446,11 +458,15 @@ cudaError_t fire(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap
   return cudaLaunchKernelEx(&cfg, kernel, ta, tb, tc, g, mapped);
 }
 
-// C for stores of 32 rows of 64 bytes; false where its rows do not start on 16 bytes.
+// Whether the TMA unit can write C: rows that start on 16 bytes.
+bool can_map_out(const Args& g) {
+  const uint64_t size = g.type == 7 ? 4 : 2;
+  return (reinterpret_cast<uintptr_t>(g.c) & 15u) == 0 && g.ldc * size % 16 == 0 && g.ldc * size < (1ull << 40);
+}
+// C for stores of 32 rows of 64 bytes.
 bool make_tensor_map_out(CUtensorMap* map, const Args& g) {
   const CudaDriver* d = CudaDriver::get();
   const cuuint64_t size = g.type == 7 ? 4 : 2;
-  if ((reinterpret_cast<uintptr_t>(g.c) & 15u) != 0 || g.ldc * size % 16 != 0 || g.ldc * size >= (1ull << 40)) return false;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(g.N), static_cast<cuuint64_t>(g.M)};
   cuuint64_t strides[1] = {g.ldc * size};
   cuuint32_t box[2] = {static_cast<cuuint32_t>(kOutRow / size), 32};
@@ -460,21 +476,23 @@ bool make_tensor_map_out(CUtensorMap* map, const Args& g) {
                                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The tile width with the least estimated time (ns): a wave of tiles takes about a microsecond and so much a block of K (measured: 8192 x 4096 x 1024, seven
-// waves of 256, 41 us; 512 x 4096 x 4096, one wave of 128, 15.8 us; 4096 x 4096 x 4096, four of 256, 67 us, and 101 with a scale for every row of
-// B).  A narrower tile pays where it saves a wave or leaves fewer SMs idle.
-int pick_width(int M, int N, int K, bool b_rows, int pairs, long* ns) {
+// The tile width with the least estimated time (ns): a wave of tiles takes about two microseconds and so much a block of K, more with a scale for
+// every row of B (measured, us without / with those: 512 x 1024 x 1024, one wave of 128, 7.7 / 8.5; 1001 x 1288 x 5000 19.1 / 22.0; 1001 x
+// 5000 x 1288, two of 192, 17.7 / 20.7; 4096 x 4096 x 4096, four of 256, 67 / 101; 8192 x 4096 x 1024, seven of 256, 41).  Rows of C that the TMA unit cannot
+// write cost a wave of 128 columns three more (777 x 1003 x 1544 13.1, 777 x 1000 x 1544 10.1).  A narrower tile pays where it saves a wave or leaves fewer
+// SMs idle.
+int pick_width(int M, int N, int K, bool b_rows, bool mapped, int pairs, long* ns) {
   struct Width {
     int bn;
     long per_block, per_block_rows;
   };
-  constexpr Width kWidths[] = {{256, 480, 740}, {192, 400, 580}, {128, 310, 420}};
+  constexpr Width kWidths[] = {{256, 430, 720}, {192, 390, 560}, {128, 355, 423}};
   const long num_kb = (K + kBlockK - 1) / kBlockK;
   int best = 256;
   *ns = -1;
   for (const Width& w : kWidths) {
     const long tiles = static_cast<long>((M + 255) / 256) * ((N + w.bn - 1) / w.bn), waves = (tiles + pairs - 1) / pairs;
-    const long t = 5000 + waves * (1000 + num_kb * (b_rows ? w.per_block_rows : w.per_block));
+    const long t = 3100 + waves * (2000 + (mapped ? 0 : 3000 * w.bn / 128) + num_kb * (b_rows ? w.per_block_rows : w.per_block));
     if (*ns < 0 || t < *ns) {
       *ns = t;
       best = w.bn;
@@ -488,10 +506,10 @@ struct Plan {
   SmallPlan p;
   int bn;   // pairs: tile width
 };
-Plan make_plan(int M, int N, int K, bool b_rows, int sms) {
+Plan make_plan(int M, int N, int K, bool b_rows, bool mapped, int sms) {
   Plan plan{};
   long pair_ns = 0, small_ns = 0;
-  plan.bn = pick_width(M, N, K, b_rows, sms / 2, &pair_ns);
+  plan.bn = pick_width(M, N, K, b_rows, mapped, sms / 2, &pair_ns);
   plan.small = plan_small(M, N, K, sms, &plan.p, &small_ns) && small_ns < pair_ns;
   return plan;
 }
@@ -500,7 +518,7 @@ int run(const void* a, int64_t lda, const void* b, int64_t ldb, Args g, cudaStre
   std::string why;
   g.err = error_word();
   g.wait_budget_ns = 2000000000ull;
-  const Plan plan = make_plan(g.M, g.N, g.K, g.b.shift == 0, sm_count());
+  const Plan plan = make_plan(g.M, g.N, g.K, g.b.shift == 0, can_map_out(g), sm_count());
   const int bn = plan.bn;
   cudaError_t e;
   if (plan.small) {
@@ -513,7 +531,7 @@ int run(const void* a, int64_t lda, const void* b, int64_t ldb, Args g, cudaStre
     if (!make_tensor_map_e4m3(&ta, a, g.M, g.K, lda, 128, &why) || !make_tensor_map_e4m3(&tb, b, g.N, g.K, ldb, bn / 4, &why)) {
       e = cudaErrorInvalidValue;
     } else {
-      mapped = make_tensor_map_out(&tc, g);
+      mapped = can_map_out(g) && make_tensor_map_out(&tc, g);
       const auto go = [&](auto rows) {
         constexpr bool R = decltype(rows)::value;
         switch (bn) {
@@ -569,11 +587,12 @@ MNCCL_EXPORT int mncclGemmFp8(const void* a, int64_t lda, const float* sa, int64
 }
 
 // The kernel that an M x N x K product takes on `sms` SMs: returns 1 for the one for few rows or tiles (tile = rows of A per tile, slices = CTAs that
-// share a tile's K), 0 for CTA pairs (tile = columns, slices = 1).  b_rows: rows of a scale of B.  Host arithmetic only (needs no GPU).
-MNCCL_EXPORT int mncclGemmFp8Plan(int M, int N, int K, int b_rows, int sms, int* tile, int* slices) {
+// share a tile's K), 0 for CTA pairs (tile = columns, slices = 1).  b_rows: rows of a scale of B; aligned: whether C's rows start on 16 bytes.
+// Host arithmetic only (needs no GPU).
+MNCCL_EXPORT int mncclGemmFp8Plan(int M, int N, int K, int b_rows, int aligned, int sms, int* tile, int* slices) {
   using namespace mnccl::gemm::fp8;
   if (M <= 0 || N <= 0 || K <= 0 || sms < 2 || (b_rows != 1 && b_rows != 128)) return -1;
-  const Plan plan = make_plan(M, N, K, b_rows == 1, sms);
+  const Plan plan = make_plan(M, N, K, b_rows == 1, aligned != 0, sms);
   if (tile) *tile = plan.small ? plan.p.tn : plan.bn;
   if (slices) *slices = plan.small ? plan.p.slices : 1;
   return plan.small ? 1 : 0;

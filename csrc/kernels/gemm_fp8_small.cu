@@ -349,16 +349,18 @@ int per_slice(int num_kb, int slices, int tn) {
 //   1 x 4096 x 4096      16 / 4: 8.2 us, 16 / 8: 8.6, 16 / 2: 9.6          64 x 14336 x 4096   64 / 1: 20.2 us, 32 / 1: 23.1, pairs: 21.2
 //   16 x 4096 x 14336    16 / 8: 14.7 us, 16 / 4: 15.3, 16 / 2: 19.5       128 x 4096 x 4096   64 / 2: 15.1 us, 32 / 1: 16.8, pairs: 16.8
 //   256 x 1024 x 1024    16 / 1: 6.9 us, 64 / 4: 7.7, pairs: 7.8           256 x 4096 x 4096   64 / 1: 18.9 us, pairs: 16.4
-// So a tile takes a fixed time and one per block of K that grows with its width; a second CTA on an SM takes as long again, except where
-// memory is what all wait for; and nothing is faster than the operands come from memory.  Tiles of 128 rows of A never won (128 x 4096 x
-// 4096: 16.4 us).  A tile that has its K and its SM to itself takes all of the shared memory as its ring (16 x 14336 x 4096: 16.9 -> 15.5 us);
+//   512 x 1024 x 1024    32 / 1: 9.2 us, pairs: 7.7                        777 x 1003 x 1544  64 / 1: 12.7 us, pairs: 13.1
+// So a tile takes a fixed time and one per block of K that grows with its width; two narrow tiles on an SM overlap by a third, two wide
+// ones hardly; and nothing is faster than the operands come from memory.  Tiles of 128 rows of A never won (128 x 4096 x 4096: 16.4 us).  A
+// tile that has its K and its SM to itself takes all of the shared memory as its ring (16 x 14336 x 4096: 16.9 -> 15.5 us);
 // slices do better with half, which lets the next wave's CTAs in early (1 x 4096 x 4096: 9.0 -> 8.2 us).
 bool plan_small(int M, int N, int K, int sms, SmallPlan* p, long* ns) {
   struct Cost {
     int tn;
     long fixed, per_block, split;   // a tile; a block of K; the meeting of the slices
   };
-  constexpr Cost kCost[] = {{16, 4500, 270, 1300}, {32, 4700, 360, 1800}, {64, 5200, 490, 2200}};
+  constexpr Cost kCost[] = {{16, 1800, 260, 1300}, {32, 3300, 330, 1400}, {64, 5500, 320, 1500}};
+  constexpr long kLaunch = 3000;
   const int num_kb = (K + kBlockK - 1) / kBlockK;
   const long tiles_n = (N + 127) / 128, floor_ns = 4500 + static_cast<long>((static_cast<double>(K) * (static_cast<double>(M) + N) + 2.0 * M * N) / 5800.0);
   *ns = -1;
@@ -367,10 +369,10 @@ bool plan_small(int M, int N, int K, int sms, SmallPlan* p, long* ns) {
     if (tiles > (1 << 20)) continue;
     for (int slices = 1; slices <= 8; slices *= 2) {
       const int per = per_slice(num_kb, slices, c.tn);
-      const long items = tiles * slices;
+      const long items = tiles * slices, rounds = (items + sms - 1) / sms;
       if ((slices - 1) * per >= num_kb || (slices > 1 && items > 2L * sms)) break;   // a slice would be empty, or CTAs wait for others
-      const long rounds = (items + sms - 1) / sms, fixed = c.fixed + (slices > 1 ? c.split : 0) + (slices > 4 ? 1500 : 0);
-      const long t = std::max(fixed + rounds * std::min(per, num_kb) * c.per_block, floor_ns + (items > sms ? 300 : 0));
+      const long each = c.fixed + std::min(per, num_kb) * c.per_block + (slices > 1 ? c.split : 0);
+      const long t = std::max(kLaunch + (rounds > 1 && c.tn <= 32 ? rounds * each * 7 / 10 : rounds * each), floor_ns + (rounds > 1 ? 300 : 0));
       if (*ns < 0 || t < *ns) {
         *ns = t;
         *p = SmallPlan{c.tn, slices, per, static_cast<int>(tiles), slices == 1 && items <= sms};

@@ -121,8 +121,8 @@ int mncclGemmFp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, in
                  const float* sb, int64_t sb_row, int64_t sb_blk, int sb_rows, void* c, int64_t ldc, int type, const void* bias, int M, int N,
                  int K, cudaStream_t stream);
 /* The kernel that a product takes on `sms` SMs, without a launch (needs no GPU): 1 = the one for few rows or tiles (tile: rows of A per
- * tile; slices: CTAs that share a tile's K), 0 = CTA pairs (tile: columns), -1 = bad arguments. */
-int mncclGemmFp8Plan(int M, int N, int K, int b_rows, int sms, int* tile, int* slices);
+ * tile; slices: CTAs that share a tile's K), 0 = CTA pairs (tile: columns), -1 = bad arguments.  aligned: whether C's rows start on 16 bytes. */
+int mncclGemmFp8Plan(int M, int N, int K, int b_rows, int aligned, int sms, int* tile, int* slices);
 
 /* ---- distillation from a teacher's top logits -----------------------------------------------------------
  * Student logits [T, V] of `type` (6, 7 or 9), row stride ld; ids and top [T, K], K <= 1024, tau in [1e-3, 1e3].  With

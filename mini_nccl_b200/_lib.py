@@ -116,7 +116,7 @@ def lib() -> C.CDLL:
     if hasattr(L, "mncclGemmFp8"):
         sig("mncclGemmFp8", i32, vp, C.c_int64, vp, C.c_int64, C.c_int64, i32, vp, C.c_int64, vp, C.c_int64, C.c_int64, i32, vp, C.c_int64, i32,
             vp, i32, i32, i32, vp)
-        sig("mncclGemmFp8Plan", i32, i32, i32, i32, i32, i32, P(i32), P(i32))
+        sig("mncclGemmFp8Plan", i32, i32, i32, i32, i32, i32, i32, P(i32), P(i32))
     if hasattr(L, "mncclDistillForward"):
         sig("mncclDistillForward", i32, vp, i32, C.c_int64, i32, i32, vp, vp, i32, C.c_float, vp, vp, vp, vp, vp, vp, vp, vp)
         sig("mncclDistillBackward", i32, vp, i32, C.c_int64, i32, i32, vp, vp, i32, C.c_float, vp, vp, vp, i32, vp, vp, C.c_int64, vp)

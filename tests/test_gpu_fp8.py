@@ -138,14 +138,14 @@ def _product(a, sa, b, sb):
 SHAPES = [(1, 1, 1), (1, 128, 128), (1, 129, 4096), (2, 64, 72), (15, 300, 136), (16, 14336, 256), (17, 1003, 1544), (33, 257, 3000), (64, 512, 8192), (65, 127, 640),
           (127, 1024, 1024), (129, 640, 320), (256, 256, 256), (255, 4096, 129), (300, 300, 14336), (777, 1003, 1544), (1024, 2048, 512), (2000, 130, 700),
           (4096, 3584, 384), (5, 50257, 128), (8192, 136, 200),
-          (20, 2048, 2048), (32, 4096, 4096), (64, 4096, 4096), (512, 1024, 4096), (600, 1024, 300), (1001, 5000, 1288), (5000, 1288, 1001)]
+          (20, 2048, 2048), (24, 8192, 8192), (32, 4096, 4096), (64, 4096, 4096), (512, 1024, 4096), (600, 1024, 300), (1001, 5000, 1288), (5000, 1288, 1001)]
 
 
 def _plan(M, N, K, b_rows=128):
     import mini_nccl_b200 as mn
 
     tile, slices = C.c_int(0), C.c_int(0)
-    small = mn.lib().mncclGemmFp8Plan(M, N, K, b_rows, 148, C.byref(tile), C.byref(slices))
+    small = mn.lib().mncclGemmFp8Plan(M, N, K, b_rows, N % 8 == 0, 148, C.byref(tile), C.byref(slices))
     return small, tile.value, slices.value
 
 
