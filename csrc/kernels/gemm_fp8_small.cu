@@ -154,6 +154,8 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
 #pragma unroll
   for (int j = 0; j < NC; ++j) acc[j] = 0.0f;
   bool ok = true;
+  const bool one = g.b.shift != 0;   // a scale of B holds for the whole tile
+  const float bias = promoter ? bias_of(g, n) : 0.0f;
 
   if (warp == 0) {
     uint32_t s = 0, ph = 0;
@@ -197,18 +199,24 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   } else if (warp == 2 + W) {
     const float *rows[4], *cols[(TN + 31) / 32];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) rows[j] = g.b.at(min(n0 + lane + j * 32, g.N - 1)) + kb0 * g.b.blk;
+    for (int j = 0; j < 4; ++j) rows[j] = g.b.at(min(n0 + (one ? 0 : lane + j * 32), g.N - 1)) + (kb0 + (one ? lane : 0)) * g.b.blk;
 #pragma unroll
     for (int j = 0; j < (TN + 31) / 32; ++j) cols[j] = g.a.at(min(m0 + lane + j * 32, g.M - 1)) + kb0 * g.a.blk;
     uint32_t group = 0;
     for (int i0 = 0; i0 < nkb; i0 += kGroup, ++group) {
       if (!mbar_wait_warp(smem_u32(&ctl->scales_empty[group & 1u]), (group >> 1 & 1u) ^ 1u, &ctl->abort, g.wait_budget_ns)) break;
       float* slot = slots + (group & 1u) * kSlot<TN>;
+      if (one) {   // lane i fetches the group's i-th block
+        if (lane < kGroup && i0 + lane < nkb) copy4_async(slot + lane * 128, rows[0]);
+        rows[0] += kGroup * g.b.blk;
+      }
       for (int i = 0; i < kGroup && i0 + i < nkb; ++i) {
+        if (!one) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          copy4_async(slot + i * 128 + lane + j * 32, rows[j]);
-          rows[j] += g.b.blk;
+          for (int j = 0; j < 4; ++j) {
+            copy4_async(slot + i * 128 + lane + j * 32, rows[j]);
+            rows[j] += g.b.blk;
+          }
         }
 #pragma unroll
         for (int j = 0; j < (TN + 31) / 32; ++j) {
@@ -242,7 +250,7 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
         if (p >= blocks) break;
         const int in = i0 % kGroup + p;
         const float* cols = slot + kGroup * 128 + in * TN + first_col;
-        const float r = slot[in * 128 + q * 32 + lane];
+        const float r = slot[in * 128 + (one ? 0 : q * 32 + lane)];
         uint32_t v[NC];
         tmem_read(taddr + buf * (U * TN) + p * TN, v);
         if (p == blocks - 1) {
@@ -271,7 +279,6 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
 
   if (slices == 1) {
     if (promoter && ok) {
-      const float bias = bias_of(g, n);
 #pragma unroll
       for (int j = 0; j < NC; ++j) store(g, m0 + first_col + j, n, acc[j] + bias);
     }
@@ -290,7 +297,6 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
     }
     cluster_sync_all();
     if (promoter && ok) {
-      const float bias = bias_of(g, n);
       for (int c = (warp - 2) >> 2; c < own; c += W / 4) {
         const int m = m0 + slice * own + c;
         if (m >= g.M) break;
@@ -349,7 +355,7 @@ int per_slice(int num_kb, int slices, int tn) {
 //   1 x 4096 x 4096      16 / 4: 8.2 us, 16 / 8: 8.6, 16 / 2: 9.6          64 x 14336 x 4096   64 / 1: 20.2 us, 32 / 1: 23.1, pairs: 21.2
 //   16 x 4096 x 14336    16 / 8: 14.7 us, 16 / 4: 15.3, 16 / 2: 19.5       128 x 4096 x 4096   64 / 2: 15.1 us, 32 / 1: 16.8, pairs: 16.8
 //   256 x 1024 x 1024    16 / 1: 6.9 us, 64 / 4: 7.7, pairs: 7.8           256 x 4096 x 4096   64 / 1: 18.9 us, pairs: 16.4
-//   512 x 1024 x 1024    32 / 1: 9.2 us, pairs: 7.7                        777 x 1003 x 1544  64 / 1: 12.7 us, pairs: 13.1
+//   512 x 1024 x 1024    16 / 1: 8.6 us, pairs: 7.7                        777 x 1003 x 1544  64 / 1: 12.2 us, pairs: 13.1
 // So a tile takes a fixed time and one per block of K that grows with its width; two narrow tiles on an SM overlap by a third, two wide
 // ones hardly; and nothing is faster than the operands come from memory.  Tiles of 128 rows of A never won (128 x 4096 x 4096: 16.4 us).  A
 // tile that has its K and its SM to itself takes all of the shared memory as its ring (16 x 14336 x 4096: 16.9 -> 15.5 us);
