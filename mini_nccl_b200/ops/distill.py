@@ -118,7 +118,7 @@ def _native(logits, ids, top):
     """Whether the kernels take the call; the plain operators take the others."""
     if not (logits.is_cuda and _plain(logits) and _plain(ids) and _plain(top) and logits.dtype in _FLOATS):
         return False
-    if not (0 < ids.shape[-1] <= _MAX_ENTRIES and 0 < ids[..., 0].numel() < 2**31 and 0 < logits.shape[-1] < 2**31 - 2**12) or not _plain_call():
+    if not (0 < ids.shape[-1] <= _MAX_ENTRIES and 0 < ids.numel() // ids.shape[-1] < 2**31 and 0 < logits.shape[-1] < 2**31 - 2**12) or not _plain_call():
         return False
     return _no_tangent(logits)
 
@@ -142,7 +142,7 @@ def _arguments(shape, device, ids, top, temperature, reduction="mean"):
         raise ValueError("the temperature must be between 1e-3 and 1e3")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}")
-    return ids.long(), top.detach(), float(temperature)
+    return ids.long(), top.detach() if top.requires_grad else top, float(temperature)
 
 
 def distillation_loss(logits, top_ids, top_logits, temperature=1.0, reduction="mean"):
