@@ -502,6 +502,7 @@ int pick_width(int M, int N, int K, bool b_rows, bool mapped, int pairs, long* n
 }
 
 struct Plan {
+  bool rows;   // up to four tokens and a small weight: the kernel without tensor cores
   bool small;
   SmallPlan p;
   int bn;   // pairs: tile width
@@ -511,6 +512,7 @@ Plan make_plan(int M, int N, int K, bool b_rows, bool mapped, int sms) {
   long pair_ns = 0, small_ns = 0;
   plan.bn = pick_width(M, N, K, b_rows, mapped, sms / 2, &pair_ns);
   plan.small = plan_small(M, N, K, sms, &plan.p, &small_ns) && small_ns < pair_ns;
+  plan.rows = rows_ns(M, N, K) < std::min(small_ns, pair_ns);
   return plan;
 }
 
@@ -521,7 +523,9 @@ int run(const void* a, int64_t lda, const void* b, int64_t ldb, Args g, cudaStre
   const Plan plan = make_plan(g.M, g.N, g.K, g.b.shift == 0, can_map_out(g), sm_count());
   const int bn = plan.bn;
   cudaError_t e;
-  if (plan.small) {
+  if (plan.rows) {
+    e = launch_rows(a, lda, b, ldb, g, stream);
+  } else if (plan.small) {
     e = launch_small(a, lda, b, ldb, g, plan.p, stream, &why);
   } else {
     const long tiles = static_cast<long>((g.M + 255) / 256) * ((g.N + bn - 1) / bn);
@@ -586,16 +590,16 @@ MNCCL_EXPORT int mncclGemmFp8(const void* a, int64_t lda, const float* sa, int64
   }
 }
 
-// The kernel that an M x N x K product takes on `sms` SMs: returns 1 for the one for few rows or tiles (tile = rows of A per tile, slices = CTAs that
-// share a tile's K), 0 for CTA pairs (tile = columns, slices = 1).  b_rows: rows of a scale of B; aligned: whether C's rows start on 16 bytes.
+// The kernel that an M x N x K product takes on `sms` SMs: returns 2 for the one without tensor cores, 1 for the one for few rows or tiles (tile = rows of
+// A per tile, slices = CTAs that share a tile's K), 0 for CTA pairs (tile = columns, slices = 1).  b_rows: rows of a scale of B; aligned: whether C's rows start on 16 bytes.
 // Host arithmetic only (needs no GPU).
 MNCCL_EXPORT int mncclGemmFp8Plan(int M, int N, int K, int b_rows, int aligned, int sms, int* tile, int* slices) {
   using namespace mnccl::gemm::fp8;
   if (M <= 0 || N <= 0 || K <= 0 || sms < 2 || (b_rows != 1 && b_rows != 128)) return -1;
   const Plan plan = make_plan(M, N, K, b_rows == 1, aligned != 0, sms);
-  if (tile) *tile = plan.small ? plan.p.tn : plan.bn;
-  if (slices) *slices = plan.small ? plan.p.slices : 1;
-  return plan.small ? 1 : 0;
+  if (tile) *tile = plan.rows ? 8 : plan.small ? plan.p.tn : plan.bn;
+  if (slices) *slices = !plan.rows && plan.small ? plan.p.slices : 1;
+  return plan.rows ? 2 : plan.small ? 1 : 0;
 }
 
 }  // extern "C"

@@ -1,4 +1,4 @@
-// What the kernels of the 8-bit product with block scales share (gemm_fp8.cu, gemm_fp8_small.cu).
+// What the kernels of the 8-bit product with block scales share (gemm_fp8.cu, gemm_fp8_small.cu, gemm_fp8_rows.cu).
 //
 //   C[m, n] = sum over blocks b of 128 along K of  sa[m / ra, b] * sb[n / rb, b] * P_b[m, n]  (+ bias[n])
 //   P_b[m, n] = sum over k in b of a[m, k] * b[n, k]
@@ -182,6 +182,25 @@ __device__ __forceinline__ T round_to(float x) {
   else return __float2bfloat16_rn(x);
 }
 
+// One result, and its column's bias.
+__device__ __forceinline__ void store(const Args& g, int m, int n, float v) {
+  if (m >= g.M || n >= g.N) return;
+  const size_t at = static_cast<size_t>(m) * g.ldc + n;
+  switch (g.type) {
+    case 6: static_cast<__half*>(g.c)[at] = __float2half_rn(v); break;
+    case 7: static_cast<float*>(g.c)[at] = v; break;
+    default: static_cast<__nv_bfloat16*>(g.c)[at] = __float2bfloat16_rn(v);
+  }
+}
+__device__ __forceinline__ float bias_of(const Args& g, int n) {
+  if (g.bias == nullptr || n >= g.N) return 0.0f;
+  switch (g.type) {
+    case 6: return __half2float(static_cast<const __half*>(g.bias)[n]);
+    case 7: return static_cast<const float*>(g.bias)[n];
+    default: return __bfloat162float(static_cast<const __nv_bfloat16*>(g.bias)[n]);
+  }
+}
+
 // A matrix of bytes [rows, cols], boxes of box_rows x 128, 128-byte swizzle, zeros outside.
 bool make_tensor_map_e4m3(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t row_stride, uint32_t box_rows, std::string* why);
 
@@ -193,6 +212,9 @@ struct SmallPlan {
   bool deep = false;     // one CTA per SM with the whole shared memory as its ring, or two
 };
 bool plan_small(int M, int N, int K, int sms, SmallPlan* p, long* ns);
+// The kernel for up to four rows of A, and its estimated time.
+long rows_ns(int M, int N, int K);
+cudaError_t launch_rows(const void* a, int64_t lda, const void* b, int64_t ldb, const Args& g, cudaStream_t stream);
 cudaError_t launch_small(const void* a, int64_t lda, const void* b, int64_t ldb, const Args& g, const SmallPlan& p, cudaStream_t stream, std::string* why);
 
 }  // namespace fp8

@@ -57,24 +57,6 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
-__device__ __forceinline__ void store(const Args& g, int m, int n, float v) {
-  if (m >= g.M || n >= g.N) return;
-  const size_t at = static_cast<size_t>(m) * g.ldc + n;
-  switch (g.type) {
-    case 6: static_cast<__half*>(g.c)[at] = __float2half_rn(v); break;
-    case 7: static_cast<float*>(g.c)[at] = v; break;
-    default: static_cast<__nv_bfloat16*>(g.c)[at] = __float2bfloat16_rn(v);
-  }
-}
-__device__ __forceinline__ float bias_of(const Args& g, int n) {
-  if (g.bias == nullptr || n >= g.N) return 0.0f;
-  switch (g.type) {
-    case 6: return __half2float(static_cast<const __half*>(g.bias)[n]);
-    case 7: return static_cast<const float*>(g.bias)[n];
-    default: return __bfloat162float(static_cast<const __nv_bfloat16*>(g.bias)[n]);
-  }
-}
-
 template <int TN, int NS>
 __global__ void __launch_bounds__(kThreads<TN>)
 gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_x, const __grid_constant__ SmallArgs args) {
@@ -368,7 +350,7 @@ bool plan_small(int M, int N, int K, int sms, SmallPlan* p, long* ns) {
   constexpr Cost kCost[] = {{16, 1800, 260, 1300}, {32, 3300, 330, 1400}, {64, 5500, 320, 1500}};
   constexpr long kLaunch = 3000;
   const int num_kb = (K + kBlockK - 1) / kBlockK;
-  const long tiles_n = (N + 127) / 128, floor_ns = 4500 + static_cast<long>((static_cast<double>(K) * (static_cast<double>(M) + N) + 2.0 * M * N) / 5800.0);
+  const long tiles_n = (N + 127) / 128, floor_ns = 4000 + static_cast<long>((static_cast<double>(K) * (static_cast<double>(M) + N) + 2.0 * M * N) / 6300.0);
   *ns = -1;
   for (const Cost& c : kCost) {
     const long tiles = tiles_n * ((M + c.tn - 1) / c.tn);

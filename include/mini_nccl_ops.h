@@ -120,8 +120,9 @@ int mncclSumBlocks(const float* sums, int blocks, int K, void* out, int type, cu
 int mncclGemmFp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_blk, int sa_rows, const void* b, int64_t ldb,
                  const float* sb, int64_t sb_row, int64_t sb_blk, int sb_rows, void* c, int64_t ldc, int type, const void* bias, int M, int N,
                  int K, cudaStream_t stream);
-/* The kernel that a product takes on `sms` SMs, without a launch (needs no GPU): 1 = the one for few rows or tiles (tile: rows of A per
- * tile; slices: CTAs that share a tile's K), 0 = CTA pairs (tile: columns), -1 = bad arguments.  aligned: whether C's rows start on 16 bytes. */
+/* The kernel that a product takes on `sms` SMs, without a launch (needs no GPU): 2 = the one without tensor cores for up to four rows of A
+ * (tile: rows of B per CTA), 1 = the one for few rows or tiles (tile: rows of A per tile; slices: CTAs that share a tile's K), 0 = CTA
+ * pairs (tile: columns), -1 = bad arguments.  aligned: whether C's rows start on 16 bytes. */
 int mncclGemmFp8Plan(int M, int N, int K, int b_rows, int aligned, int sms, int* tile, int* slices);
 
 /* ---- distillation from a teacher's top logits -----------------------------------------------------------

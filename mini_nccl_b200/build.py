@@ -51,7 +51,7 @@ CUDA_SOURCES = [
 ]
 # Translation units compiled when present (a source tree may be trimmed to the collectives alone).
 OPTIONAL_CUDA = ["kernels/gemm_sm100.cu", "kernels/gemm_small.cu", "kernels/gemm_fused.cu", "kernels/noalloc.cu", "kernels/elementwise.cu", "kernels/lm_loss.cu",
-                 "kernels/fp8_quantize.cu", "kernels/gemm_fp8.cu", "kernels/gemm_fp8_small.cu", "kernels/distill.cu"]
+                 "kernels/fp8_quantize.cu", "kernels/gemm_fp8.cu", "kernels/gemm_fp8_small.cu", "kernels/gemm_fp8_rows.cu", "kernels/distill.cu"]
 OPTIONAL_HOST = ["net/verbs_transport.cc"]
 
 _HERA_SRCS = ["csrc/bootstrap/hera.cc", "csrc/bootstrap/socket.cc", "csrc/core/log.cc"]
