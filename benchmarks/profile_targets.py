@@ -10,6 +10,8 @@ larger than the L2 but far below a GB, so that a capture ends by itself within a
   python benchmarks/profile_targets.py --target gemm_rs     # fused GEMM->reduce-scatter kernel, one rank, 4096 x 4096 x 1792
   python benchmarks/profile_targets.py --target ag_gemm     # fused all-gather->GEMM kernel with the SwiGLU epilogue, one rank, 4096 x 3584 x 4096
   python benchmarks/profile_targets.py --target lm_loss     # cross-entropy of a language-model head, forward and backward, 2048 x 50257
+  python benchmarks/profile_targets.py --target fp8         # 8-bit quantisation 8192 x 4096 and products 8192 x 4096 x 1024, 16 x 14336 x 4096, 1 x 4096 x 4096
+  python benchmarks/profile_targets.py --target distill     # distillation from a teacher's top logits, forward and backward, 2048 x 50257
   python benchmarks/profile_targets.py --target swiglu      # one-pass SwiGLU kernel, 4096 x 2 x 14336 bf16 in
   python benchmarks/profile_targets.py --target ll          # emulated 4-rank LL AllReduce, 32 KiB per rank
   python benchmarks/profile_targets.py --target pipe        # emulated 4-rank pipelined AllReduce (peer-to-peer form), 64 MiB per rank, ordinary buffers
@@ -34,7 +36,7 @@ def main():
     from mini_nccl_b200 import _lib
 
     ap = argparse.ArgumentParser()
-    ap.add_argument("--target", required=True, choices=["gemm", "gemm_pair", "gemm_small", "lm_loss", "copy", "twoshot", "oneshot", "gemm_rs", "ag_gemm", "swiglu", "ll", "pipe", "noalloc", "auto_direct"])
+    ap.add_argument("--target", required=True, choices=["gemm", "gemm_pair", "gemm_small", "lm_loss", "fp8", "distill", "copy", "twoshot", "oneshot", "gemm_rs", "ag_gemm", "swiglu", "ll", "pipe", "noalloc", "auto_direct"])
     ap.add_argument("--launches", type=int, default=4)
     args = ap.parse_args()
     torch.cuda.set_device(0)
@@ -99,6 +101,27 @@ def main():
         t = torch.randint(0, 50257, (2048,), device="cuda")
         for _ in range(args.launches):
             _LmHeadCrossEntropy.apply(x, w, t).backward()      # 206 MB of logits
+        torch.cuda.synchronize()
+    elif args.target == "fp8":
+        from mini_nccl_b200.ops import gemm_fp8, gemm_status, quantize_fp8
+
+        x = torch.randn(8192, 4096, device="cuda", dtype=torch.bfloat16)                  # 67 MB in, 67 MB out with the transpose
+        shapes = [(8192, 4096, 1024), (16, 14336, 4096), (1, 4096, 4096)]
+        operands = [(*quantize_fp8(torch.randn(m, k, device="cuda")), *quantize_fp8(torch.randn(n, k, device="cuda"), block_rows=128)) for m, n, k in shapes]
+        for _ in range(args.launches):
+            quantize_fp8(x, transposed=True)
+            for o in operands:
+                gemm_fp8(*o)
+        torch.cuda.synchronize()
+        assert gemm_status() == 0
+    elif args.target == "distill":
+        from mini_nccl_b200.ops import distillation_loss
+
+        z = (torch.randn(2048, 50257, device="cuda") * 2).to(torch.bfloat16).requires_grad_()      # 206 MB of logits
+        ids, top = torch.randint(0, 50257, (2048, 64), device="cuda"), torch.randn(2048, 64, device="cuda")
+        for _ in range(args.launches):
+            z.grad = None
+            distillation_loss(z, ids, top, temperature=2.0).backward()
         torch.cuda.synchronize()
     elif args.target == "swiglu":
         from mini_nccl_b200.ops import swiglu_bf16

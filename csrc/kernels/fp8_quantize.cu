@@ -15,6 +15,8 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <cstring>
+#include <type_traits>
 
 namespace {
 
@@ -105,8 +107,25 @@ __device__ __forceinline__ uint32_t quantise4(float a, float b, float c, float d
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
 }
+// The product of a word's two bf16 numbers with two scales' inverses.  Powers of two: it is exact, or so small that e4m3 makes it zero.
+__device__ __forceinline__ uint32_t times(uint32_t w, uint32_t inverses) {
+  __nv_bfloat162 a, b;
+  memcpy(&a, &w, 4);
+  memcpy(&b, &inverses, 4);
+  a = __hmul2(a, b);
+  memcpy(&w, &a, 4);
+  return w;
+}
+__device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ uint32_t twice(float inverse) { return __byte_perm(__float_as_uint(inverse), 0u, 0x3232); }   // as two bf16 numbers
+
 template <typename T>
 __device__ __forceinline__ uint2 quantise8(const Eight<T>& v, float inverse) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    const uint32_t s = twice(inverse), a = times(v.w[0], s), b = times(v.w[1], s), c = times(v.w[2], s), d = times(v.w[3], s);
+    return make_uint2(quantise4(low(a), high(a), low(b), high(b)), quantise4(low(c), high(c), low(d), high(d)));
+  }
   return make_uint2(quantise4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse),
                     quantise4(v[4] * inverse, v[5] * inverse, v[6] * inverse, v[7] * inverse));
 }
@@ -139,16 +158,16 @@ quantise_rows_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t*
 // A tile of 128 x 128 elements, which holds whole blocks of either kind along both dimensions: x is read once for q, the transpose qt and the sums
 // of the tile's columns.  A thread holds 4 neighbouring rows of 2 x 8 columns, as they lie in memory (as fp32 numbers 16-bit types took 128
 // registers, and half of the memory's rate: 64 us for 8192 x 4096), so that 4 elements of a column are one word of the transposed tile in shared
-// memory, [column][32 words + 1].
-constexpr int kPitch = 33;
+// memory: [column][8 units of 16 bytes], unit u of column c at u ^ (c / 8 mod 8), which keeps the banks apart both for the words that come in
+// and for the units that go out.
 
 template <typename T, bool SQUARE>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
 quantise_tile_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t* __restrict__ q, size_t ldq, float* __restrict__ scale,
                      uint8_t* __restrict__ qt, size_t ldt, float* __restrict__ scale_t, float* __restrict__ sums, bool vec) {
-  __shared__ uint32_t tile[kBlock * kPitch];
+  __shared__ __align__(16) uint32_t tile[kBlock * 32];
   __shared__ uint32_t part[8][kBlock];   // a warp's largest magnitude of each column, then its sum
-  __shared__ float inverse[kBlock];
+  __shared__ __align__(16) float inverse[kBlock];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m0 = static_cast<int>(blockIdx.x) * kBlock, k0 = static_cast<int>(blockIdx.y) * kBlock;
   const int r0 = warp * 16 + (lane >> 3) * 4, c0 = (lane & 7) * 8;   // columns c0 .. and c0 + 64 ..
@@ -236,19 +255,32 @@ quantise_tile_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t*
         }
     }
   }
+  uint32_t* out = tile + ((warp ^ (lane & 7)) * 4 + (lane >> 3));   // c / 8 mod 8 is lane mod 8
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 8; j += 2) {
       const int c = c0 + h * 64 + j;
-      const float s = SQUARE ? row_inverse[0] : inverse[c];
-      tile[c * kPitch + r0 / 4] = quantise4(v[0][h][j] * s, v[1][h][j] * s, v[2][h][j] * s, v[3][h][j] * s);
+      const float2 s = SQUARE ? make_float2(row_inverse[0], row_inverse[0]) : *reinterpret_cast<const float2*>(inverse + c);
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        const uint32_t both = __byte_perm(__float_as_uint(s.x), __float_as_uint(s.y), 0x7632);
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = times(v[i][h].w[j / 2], both);
+        out[c * 32] = quantise4(low(w[0]), low(w[1]), low(w[2]), low(w[3]));
+        out[(c + 1) * 32] = quantise4(high(w[0]), high(w[1]), high(w[2]), high(w[3]));
+      } else {
+        out[c * 32] = quantise4(v[0][h][j] * s.x, v[1][h][j] * s.x, v[2][h][j] * s.x, v[3][h][j] * s.x);
+        out[(c + 1) * 32] = quantise4(v[0][h][j + 1] * s.y, v[1][h][j + 1] * s.y, v[2][h][j + 1] * s.y, v[3][h][j + 1] * s.y);
+      }
     }
   __syncthreads();
-#pragma unroll 4
-  for (int c = warp; c < kBlock; c += 8)   // a column leaves as 128 bytes; rows of qt are padded to 16
-    if (k0 + c < K && m0 + lane * 4 < static_cast<int>(ldt))
-      *reinterpret_cast<uint32_t*>(qt + static_cast<size_t>(k0 + c) * ldt + m0 + lane * 4) = tile[c * kPitch + lane];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {   // a column leaves as 128 bytes; rows of qt are padded to 16
+    const int c = i * 32 + warp * 4 + (lane >> 3), u = lane & 7;
+    if (k0 + c < K && m0 + u * 16 < static_cast<int>(ldt))
+      *reinterpret_cast<uint4*>(qt + static_cast<size_t>(k0 + c) * ldt + m0 + u * 16) = *reinterpret_cast<const uint4*>(tile + c * 32 + (u ^ (c >> 3 & 7)) * 4);
+  }
   if (!SQUARE && sums != nullptr && threadIdx.x < kBlock && k0 + static_cast<int>(threadIdx.x) < K) {
     float s = 0.0f;
 #pragma unroll
