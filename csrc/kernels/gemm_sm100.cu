@@ -121,9 +121,20 @@ uint32_t* error_word() {
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices) dev = 0;
   if (g_err_dev[dev] == nullptr) {
+    // The first product of a process may be one that is being captured: this thread's other calls are not part of that, and the word is zeroed on a
+    // stream of its own.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     uint32_t* p = nullptr;
-    if (cudaMalloc(&p, 64) != cudaSuccess) return nullptr;
-    cudaMemset(p, 0, 64);
+    cudaStream_t own = nullptr;
+    const bool ready = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking) == cudaSuccess && cudaMalloc(&p, 64) == cudaSuccess &&
+                       cudaMemsetAsync(p, 0, 64, own) == cudaSuccess && cudaStreamSynchronize(own) == cudaSuccess;
+    if (own != nullptr) cudaStreamDestroy(own);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ready) {
+      if (p != nullptr) cudaFree(p);
+      return nullptr;
+    }
     g_err_dev[dev] = p;
   }
   return g_err_dev[dev];

@@ -1,5 +1,8 @@
 """8-bit quantisation, products and the linear layer against their definitions in 64 bits."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -249,6 +252,23 @@ def test_products_of_nothing_on_other_streams_and_in_graphs():
     torch.cuda.synchronize()
     eager = gemm_fp8(*quantize_fp8(x), b, sb, out_dtype=torch.float32)
     assert all(torch.equal(r, eager) for r in results)
+
+
+@pytest.mark.gpu
+def test_first_product_of_a_process_may_be_captured():
+    """What a product needs once for each process (the word for waits that ran out) is made without breaking a capture that is under way."""
+    code = """
+import torch
+from mini_nccl_b200.ops import gemm_fp8
+a, s = torch.ones(16, 256, device="cuda").to(torch.float8_e4m3fn), torch.ones(16, 2, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = gemm_fp8(a, s, a, s)
+graph.replay()
+assert bool((out == 256).all())
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
 
 
 # ---- the linear layer
