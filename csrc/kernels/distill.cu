@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(1024)
 distill_mean_kernel(const float* __restrict__ row_loss, const int* __restrict__ counts, int T, float* __restrict__ sum, float* __restrict__ mean,
                     float* __restrict__ tokens) {
   __shared__ float box[2][32];
-  float s = 0.0f, n = 0.0f;   // n: whole numbers, exact
+  float s = 0.0f, n = 0.0f;   // n: whole numbers, exact up to 2^24
   for (int t = threadIdx.x; t < T; t += 1024) {
     s += row_loss[t];
     n += static_cast<float>(counts[t]);

@@ -276,9 +276,9 @@ quantise_tile_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t*
     }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {   // a column leaves as 128 bytes; rows of qt are padded to 16
+  for (int i = 0; i < 4; ++i) {   // a column leaves as 128 bytes, the last as M rounded up to 16
     const int c = i * 32 + warp * 4 + (lane >> 3), u = lane & 7;
-    if (k0 + c < K && m0 + u * 16 < static_cast<int>(ldt))
+    if (k0 + c < K && m0 + u * 16 < M)
       *reinterpret_cast<uint4*>(qt + static_cast<size_t>(k0 + c) * ldt + m0 + u * 16) = *reinterpret_cast<const uint4*>(tile + c * 32 + (u ^ (c >> 3 & 7)) * 4);
   }
   if (!SQUARE && sums != nullptr && threadIdx.x < kBlock && k0 + static_cast<int>(threadIdx.x) < K) {
@@ -340,7 +340,7 @@ extern "C" {
 #define MNCCL_EXPORT __attribute__((visibility("default")))
 
 // x [M, K] (type 6 fp16, 7 fp32, 9 bf16; row stride ldx elements) -> q [M, K] e4m3 (row stride ldq, a multiple of 16 that holds K
-// rounded up to one; 16-byte aligned; the padding is written) and its scales: block_rows 1: scale[K blocks][M]; block_rows 128:
+// rounded up to one; 16-byte aligned; bytes up to that may be written, none behind it) and its scales: block_rows 1: scale[K blocks][M]; block_rows 128:
 // scale[M blocks][K blocks].  qt, if not null: the transpose [K, M] (ldt like ldq), for block_rows 1 quantised anew in blocks along M
 // with scale_t[M blocks][K].  sums, if not null (only with qt and block_rows 1): [M blocks][K], the columns' sums over each 128 rows.
 // Returns 0, -1 null or empty, -2 shape or alignment, or a cudaError_t + 1000.

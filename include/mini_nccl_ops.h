@@ -107,7 +107,7 @@ int mncclTransposeBf16(const void* src, int64_t lds, int rows, int cols, void* d
  *
  * Quantise x [M, K] (row stride ldx elements): a block of block_rows (1 or 128) x 128 elements has the scale 2^e, the
  * smallest with e >= -126 and 448 * 2^e >= its largest magnitude; q = x / scale, rounded to nearest even.  A block with an
- * infinity or a NaN becomes NaN.  Rows of q hold K rounded up to 16; the padding is written.  block_rows 1:
+ * infinity or a NaN becomes NaN.  Rows of q hold K rounded up to 16 (K at most 65535 * 128); bytes up to there may be written, none behind.  block_rows 1:
  * scale[K blocks][M]; 128: scale[M blocks][K blocks].  qt (may be null): the transpose [K, M], for block_rows 1 quantised
  * along M with scale_t[M blocks][K]; for 128 with the same scales (scale_t unused).  sums (may be null; only with qt and
  * block_rows 1): [M blocks][K], the columns' sums over each 128 rows, which mncclSumBlocks adds up to out[K]. */

@@ -423,6 +423,25 @@ def test_calls_through_ctypes_do_the_same():
                 bad(c)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("M,K", [(100, 24), (5, 130), (128, 128), (250, 300)])
+def test_quantize_writes_nothing_behind_its_rows(M, K, rows):
+    """Buffers of the C interface with longer rows than they need: bytes behind the padding, and the rows after the last, stay as they were."""
+    import mini_nccl_b200 as mn
+
+    x = torch.randn(M, K, device="cuda")
+    q, qt = torch.full((M + 1, 512), 7, dtype=torch.uint8, device="cuda"), torch.full((K + 1, 512), 7, dtype=torch.uint8, device="cuda")
+    scale, scale_t = torch.empty(_blocks(K) * M, device="cuda"), torch.empty(_blocks(M) * K, device="cuda")
+    rc = mn.lib().mncclQuantizeFp8(x.data_ptr(), 7, K, M, K, rows, q.data_ptr(), 512, scale.data_ptr(), qt.data_ptr(), 512, scale_t.data_ptr(), None,
+                                   torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    for buffer, (m, k) in ((q, (M, K)), (qt, (K, M))):
+        assert bool((buffer[m:] == 7).all()) and bool((buffer[:, -(-k // 16) * 16:] == 7).all())
+    want = quantize_fp8(x, block_rows=rows, transposed=True)
+    assert torch.equal(q[:M, :K], want[0].view(torch.uint8)) and torch.equal(qt[:K, :M], want[2].view(torch.uint8))
+
+
 # ---- refusals
 
 
