@@ -325,7 +325,7 @@ PyObject* ag_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // ---- 8-bit operators and distillation (ops/fp8.py, ops/distill.py).  They run on their tensors' GPU, whichever is current, and on the given
 // stream or that GPU's current one; what they allocate belongs to that stream.
 
-constexpr int64_t kBlock = 128, kMost = 2147483647 - 65536;
+constexpr int64_t kBlock = 128, kMost = 2147483647 - 65536, kMostColumns = 65535 * kBlock;   // kMostColumns: of what mncclQuantizeFp8 takes
 int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
 int64_t padded(int64_t n) { return (n + 15) / 16 * 16; }
 
@@ -427,6 +427,10 @@ PyObject* quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!matrix(*x, "x", float_code(*x) >= 0, &ld)) return nullptr;
   if (block_rows != 1 && block_rows != kBlock) {
     PyErr_SetString(PyExc_ValueError, "block_rows must be 1 or 128");
+    return nullptr;
+  }
+  if (x->size(1) > kMostColumns) {
+    PyErr_Format(PyExc_ValueError, "x must have at most %lld columns", static_cast<long long>(kMostColumns));
     return nullptr;
   }
   On o;

@@ -127,6 +127,7 @@ _BLOCK = 128
 _E4M3 = torch.float8_e4m3fn
 _FLOATS = {torch.float16: 6, torch.float32: 7, torch.bfloat16: 9}
 _MOST = 2**31 - 1 - 2**16   # rows and columns of a matrix: indices are 32-bit, elements are addressed with 64
+_MOST_COLUMNS = 65535 * _BLOCK   # of what mncclQuantizeFp8 takes
 
 
 def _blocks(n):
@@ -196,6 +197,8 @@ def quantize_fp8(lib, x, block_rows, transposed, stream):
     _matrix(x, "x", _FLOATS)
     if block_rows not in (1, _BLOCK):
         raise ValueError("block_rows must be 1 or 128")
+    if x.shape[1] > _MOST_COLUMNS:
+        raise ValueError(f"x must have at most {_MOST_COLUMNS} columns")
     with _on(x.device, stream) as s:
         return _quantize(lib, x, block_rows, transposed, False, s)[:4]
 

@@ -12,6 +12,7 @@ from torch.autograd.function import once_differentiable
 from .._lib import ext, lib
 
 BLOCK = 128
+_MOST_ROWS, _MOST_COLUMNS = 2**31 - 1 - 2**16, 65535 * BLOCK   # mncclQuantizeFp8
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _calls = {}   # the extension's entry points, looked up on the first call
 
@@ -38,7 +39,8 @@ def quantize_fp8(x, block_rows=1, transposed=False, stream=None):
     block with an infinity or a NaN becomes NaN throughout.
 
     ``transposed=True``: ``(q, scale, qt, scale_t)``, with the transpose ``qt [K, M]`` as well, from one reading of ``x``; with
-    ``block_rows=1`` it is quantised anew, in blocks of 128 along M (``scale_t [K, ceil(M / 128)]``).  Not differentiable."""
+    ``block_rows=1`` it is quantised anew, in blocks of 128 along M (``scale_t [K, ceil(M / 128)]``).  K is at most 65535 * 128.
+    Not differentiable."""
     q, scale, qt, scale_t = _quantize(x, block_rows, transposed, stream)
     M, K = x.shape
     out = (q[:, :K], scale.t() if block_rows == 1 else scale)
@@ -91,5 +93,7 @@ def linear_fp8(x, weight, bias=None):
         raise ValueError("shapes: x [..., K], weight [N, K], bias [N]")
     if weight.shape[1] == 0:
         raise ValueError("a layer without input features")
+    if x.numel() // x.shape[-1] > _MOST_ROWS or max(weight.shape) > _MOST_COLUMNS:
+        raise ValueError(f"at most {_MOST_ROWS} tokens and {_MOST_COLUMNS} features")
     _call("linear_fp8_backward", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")
     return _LinearFp8.apply(x, weight, bias)

@@ -477,6 +477,17 @@ def test_cpu_tensors_are_refused():
 
 
 @pytest.mark.gpu
+def test_sizes_behind_32_bit_indices_are_refused():
+    one = torch.zeros(1, device="cuda")   # matrices that are one element over and over
+    w = torch.zeros(8, 16, device="cuda")
+    for bad in (lambda: quantize_fp8(torch.zeros(1, 65535 * 128 + 1, device="cuda")),
+                lambda: linear_fp8(one.expand(2**31, 16), w), lambda: linear_fp8(one.expand(2**16, 2**15, 16), w),
+                lambda: linear_fp8(w, one.expand(65535 * 128 + 1, 16))):
+        with pytest.raises(ValueError, match="at most"):
+            bad()
+
+
+@pytest.mark.gpu
 def test_refusals():
     x = torch.zeros(40, 256, device="cuda")
     for bad, error in ((lambda: quantize_fp8(x.double()), TypeError), (lambda: quantize_fp8(x.t()), ValueError), (lambda: quantize_fp8(x[0]), ValueError),
