@@ -215,6 +215,29 @@ def test_layouts_give_one_result(dtype):
 
 
 @pytest.mark.gpu
+def test_offsets_behind_32_bits():
+    """Logits of more than 2^31 elements, and rows so far apart that offsets pass it: the last rows' losses and gradients are those of these rows alone."""
+    T, V, K = 43000, 50257, 5
+    few, ids, top = (t.detach() for t in _case((6,), V, K, torch.bfloat16, seed=11))
+    logits = torch.zeros(T, V, dtype=torch.bfloat16, device="cuda")
+    logits[-6:] = few
+    all_ids, all_top = torch.full((T, K), -1, device="cuda"), torch.zeros(T, K, device="cuda")
+    all_ids[-6:], all_top[-6:] = ids, top
+    few = few.requires_grad_()
+    want = distillation_loss(few, ids, top, 2.0, "none")
+    dwant, = torch.autograd.grad(want.sum(), [few])
+    far = torch.empty(5 * 2**29 + V, dtype=torch.bfloat16, device="cuda").as_strided((6, V), (2**29, 1))
+    far.copy_(few.detach())
+    for z, i, t in ((logits, all_ids, all_top), (far, ids, top)):
+        z = z.requires_grad_()
+        got = distillation_loss(z, i, t, 2.0, "none")
+        d, = torch.autograd.grad(got.sum(), [z])
+        assert torch.allclose(got[-6:], want, rtol=1e-5) and not got[:-6].any()
+        assert torch.allclose(d[-6:].float(), dwant.float(), rtol=2 * torch.finfo(torch.bfloat16).eps, atol=1e-7)
+        assert len(d) == 6 or not d[:1000].any() and not d[-1006:-6].any()
+
+
+@pytest.mark.gpu
 def test_captured_and_replayed():
     logits, ids, top = (t.detach() for t in _case((40,), 4001, 9, torch.bfloat16, seed=4))
     z, i, t = torch.zeros_like(logits).requires_grad_(), torch.zeros_like(ids), torch.zeros_like(top)

@@ -255,6 +255,28 @@ def test_products_of_nothing_on_other_streams_and_in_graphs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M", [3, 40, 600])
+def test_offsets_behind_32_bits(M):
+    """Rows so far apart that the last element's offset passes 2^31 elements (and, for what is not 8 bits, 2^32 bytes)."""
+    step = -(-(2**31 + 4096) // (M - 1) // 16) * 16 + 16
+
+    def apart(t):
+        far = torch.empty((M - 1) * step + t.shape[1], dtype=t.dtype, device="cuda").as_strided(t.shape, (step, 1))
+        return far.copy_(t) if t.dtype != E4M3 else far.view(torch.uint8).copy_(t.view(torch.uint8)).view(E4M3)
+
+    x, b = torch.randn(M, 520, device="cuda", dtype=torch.bfloat16), torch.randn(1100, 520, device="cuda")
+    q, s, qt, st = quantize_fp8(x, transposed=True)
+    for got, want in zip(quantize_fp8(apart(x), transposed=True), (q, s, qt, st)):
+        assert torch.equal(got.float(), want.float())
+    w, ws = quantize_fp8(b, block_rows=128)
+    want = gemm_fp8(q, s, w, ws)
+    assert torch.equal(gemm_fp8(apart(q), s, w, ws), want)
+    out = apart(torch.zeros_like(want))
+    assert torch.equal(gemm_fp8(q, s, w, ws, out=out), want) and out.stride(0) == step
+    assert torch.equal(gemm_fp8(w, ws, apart(q), s), gemm_fp8(w, ws, q, s))
+
+
+@pytest.mark.gpu
 def test_first_product_of_a_process_may_be_captured():
     """What a product needs once for each process (the word for waits that ran out) is made without breaking a capture that is under way."""
     code = """
