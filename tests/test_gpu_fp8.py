@@ -395,6 +395,41 @@ def test_linear_strides_hooks_autocast_and_nothing():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,n,k", [(2, 256, 384), (40, 300, 264), (1100, 1288, 520)])
+def test_linear_step_captured_and_replayed_on_two_streams(tokens, n, k):
+    torch.manual_seed(tokens)
+    steps = []
+    for _ in range(2):
+        x, w, b = (torch.randn(*shape, device="cuda", dtype=torch.bfloat16).requires_grad_() for shape in ((tokens, k), (n, k), (n,)))
+        grad = torch.randn(tokens, n, device="cuda", dtype=torch.bfloat16)
+
+        def step(x=x, w=w, b=b, grad=grad):
+            y = linear_fp8(x, w, b)
+            return [y.detach(), *torch.autograd.grad(y, [x, w, b], grad)]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results = step()
+        with torch.no_grad():
+            for t in (x, w, b, grad):
+                t.normal_()
+        steps.append((graph, results, step, side))
+    torch.cuda.synchronize()
+    for _ in range(10):   # both at once, over and over
+        for graph, _, _, side in steps:
+            with torch.cuda.stream(side):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, results, step, _ in steps:
+        assert all(torch.equal(got, want) for got, want in zip(results, step()))
+
+
+@pytest.mark.gpu
 def test_calls_through_ctypes_do_the_same():
     """What stands in for the extension where that cannot be built."""
     import mini_nccl_b200 as mn
