@@ -69,17 +69,20 @@ constexpr int kPitch = 33;                                     // floats of a sc
 template <int BN>
 constexpr int kPairStage = kTileBytes + BN / 2 * kBlockK;      // this CTA's 128 rows of A and BN / 2 rows of B
 
-constexpr int kStages = 5;
+constexpr int kStages = 5;                                     // (seven for the narrow tiles, which shared memory would hold, changed nothing)
 template <int BN, bool B_ROWS>
 constexpr int kCols = B_ROWS ? BN : 4;                         // scales of B a block: of the tile's columns, or of the two blocks of rows that a half touches
 template <int BN, bool B_ROWS>
 constexpr int kSlot = kGroup * (128 + kCols<BN, B_ROWS>);      // floats: a group's scales
 
+template <int BN>
+constexpr uint32_t kBuffers = BN <= 128 ? 4 : 2;               // accumulators in tensor memory (256 x 4096 x 4096 with 128 columns: 16.2 -> 15.4 us)
+
 struct __align__(16) PairCtl {
   uint64_t full[kStages];        // used in the leader: 2 arrivals (one per producer) and both CTAs' bytes
   uint64_t empty[kStages];       // one per CTA, released by the leader's two commits
-  uint64_t acc_full[2][2];       // [accumulator][half of the tile's columns], one per CTA
-  uint64_t acc_empty[2][2];      // used in the leader: the half's four promotion warps of both CTAs
+  uint64_t acc_full[4][2];       // [accumulator][half of the tile's columns], one per CTA
+  uint64_t acc_empty[4][2];      // used in the leader: the half's four promotion warps of both CTAs
   uint64_t scales_full[2];       // 32 arrivals: the lanes of the warp that brings them
   uint64_t scales_empty[2];      // the promotion warps
   uint32_t tmem_base;
@@ -179,6 +182,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
                      const __grid_constant__ Args g, bool mapped) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int NS = kStages, NC = BN / 2;
+  constexpr uint32_t NB = kBuffers<BN>;
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
@@ -203,7 +207,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
       mbar_init(smem_u32(&ctl->scales_full[b]), 32);
       mbar_init(smem_u32(&ctl->scales_empty[b]), kPromoters);
     }
-    for (int b = 0; b < 4; ++b) {
+    for (int b = 0; b < 2 * static_cast<int>(NB); ++b) {
       mbar_init(smem_u32(&ctl->acc_full[b >> 1][b & 1]), 1);
       mbar_init(smem_u32(&ctl->acc_empty[b >> 1][b & 1]), kPromoters);
     }
@@ -267,7 +271,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
         bool ok = true;
         for (int t = pair; t < num_tiles && ok; t += n_pairs) {
           for (int kb = 0; kb < num_kb; ++kb, ++it) {
-            const uint32_t buf = it & 1u, acc_ph = (it >> 1) & 1u;
+            const uint32_t buf = it % NB, acc_ph = it / NB & 1u;
             ok = mbar_wait_both(full + s * 8u, ph, acc_empty + buf * 16u, acc_ph ^ 1u, &ctl->abort, budget);
             if (!ok) break;
             tc_fence_after_sync();
@@ -275,7 +279,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
             if (leader) {
 #pragma unroll
               for (int k = 0; k < kBlockK / kMmaK; ++k)   // 32 bytes on inside a 128-byte swizzle row: +2 in the address field
-                umma_e4m3_pair(tmem_base + buf * 256u + half * NC, da + static_cast<uint64_t>(k * 2), db + static_cast<uint64_t>(k * 2), idesc, k != 0 ? 1u : 0u);
+                umma_e4m3_pair(tmem_base + buf * (kTmemCols / NB) + half * NC, da + static_cast<uint64_t>(k * 2), db + static_cast<uint64_t>(k * 2), idesc, k != 0 ? 1u : 0u);
               umma_commit_pair(acc_full + buf * 16u, 3);
               umma_commit_pair(empty + s * 8u, 3);   // with the other half's: the stage is free in both CTAs
             }
@@ -367,13 +371,13 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
           x[0] = r * cols[0];
           x[1] = r * cols[1];
         }
-        const uint32_t buf = it & 1u, acc_ph = (it >> 1) & 1u;
+        const uint32_t buf = it % NB, acc_ph = it / NB & 1u;
         ++it;
         ok = __all_sync(0xffffffffu, ready) || mbar_wait_warp(acc_full + buf * 16u, acc_ph, &ctl->abort, budget);
         if (!ok) break;
         tc_fence_after_sync();
         promote<NC, B_ROWS ? 32 : 64>(
-            taddr + buf * 256u,
+            taddr + buf * (kTmemCols / NB),
             [&](int c, const auto& v) {
               constexpr int kPiece = sizeof(v) / 4;
               if constexpr (B_ROWS) {
@@ -398,7 +402,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
               tc_fence_before_sync();
               __syncwarp();
               if (lane == 0) mbar_arrive_cluster(acc_empty + buf * 16u);
-              ready = mbar_test(acc_full + (buf ^ 1u) * 16u, (it >> 1) & 1u);   // the next block: its answer is there when the sums are done
+              ready = mbar_test(acc_full + it % NB * 16u, it / NB & 1u);   // the next block: its answer is there when the sums are done
             });
         if (i == kGroup - 1 || kb + 1 == num_kb) {   // this group's scales have been read
           __syncwarp();
@@ -483,16 +487,16 @@ bool make_tensor_map_out(CUtensorMap* map, const Args& g) {
 }
 
 // The tile width with the least estimated time (ns): a wave of tiles takes about two microseconds and so much a block of K, more with a scale for
-// every row of B (measured, us without / with those: 512 x 1024 x 1024, one wave of 128, 7.7 / 8.5; 1001 x 1288 x 5000 19.1 / 22.0; 1001 x
-// 5000 x 1288, two of 192, 17.7 / 20.7; 4096 x 4096 x 4096, four of 256, 67 / 101; 8192 x 4096 x 1024, seven of 256, 41).  Rows of C that the TMA unit cannot
-// write cost a wave of 128 columns three more (777 x 1003 x 1544 13.1, 777 x 1000 x 1544 10.1).  A narrower tile pays where it saves a wave or leaves fewer
-// SMs idle.
+// every row of B (measured, us without / with those: 256 x 4096 x 4096, one wave of 64, 13.5 / 14.4, and of 128, 15.4 / 18.0; 1001 x 1288 x 5000,
+// one of 128, 18.3 / 21.5; 1001 x 5000 x 1288, two of 192, 17.6 / 21.0; 4096 x 4096 x 4096, four of 256, 67 / 101; 8192 x 4096 x 1024, seven of 256,
+// 41).  Rows of C that the TMA unit cannot write cost a wave of 128 columns three more (777 x 1003 x 1544 with 128: 13.1, 777 x 1000 x 1544 10.1; with 64:
+// 10.3 and 8.4).  A narrower tile pays where it saves a wave or leaves fewer SMs idle; 64 columns on all SMs read 10 TB/s from the L2.
 int pick_width(int M, int N, int K, bool b_rows, bool mapped, int pairs, long* ns) {
   struct Width {
     int bn;
     long per_block, per_block_rows;
   };
-  constexpr Width kWidths[] = {{256, 430, 720}, {192, 390, 560}, {128, 355, 423}};
+  constexpr Width kWidths[] = {{256, 430, 720}, {192, 390, 560}, {128, 330, 400}, {64, 245, 280}};
   const long num_kb = (K + kBlockK - 1) / kBlockK;
   int best = 256;
   *ns = -1;
@@ -547,7 +551,8 @@ int run(const void* a, int64_t lda, const void* b, int64_t ldb, Args g, cudaStre
         switch (bn) {
           case 256: return fire<256, R>(ta, tb, tc, mapped, g, static_cast<int>(tiles), stream);
           case 192: return fire<192, R>(ta, tb, tc, mapped, g, static_cast<int>(tiles), stream);
-          default: return fire<128, R>(ta, tb, tc, mapped, g, static_cast<int>(tiles), stream);
+          case 128: return fire<128, R>(ta, tb, tc, mapped, g, static_cast<int>(tiles), stream);
+          default: return fire<64, R>(ta, tb, tc, mapped, g, static_cast<int>(tiles), stream);
         }
       };
       e = g.b.shift == 0 ? go(std::true_type{}) : go(std::false_type{});

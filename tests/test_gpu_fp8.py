@@ -142,7 +142,7 @@ SHAPES = [(1, 1, 1), (1, 128, 128), (1, 129, 4096), (2, 64, 72), (15, 300, 136),
           (127, 1024, 1024), (129, 640, 320), (256, 256, 256), (255, 4096, 129), (300, 300, 14336), (777, 1003, 1544), (1024, 2048, 512), (2000, 130, 700),
           (4096, 3584, 384), (5, 50257, 128), (8192, 136, 200),
           (1, 4096, 4096), (1, 77, 9001), (2, 1001, 1031), (3, 600, 129), (4, 1024, 2048), (4, 4096, 4096), (1, 14336, 4096),
-          (20, 2048, 2048), (24, 8192, 8192), (32, 4096, 4096), (64, 4096, 4096), (512, 1024, 4096), (600, 1024, 300), (1001, 5000, 1288), (5000, 1288, 1001)]
+          (20, 2048, 2048), (64, 2048, 2048), (24, 8192, 8192), (32, 4096, 4096), (64, 4096, 4096), (512, 1024, 4096), (600, 1024, 300), (1001, 5000, 1288), (5000, 1288, 1001)]
 
 
 def _plan(M, N, K, b_rows=128):
@@ -156,7 +156,7 @@ def _plan(M, N, K, b_rows=128):
 def test_the_shapes_reach_every_kernel():
     plans = {_plan(*shape, b_rows) for shape in SHAPES for b_rows in (1, 128)}
     assert {t for kind, t, _ in plans if kind == 1} == {16, 32, 64} and {s for kind, _, s in plans if kind == 1} == {1, 2, 4, 8}
-    assert {t for kind, t, _ in plans if kind == 0} == {128, 192, 256}
+    assert {t for kind, t, _ in plans if kind == 0} == {64, 128, 192, 256}
     assert {M for M, N, K in SHAPES if _plan(M, N, K)[0] == 2} == {1, 2, 3, 4}
     assert _plan(0, 8, 8)[0] == -1 and _plan(8, 8, 8, 64)[0] == -1
     assert _plan(1, 4096, 4096)[0] == 2 and _plan(1, 14336, 4096)[:2] == (1, 16) and _plan(16, 14336, 4096)[:2] == (1, 16)
