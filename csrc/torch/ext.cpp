@@ -19,7 +19,11 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <optional>
 
@@ -382,10 +386,12 @@ bool matrix(const at::Tensor& t, const char* name, bool right_type, int64_t* ld)
   return false;
 }
 
-PyObject* failed(const char* what, int rc) {
-  PyErr_Format(PyExc_RuntimeError, "%s failed with code %d", what, rc);
-  return nullptr;
-}
+void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with code ", rc); }
+// The GIL is not held while one of these lives; what it covers may throw.
+struct NoGil {
+  PyThreadState* state = PyEval_SaveThread();
+  ~NoGil() { PyEval_RestoreThread(state); }
+};
 PyObject* wrap(const at::Tensor& t) { return t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None); }
 
 // A matrix in 8 bits as the kernels write it: rows padded to 16 bytes, scales [K blocks, M] (block_rows 1) or [M blocks, K blocks]; the
@@ -393,7 +399,7 @@ PyObject* wrap(const at::Tensor& t) { return t.defined() ? THPVariable_Wrap(t) :
 struct Quantized {
   at::Tensor q, scale, qt, scale_t, sums;
 };
-int quantize(const at::Tensor& x, int64_t ld, bool row, bool transposed, bool sums, cudaStream_t stream, Quantized* out) {
+void quantize(const at::Tensor& x, int64_t ld, bool row, bool transposed, bool sums, cudaStream_t stream, Quantized* out) {
   const int64_t M = x.size(0), K = x.size(1);
   const auto e4m3 = x.options().dtype(at::kFloat8_e4m3fn).requires_grad(false), f32 = x.options().dtype(at::kFloat).requires_grad(false);
   out->q = at::empty({M, padded(K)}, e4m3);
@@ -403,15 +409,12 @@ int quantize(const at::Tensor& x, int64_t ld, bool row, bool transposed, bool su
     if (row) out->scale_t = at::empty({blocks(M), K}, f32);
     if (sums) out->sums = at::empty({blocks(M), K}, f32);
   }
-  if (M == 0 || K == 0) return 0;
+  if (M == 0 || K == 0) return;
   const auto floats = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
-  int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = lib.quantize_fp8(x.data_ptr(), float_code(x), ld, static_cast<int>(M), static_cast<int>(K), row ? 1 : static_cast<int>(kBlock), out->q.data_ptr(),
-                        out->q.size(1), floats(out->scale), transposed ? out->qt.data_ptr() : nullptr, transposed ? out->qt.size(1) : 0, floats(out->scale_t),
-                        floats(out->sums), stream);
-  Py_END_ALLOW_THREADS
-  return rc;
+  check(lib.quantize_fp8(x.data_ptr(), float_code(x), ld, static_cast<int>(M), static_cast<int>(K), row ? 1 : static_cast<int>(kBlock), out->q.data_ptr(),
+                         out->q.size(1), floats(out->scale), transposed ? out->qt.data_ptr() : nullptr, transposed ? out->qt.size(1) : 0, floats(out->scale_t),
+                         floats(out->sums), stream),
+        "mncclQuantizeFp8");
 }
 
 // quantize_fp8(x, block_rows, transposed, stream | None) -> (q, scale, qt | None, scale_t | None), see Quantized
@@ -436,7 +439,10 @@ PyObject* quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   On o;
   if (!on(*x, args[3], &o)) return nullptr;
   Quantized q;
-  if (const int rc = quantize(*x, ld, block_rows == 1, transposed != 0, false, o.raw, &q)) return failed("mncclQuantizeFp8", rc);
+  {
+    NoGil free;
+    quantize(*x, ld, block_rows == 1, transposed != 0, false, o.raw, &q);
+  }
   return Py_BuildValue("(NNNN)", wrap(q.q), wrap(q.scale), wrap(q.qt), wrap(q.scale_t));
   END_HANDLE_TH_ERRORS
 }
@@ -527,7 +533,7 @@ PyObject* gemm_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
                       sb->stride(1), pb, out->data_ptr(), ldc, code, bias ? bias->data_ptr() : nullptr, static_cast<int>(M), static_cast<int>(N),
                       static_cast<int>(K), o.raw);
     Py_END_ALLOW_THREADS
-    if (rc != 0) return failed("mncclGemmFp8", rc);
+    check(rc, "mncclGemmFp8");
   }
   return fresh.defined() ? THPVariable_Wrap(fresh) : Py_NewRef(args[4]);
   END_HANDLE_TH_ERRORS
@@ -543,94 +549,169 @@ at::Tensor rows_of(const at::Tensor& t, int64_t cols, int64_t* ld) {
 }
 
 // out [M, N] = a * b^T (+ bias) of padded buffers: a [M, padded K] with scales [K blocks, M], b [N, padded K] with scales that have these strides.
-int product(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb, int64_t sb_row, int64_t sb_blk, int sb_rows, int64_t M, int64_t N,
-            int64_t K, const at::Tensor& out, const at::Tensor* bias, cudaStream_t stream) {
-  if (M == 0 || N == 0) return 0;
+void product(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb, int64_t sb_row, int64_t sb_blk, int sb_rows, int64_t M, int64_t N,
+             int64_t K, const at::Tensor& out, const at::Tensor& bias, cudaStream_t stream) {
+  if (M == 0 || N == 0) return;
   if (K == 0) {
     c10::AutoGradMode no_grad(false);
     out.zero_();
-    return 0;
+    return;
   }
-  int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = lib.gemm_fp8(a.data_ptr(), a.size(1), sa.data_ptr<float>(), 1, M, 1, b.data_ptr(), b.size(1), sb.data_ptr<float>(), sb_row, sb_blk, sb_rows, out.data_ptr(),
-                    N, float_code(out), bias ? bias->data_ptr() : nullptr, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), stream);
-  Py_END_ALLOW_THREADS
-  return rc;
+  check(lib.gemm_fp8(a.data_ptr(), a.size(1), sa.data_ptr<float>(), 1, M, 1, b.data_ptr(), b.size(1), sb.data_ptr<float>(), sb_row, sb_blk, sb_rows, out.data_ptr(),
+                     N, float_code(out), bias.defined() ? bias.data_ptr() : nullptr, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), stream),
+        "mncclGemmFp8");
 }
 
-// linear_fp8_forward(x [..., K], weight [N, K], bias [N] | None, want_x, want_w) -> (y [..., N], and for the backward pass x^T and its scales,
-// weight^T and the weight's scales, each None where it is not wanted); ops/fp8.py has checked the arguments
-PyObject* linear_fp8_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+// The backward pass of linear_fp8: x^T and its scales, weight^T and the weight's scales, each undefined where it is not wanted.
+struct LinearFp8Backward final : torch::autograd::Node {
+  SavedVariable xt, xt_scale, wt, w_scale;
+  std::vector<int64_t> x_sizes;
+  bool want_x = false, want_w = false;
+
+  std::string name() const override { return "LinearFp8Backward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&xt, &xt_scale, &wt, &w_scale}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list out(3);   // dx, dweight, dbias
+    if (!grads[0].defined()) return out;
+    const bool once = c10::GradMode::is_enabled();   // create_graph
+    {
+      c10::AutoGradMode no_grad(false);
+      const bool to_x = want_x && task_should_compute_output(0), to_w = want_w && task_should_compute_output(1), to_b = task_should_compute_output(2);
+      const at::Tensor grad = grads[0];
+      const c10::cuda::CUDAGuard device(grad.device());
+      const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
+      const int64_t N = grad.size(-1), K = x_sizes.back();
+      int64_t ld = 0;
+      const at::Tensor g = rows_of(grad, N, &ld);
+      const int64_t T = g.size(0);
+      const auto like = g.options().requires_grad(false);
+      if (N == 0) {   // a layer without output features
+        if (to_x) out[0] = at::zeros(x_sizes, like);
+        if (to_w) out[1] = at::zeros({N, K}, like);
+        if (to_b) out[2] = at::zeros({N}, like);
+        return out;
+      }
+      Quantized q;
+      quantize(g, ld, true, to_w || to_b, to_b, stream, &q);
+      if (to_x) {   // rows of weight^T are columns of the weight
+        const at::Tensor t = wt.unpack().contiguous(), s = w_scale.unpack().contiguous();
+        out[0] = at::empty(x_sizes, like);
+        product(q.q, q.scale, t, s, 1, s.size(1), static_cast<int>(kBlock), T, K, N, out[0], at::Tensor(), stream);
+      }
+      if (to_w) {
+        const at::Tensor t = xt.unpack().contiguous(), s = xt_scale.unpack().contiguous();
+        out[1] = at::empty({N, K}, like);
+        product(q.qt, q.scale_t, t, s, 1, K, 1, N, K, T, out[1], at::Tensor(), stream);
+      }
+      if (to_b) {
+        out[2] = T > 0 ? at::empty({N}, like) : at::zeros({N}, like);
+        if (T > 0)
+          check(lib.sum_blocks(q.sums.data_ptr<float>(), static_cast<int>(q.sums.size(0)), static_cast<int>(N), out[2].data_ptr(), float_code(out[2]), stream),
+                "mncclSumBlocks");
+      }
+    }
+    if (!once) return out;
+    // differentiable once: what is made of these gradients may not be differentiated
+    for (at::Tensor& t : out)
+      if (t.defined()) t = t.detach().requires_grad_(true);
+    return torch::autograd::DelayedError("trying to differentiate linear_fp8 twice", static_cast<int64_t>(out.size())).apply(std::move(out));
+  }
+};
+
+// linear_fp8(x [..., K], weight [N, K], bias [N] | None) -> y [..., N]; ops/fp8.py has checked the arguments
+PyObject* linear_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arg_count(n, 5)) return nullptr;
+  if (!arg_count(n, 3)) return nullptr;
   const at::Tensor *x = tensor_arg(args[0], "x"), *weight = x ? tensor_arg(args[1], "weight") : nullptr, *bias = nullptr;
   if (!weight || (args[2] != Py_None && !(bias = tensor_arg(args[2], "bias")))) return nullptr;
-  const bool want_x = args[3] == Py_True, want_w = args[4] == Py_True;
   On o;
   if (!on(*x, Py_None, &o)) return nullptr;
-  const int64_t N = weight->size(0), K = weight->size(1);
-  int64_t ldx = 0, ldw = 0;
-  const at::Tensor rows = rows_of(*x, K, &ldx), w = rows_of(*weight, K, &ldw), dense = bias ? bias->contiguous() : at::Tensor();
-  Quantized qx, qw;
-  if (const int rc = quantize(rows, ldx, true, want_w, false, o.raw, &qx)) return failed("mncclQuantizeFp8", rc);
-  if (const int rc = quantize(w, ldw, false, want_x, false, o.raw, &qw)) return failed("mncclQuantizeFp8", rc);
-  auto shape = x->sizes().vec();
-  shape.back() = N;
-  at::Tensor y = at::empty(shape, x->options().requires_grad(false));
-  if (const int rc = product(qx.q, qx.scale, qw.q, qw.scale, qw.scale.size(1), 1, static_cast<int>(kBlock), rows.size(0), N, K, y, bias ? &dense : nullptr, o.raw))
-    return failed("mncclGemmFp8", rc);
-  return Py_BuildValue("(NNNNN)", wrap(y), wrap(qx.qt), wrap(qx.scale_t), wrap(qw.qt), wrap(want_x ? qw.scale : at::Tensor()));
-  END_HANDLE_TH_ERRORS
-}
-
-// linear_fp8_backward(grad [..., N], xt | None, xt_scale | None, wt | None, w_scale | None, K, want_bias) -> (dx [tokens, K] | None, dweight [N, K] | None,
-// dbias [N] | None); xt .. w_scale as the forward call gave them
-PyObject* linear_fp8_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  if (!arg_count(n, 7)) return nullptr;
-  const at::Tensor *grad = tensor_arg(args[0], "grad"), *t[4] = {};
-  if (!grad) return nullptr;
-  for (int i = 0; i < 4; ++i)
-    if (args[i + 1] != Py_None && !(t[i] = tensor_arg(args[i + 1], "argument"))) return nullptr;
-  const int64_t K = PyLong_AsLongLong(args[5]);
-  if (PyErr_Occurred()) return nullptr;
-  const bool want_bias = args[6] == Py_True;
-  On o;
-  if (!on(*grad, Py_None, &o)) return nullptr;
-  const int64_t N = grad->size(-1);
-  int64_t ld = 0;
-  const at::Tensor g = rows_of(*grad, N, &ld);
-  const int64_t T = g.size(0);
-  const auto like = g.options().requires_grad(false);
-  Quantized q;
-  if (const int rc = quantize(g, ld, true, t[0] || want_bias, want_bias, o.raw, &q)) return failed("mncclQuantizeFp8", rc);
-  at::Tensor dx, dw, db;
-  if (t[2]) {
-    dx = at::empty({T, K}, like);
-    const at::Tensor &wt = *t[2], &ws = *t[3];   // rows of weight^T are columns of the weight
-    if (const int rc = product(q.q, q.scale, wt, ws, 1, ws.size(1), static_cast<int>(kBlock), T, K, N, dx, nullptr, o.raw)) return failed("mncclGemmFp8", rc);
-  }
-  if (t[0]) {
-    dw = at::empty({N, K}, like);
-    if (const int rc = product(q.qt, q.scale_t, *t[0], *t[1], 1, K, 1, N, K, T, dw, nullptr, o.raw)) return failed("mncclGemmFp8", rc);
-  }
-  if (want_bias) {
-    db = T > 0 ? at::empty({N}, like) : at::zeros({N}, like);
-    if (T > 0 && N > 0) {
-      int rc;
-      Py_BEGIN_ALLOW_THREADS
-      rc = lib.sum_blocks(q.sums.data_ptr<float>(), static_cast<int>(q.sums.size(0)), static_cast<int>(N), db.data_ptr(), float_code(db), o.raw);
-      Py_END_ALLOW_THREADS
-      if (rc != 0) return failed("mncclSumBlocks", rc);
+  at::Tensor y;
+  {
+    NoGil free;
+    const at::Tensor b = bias ? *bias : at::Tensor();
+    const bool grad = c10::GradMode::is_enabled(), want_x = grad && x->requires_grad(), want_w = grad && weight->requires_grad();
+    const bool any = want_x || want_w || (grad && b.defined() && b.requires_grad());
+    Quantized qx, qw;
+    {
+      c10::AutoGradMode no_grad(false);
+      const int64_t N = weight->size(0), K = weight->size(1);
+      int64_t ldx = 0, ldw = 0;
+      const at::Tensor rows = rows_of(*x, K, &ldx), w = rows_of(*weight, K, &ldw), dense = b.defined() ? b.contiguous() : b;
+      quantize(rows, ldx, true, want_w, false, o.raw, &qx);
+      quantize(w, ldw, false, want_x, false, o.raw, &qw);
+      auto shape = x->sizes().vec();
+      shape.back() = N;
+      y = at::empty(shape, x->options().requires_grad(false));
+      product(qx.q, qx.scale, qw.q, qw.scale, qw.scale.size(1), 1, static_cast<int>(kBlock), rows.size(0), N, K, y, dense, o.raw);
+    }
+    if (any) {
+      std::shared_ptr<LinearFp8Backward> node(new LinearFp8Backward(), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(*x, *weight, b));
+      node->want_x = want_x;
+      node->want_w = want_w;
+      node->x_sizes = x->sizes().vec();
+      if (want_w) {
+        node->xt = SavedVariable(qx.qt, false);
+        node->xt_scale = SavedVariable(qx.scale_t, false);
+      }
+      if (want_x) {
+        node->wt = SavedVariable(qw.qt, false);
+        node->w_scale = SavedVariable(qw.scale, false);
+      }
+      torch::autograd::set_history(y, node);
     }
   }
-  return Py_BuildValue("(NNN)", wrap(dx), wrap(dw), wrap(db));
+  return wrap(y);
   END_HANDLE_TH_ERRORS
 }
 
-// distill_forward(logits [..., V], ids [T, K], top [T, K], tau, reduction) -> (loss, p, stats, counts, tokens); reduction: 0 a loss for each row, 1 their
-// sum, 2 their mean.  ops/distill.py has checked the arguments
+// A loss and what its backward pass needs.
+struct Distilled {
+  at::Tensor loss, p, stats, counts, tokens;
+};
+// reduction: 0 a loss for each row, 1 their sum, 2 their mean
+Distilled distill(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& top, double tau, long reduction, cudaStream_t stream) {
+  const int64_t V = logits.size(-1);
+  int64_t ld = 0;
+  const at::Tensor rows = rows_of(logits, V, &ld);
+  const int64_t T = rows.size(0), K = ids.size(1);
+  const auto f32 = rows.options().dtype(at::kFloat).requires_grad(false);
+  Distilled d{at::empty({}, f32), at::empty({T, K}, f32), at::empty({T, 2}, f32), at::empty({T}, f32.dtype(at::kInt)), at::empty({}, f32)};
+  const at::Tensor row_loss = at::empty(logits.sizes().slice(0, logits.dim() - 1), f32);
+  check(lib.distill_forward(rows.data_ptr(), float_code(rows), ld, static_cast<int>(T), static_cast<int>(V), ids.data_ptr<int64_t>(), top.data_ptr<float>(),
+                            static_cast<int>(K), static_cast<float>(tau), d.p.data_ptr<float>(), d.stats.data_ptr<float>(), row_loss.data_ptr<float>(),
+                            d.counts.data_ptr<int>(), reduction == 1 ? d.loss.data_ptr<float>() : nullptr, reduction == 2 ? d.loss.data_ptr<float>() : nullptr,
+                            d.tokens.data_ptr<float>(), stream),
+        "mncclDistillForward");
+  if (reduction == 0) d.loss = row_loss;
+  return d;
+}
+// The gradient of the logits, for a gradient of each row's loss or of their sum; tokens: what it is divided by, if defined.
+at::Tensor distill_gradient(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& p, const at::Tensor& stats, const at::Tensor& counts,
+                            const at::Tensor& tokens, double tau, const at::Tensor& of_loss, cudaStream_t stream) {
+  const int64_t V = logits.size(-1);
+  int64_t ld = 0;
+  const at::Tensor rows = rows_of(logits, V, &ld), grad = of_loss.contiguous();
+  // the gradient's rows lie to 16 bytes as the logits' do: padded where those are
+  const int64_t T = rows.size(0), per = 16 / rows.element_size(), ldd = rows.stride(0) != V ? (V + per - 1) / per * per : V;
+  at::Tensor d = at::empty({T, ldd}, rows.options().requires_grad(false));
+  check(lib.distill_backward(rows.data_ptr(), float_code(rows), ld, static_cast<int>(T), static_cast<int>(V), ids.data_ptr<int64_t>(), p.data_ptr<float>(),
+                             static_cast<int>(ids.size(1)), static_cast<float>(tau), stats.data_ptr<float>(), counts.data_ptr<int>(), grad.data_ptr<float>(),
+                             grad.dim() > 0 ? 1 : 0, tokens.defined() ? tokens.data_ptr<float>() : nullptr, d.data_ptr(), ldd, stream),
+        "mncclDistillBackward");
+  if (ldd != V) d = d.slice(1, 0, V);
+  return logits.dim() == 2 ? d : d.view(logits.sizes());
+}
+
+// distill_forward(logits [..., V], ids [T, K], top [T, K], tau, reduction) -> (loss, p, stats, counts, tokens); ops/distill.py has checked the arguments
 PyObject* distill_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arg_count(n, 5)) return nullptr;
@@ -641,54 +722,111 @@ PyObject* distill_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   On o;
   if (!on(*logits, Py_None, &o)) return nullptr;
-  const int64_t V = logits->size(-1);
-  int64_t ld = 0;
-  const at::Tensor rows = rows_of(*logits, V, &ld);
-  const int64_t T = rows.size(0), K = ids->size(1);
-  const auto f32 = rows.options().dtype(at::kFloat).requires_grad(false);
-  at::Tensor p = at::empty({T, K}, f32), stats = at::empty({T, 2}, f32), counts = at::empty({T}, f32.dtype(at::kInt)), tokens = at::empty({}, f32),
-             row_loss = at::empty(logits->sizes().slice(0, logits->dim() - 1), f32), loss = at::empty({}, f32);
-  int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = lib.distill_forward(rows.data_ptr(), float_code(rows), ld, static_cast<int>(T), static_cast<int>(V), ids->data_ptr<int64_t>(), top->data_ptr<float>(),
-                           static_cast<int>(K), static_cast<float>(tau), p.data_ptr<float>(), stats.data_ptr<float>(), row_loss.data_ptr<float>(),
-                           counts.data_ptr<int>(), reduction == 1 ? loss.data_ptr<float>() : nullptr, reduction == 2 ? loss.data_ptr<float>() : nullptr,
-                           tokens.data_ptr<float>(), o.raw);
-  Py_END_ALLOW_THREADS
-  if (rc != 0) return failed("mncclDistillForward", rc);
-  return Py_BuildValue("(NNNNN)", wrap(reduction == 0 ? row_loss : loss), wrap(p), wrap(stats), wrap(counts), wrap(tokens));
+  Distilled d;
+  {
+    NoGil free;
+    d = distill(*logits, *ids, *top, tau, reduction, o.raw);
+  }
+  return Py_BuildValue("(NNNNN)", wrap(d.loss), wrap(d.p), wrap(d.stats), wrap(d.counts), wrap(d.tokens));
   END_HANDLE_TH_ERRORS
 }
 
-// distill_backward(logits [..., V], ids, p, stats, counts, tokens | None, tau, grad) -> gradient of the logits, for a gradient of each row's loss or of
-// their sum; tokens: what it is divided by
+// distill_backward(logits [..., V], ids, p, stats, counts, tokens | None, tau, grad) -> gradient of the logits
 PyObject* distill_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arg_count(n, 8)) return nullptr;
-  const at::Tensor* t[8] = {};
+  at::Tensor t[8];
   for (int i = 0; i < 8; ++i) {
     if (i == 6 || (i == 5 && args[i] == Py_None)) continue;
-    if (!(t[i] = tensor_arg(args[i], "argument"))) return nullptr;
+    const at::Tensor* given = tensor_arg(args[i], "argument");
+    if (!given) return nullptr;
+    t[i] = *given;
   }
   const double tau = PyFloat_AsDouble(args[6]);
   if (PyErr_Occurred()) return nullptr;
   On o;
-  if (!on(*t[0], Py_None, &o)) return nullptr;
-  const int64_t V = t[0]->size(-1);
-  int64_t ld = 0;
-  const at::Tensor rows = rows_of(*t[0], V, &ld), grad = t[7]->contiguous();
-  // the gradient's rows lie to 16 bytes as the logits' do: padded where those are
-  const int64_t T = rows.size(0), per = 16 / rows.element_size(), ldd = rows.stride(0) != V ? (V + per - 1) / per * per : V;
-  at::Tensor d = at::empty({T, ldd}, rows.options().requires_grad(false));
-  int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = lib.distill_backward(rows.data_ptr(), float_code(rows), ld, static_cast<int>(T), static_cast<int>(V), t[1]->data_ptr<int64_t>(), t[2]->data_ptr<float>(),
-                            static_cast<int>(t[1]->size(1)), static_cast<float>(tau), t[3]->data_ptr<float>(), t[4]->data_ptr<int>(), grad.data_ptr<float>(),
-                            grad.dim() > 0 ? 1 : 0, t[5] ? t[5]->data_ptr<float>() : nullptr, d.data_ptr(), ldd, o.raw);
-  Py_END_ALLOW_THREADS
-  if (rc != 0) return failed("mncclDistillBackward", rc);
-  if (ldd != V) d = d.slice(1, 0, V);
-  return wrap(t[0]->dim() == 2 ? d : d.view(t[0]->sizes()));
+  if (!on(t[0], Py_None, &o)) return nullptr;
+  at::Tensor d;
+  {
+    NoGil free;
+    d = distill_gradient(t[0], t[1], t[2], t[3], t[4], t[5], tau, t[7], o.raw);
+  }
+  return wrap(d);
+  END_HANDLE_TH_ERRORS
+}
+
+// What takes over where the gradient itself is to be differentiated (create_graph): f(logits, ids, top, tau, reduction, grad) -> gradient.  Held for
+// the life of the process.
+PyObject* distill_again = nullptr;
+
+struct DistillationBackward final : torch::autograd::Node {
+  SavedVariable logits, ids, top, p, stats, counts, tokens;
+  double tau = 1.0;
+  long reduction = 0;
+
+  std::string name() const override { return "DistillationBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&logits, &ids, &top, &p, &stats, &counts, &tokens}) v->reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
+    const at::Tensor z = logits.unpack();
+    if (c10::GradMode::is_enabled()) {
+      const at::Tensor i = ids.unpack(), t = top.unpack();
+      const PyGILState_STATE gil = PyGILState_Ensure();
+      at::Tensor got;
+      PyObject* r = distill_again ? PyObject_CallFunction(distill_again, "NNNdlN", wrap(z), wrap(i), wrap(t), tau, reduction, wrap(grads[0])) : nullptr;
+      if (r && THPVariable_Check(r)) got = THPVariable_Unpack(r);
+      Py_XDECREF(r);
+      if (!got.defined()) {
+        python_error e;
+        if (PyErr_Occurred()) e.persist();
+        PyGILState_Release(gil);
+        throw e;
+      }
+      PyGILState_Release(gil);
+      return {got};
+    }
+    const c10::cuda::CUDAGuard device(z.device());
+    return {distill_gradient(z, ids.unpack(), p.unpack(), stats.unpack(), counts.unpack(), reduction == 2 ? tokens.unpack() : at::Tensor(), tau, grads[0],
+                             c10::cuda::getCurrentCUDAStream().stream())};
+  }
+};
+
+// distillation(logits [..., V], ids [T, K], top [T, K], tau, reduction, again) -> loss, differentiable in the logits; again: see distill_again
+PyObject* distillation(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 6)) return nullptr;
+  const at::Tensor *logits = tensor_arg(args[0], "logits"), *ids = logits ? tensor_arg(args[1], "ids") : nullptr, *top = ids ? tensor_arg(args[2], "top") : nullptr;
+  if (!top) return nullptr;
+  const double tau = PyFloat_AsDouble(args[3]);
+  const long reduction = PyLong_AsLong(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!distill_again) distill_again = Py_NewRef(args[5]);
+  On o;
+  if (!on(*logits, Py_None, &o)) return nullptr;
+  Distilled d;
+  {
+    NoGil free;
+    d = distill(*logits, *ids, *top, tau, reduction, o.raw);
+    if (c10::GradMode::is_enabled() && logits->requires_grad()) {
+      std::shared_ptr<DistillationBackward> node(new DistillationBackward(), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(*logits));
+      node->tau = tau;
+      node->reduction = reduction;
+      node->logits = SavedVariable(*logits, false);
+      node->ids = SavedVariable(*ids, false);
+      node->top = SavedVariable(*top, false);
+      node->p = SavedVariable(d.p, false);
+      node->stats = SavedVariable(d.stats, false);
+      node->counts = SavedVariable(d.counts, false);
+      node->tokens = SavedVariable(d.tokens, false);
+      torch::autograd::set_history(d.loss, node);
+    }
+  }
+  return wrap(d.loss);
   END_HANDLE_TH_ERRORS
 }
 
@@ -706,8 +844,8 @@ PyMethodDef methods[] = {
     {"ag_gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(ag_gemm)), METH_FASTCALL, nullptr},
     {"quantize_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(quantize_fp8)), METH_FASTCALL, nullptr},
     {"gemm_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gemm_fp8)), METH_FASTCALL, nullptr},
-    {"linear_fp8_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear_fp8_forward)), METH_FASTCALL, nullptr},
-    {"linear_fp8_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear_fp8_backward)), METH_FASTCALL, nullptr},
+    {"linear_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear_fp8)), METH_FASTCALL, nullptr},
+    {"distillation", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(distillation)), METH_FASTCALL, nullptr},
     {"distill_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(distill_forward)), METH_FASTCALL, nullptr},
     {"distill_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(distill_backward)), METH_FASTCALL, nullptr},
     {"async_error", async_error, METH_O, nullptr},

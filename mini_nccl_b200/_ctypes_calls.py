@@ -6,6 +6,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _CODES = {torch.int8: 0, torch.uint8: 1, torch.int32: 2, torch.int64: 4, torch.float16: 6, torch.float32: 7, torch.float64: 8,
           torch.bfloat16: 9}
@@ -255,7 +256,8 @@ def _rows(t, cols):
     return t if (cols <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= cols) else t.contiguous()
 
 
-def linear_fp8_forward(lib, x, weight, bias, want_x, want_w):
+def _linear_forward(lib, x, weight, bias, want_x, want_w):
+    """y, and for the backward pass x^T and its scales, weight^T and the weight's scales, each None where it is not wanted."""
     N, K = weight.shape
     rows, w = _rows(x, K), _rows(weight, K)
     with _on(x.device, None) as s:
@@ -265,7 +267,7 @@ def linear_fp8_forward(lib, x, weight, bias, want_x, want_w):
     return y.view(*x.shape[:-1], N), qt, scale_t, wt, w_scale if want_x else None
 
 
-def linear_fp8_backward(lib, grad, xt, xt_scale, wt, w_scale, K, want_bias):
+def _linear_backward(lib, grad, xt, xt_scale, wt, w_scale, K, want_bias):
     N = grad.shape[-1]
     g = _rows(grad, N)
     T = g.shape[0]
@@ -274,13 +276,36 @@ def linear_fp8_backward(lib, grad, xt, xt_scale, wt, w_scale, K, want_bias):
         q, scale, qt, scale_t, sums = _quantize(lib, g, 1, xt is not None or want_bias, want_bias, s)
         if want_bias:
             db = torch.zeros(N, dtype=g.dtype, device=g.device)
-            if T and N:
+            if T:
                 _check(lib.mncclSumBlocks(sums.data_ptr(), sums.shape[0], N, db.data_ptr(), _FLOATS[db.dtype], s), "mncclSumBlocks")
     if wt is not None:
         dx = gemm_fp8(lib, q[:, :N], scale.t(), wt[:, :N], w_scale.t(), None, g.dtype, None, None)
     if xt is not None:
         dw = gemm_fp8(lib, qt[:, :T], scale_t.t(), xt[:, :T], xt_scale.t(), None, g.dtype, None, None)
     return dx, dw, db
+
+
+class _LinearFp8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, lib, x, weight, bias, grad):
+        want_x, want_w = (grad and want for want in ctx.needs_input_grad[1:3])
+        y, *kept = _linear_forward(lib, x, weight, bias, want_x, want_w)
+        ctx.save_for_backward(*kept)
+        ctx.lib, ctx.shape = lib, x.shape
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        if grad.shape[-1] == 0:   # a layer without output features
+            shapes = (ctx.shape, (0, ctx.shape[-1]), (0,))
+            return (None, *(grad.new_zeros(shape) if want else None for shape, want in zip(shapes, ctx.needs_input_grad[1:4])), None)
+        dx, dw, db = _linear_backward(ctx.lib, grad, *ctx.saved_tensors, ctx.shape[-1], ctx.needs_input_grad[3])
+        return None, None if dx is None else dx.view(ctx.shape), dw, db, None
+
+
+def linear_fp8(lib, x, weight, bias):
+    return _LinearFp8.apply(lib, x, weight, bias, torch.is_grad_enabled())
 
 
 def distill_forward(lib, logits, ids, top, tau, reduction):
@@ -307,12 +332,34 @@ def distill_backward(lib, logits, ids, p, stats, counts, tokens, tau, grad):
     return d[:, :V].view(logits.shape)
 
 
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, lib, logits, ids, top, tau, reduction, again):
+        loss, *kept = distill_forward(lib, logits, ids, top, tau, reduction)
+        ctx.save_for_backward(logits, ids, top, *kept)
+        ctx.rest = lib, tau, reduction, again
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad):
+        logits, ids, top, p, stats, counts, tokens = ctx.saved_tensors
+        lib, tau, reduction, again = ctx.rest
+        if torch.is_grad_enabled():
+            d = again(logits, ids, top, tau, reduction, grad)
+        else:
+            d = distill_backward(lib, logits, ids, p, stats, counts, tokens if reduction == 2 else None, tau, grad)
+        return None, d, None, None, None, None, None
+
+
+def distillation(lib, logits, ids, top, tau, reduction, again):
+    return _Distillation.apply(lib, logits, ids, top, tau, reduction, again)
+
+
 class Calls:
     """The extension's functions, bound to a loaded library."""
 
     def __init__(self, lib):
         from functools import partial
 
-        for f in (all_reduce, gemm, gemm_rs, ag_gemm, quantize_fp8, gemm_fp8, linear_fp8_forward, linear_fp8_backward,
-                  distill_forward, distill_backward):
+        for f in (all_reduce, gemm, gemm_rs, ag_gemm, quantize_fp8, gemm_fp8, linear_fp8, distill_forward, distill_backward, distillation):
             setattr(self, f.__name__, partial(f, lib))

@@ -10,7 +10,7 @@ import math
 import torch
 import torch.nn.functional as F
 
-from .fp8 import _FLOATS, _call
+from .fp8 import _FLOATS, _call, no_tangent
 from .gemm import gemm_bf16
 from .lm_loss import _MAX_ROWS, _eight, _pays, _plain, _transposed
 from .lm_loss import _rows as _dense_rows
@@ -57,22 +57,12 @@ def _again(ctx, inputs, f, grad):
     return [out.get(i) for i in range(len(inputs))]
 
 
-class _Distillation(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, top, tau, reduction):
-        loss, *kept = _forward(logits, ids, top, tau, reduction)
-        ctx.save_for_backward(logits, ids, top, *kept)
-        ctx.tau, ctx.reduction = tau, reduction
-        return loss
-
-    @staticmethod
-    def backward(ctx, grad):
-        logits, ids, top, *kept = ctx.saved_tensors
-        none = (None,) * 4
-        if torch.is_grad_enabled():
-            at = ids.view(*logits.shape[:-1], -1), top.view(*logits.shape[:-1], -1)
-            return (*_again(ctx, [logits], lambda z: _reference(z, *at, ctx.tau, ctx.reduction), grad), *none)
-        return (_backward(logits, ids, *kept, ctx.tau, ctx.reduction, grad), *none)
+def _gradient_again(logits, ids, top, tau, reduction, grad):
+    """The gradient of the logits by operators that can be differentiated."""
+    at = ids.view(*logits.shape[:-1], -1), top.view(*logits.shape[:-1], -1)
+    with torch.enable_grad():
+        z = logits.view_as(logits)
+        return torch.autograd.grad(_reference(z, *at, tau, _REDUCTIONS[reduction]), [z], grad, create_graph=True)[0]
 
 
 class _LmHeadDistillation(torch.autograd.Function):
@@ -120,11 +110,7 @@ def _native(logits, ids, top):
         return False
     if not (0 < ids.shape[-1] <= _MAX_ENTRIES and 0 < ids.numel() // ids.shape[-1] < 2**31 and 0 < logits.shape[-1] < 2**31 - 2**12) or not _plain_call():
         return False
-    return _no_tangent(logits)
-
-
-def _no_tangent(t):
-    return torch.autograd.forward_ad._current_level < 0 or torch.autograd.forward_ad.unpack_dual(t).tangent is None
+    return no_tangent(logits)
 
 
 def _arguments(shape, device, ids, top, temperature, reduction="mean"):
@@ -162,7 +148,8 @@ def distillation_loss(logits, top_ids, top_logits, temperature=1.0, reduction="m
     if not _native(logits, ids, top):
         return _reference(logits, ids, top, tau, reduction)
     K = ids.shape[-1]
-    return _Distillation.apply(logits, ids.reshape(-1, K).contiguous(), top.float().reshape(-1, K).contiguous(), tau, reduction)
+    return _call("distillation", "mncclDistillForward", "csrc/kernels/distill.cu")(
+        logits, ids.reshape(-1, K).contiguous(), top.float().reshape(-1, K).contiguous(), tau, _REDUCTIONS.index(reduction), _gradient_again)
 
 
 def lm_head_distillation(x, weight, top_ids, top_logits, temperature=1.0):
@@ -176,7 +163,7 @@ def lm_head_distillation(x, weight, top_ids, top_logits, temperature=1.0):
     native = (x.dim() >= 2 and x.dtype == weight.dtype == torch.bfloat16 and x.device == weight.device and _plain(x) and _plain(weight)
               and x.is_cuda and x.device.index == torch.cuda.current_device() and V >= 8 and d >= 8 and d % 8 == 0 and 0 < T
               and max(T, V) <= _MAX_ROWS and not torch.is_autocast_enabled() and _native(x, ids, top)
-              and _no_tangent(weight))
+              and no_tangent(weight))
     if not native or not _pays(T, V, d):
         return distillation_loss(F.linear(x, weight), ids, top, tau)
     K = ids.shape[-1]

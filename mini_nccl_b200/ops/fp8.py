@@ -7,7 +7,6 @@ scales, such as a checkpoint's.  Like :func:`gemm_bf16` these fail loudly where 
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .._lib import ext, lib
 
@@ -56,20 +55,9 @@ def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=None, bias=None, stream
     return _call("gemm_fp8", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")(a, a_scale, b, b_scale, out, out_dtype, bias, stream)
 
 
-class _LinearFp8(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias):
-        want_x, want_w = ctx.needs_input_grad[:2]
-        y, *kept = _call("linear_fp8_forward", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")(x, weight, bias, want_x, want_w)
-        ctx.save_for_backward(*kept)
-        ctx.shape = x.shape
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        dx, dw, db = _calls["linear_fp8_backward"](grad, *ctx.saved_tensors, ctx.shape[-1], ctx.needs_input_grad[2])
-        return None if dx is None else dx.view(ctx.shape), dw, db
+def no_tangent(t):
+    """Whether a tensor carries no forward-mode tangent."""
+    return torch.autograd.forward_ad._current_level < 0 or torch.autograd.forward_ad.unpack_dual(t).tangent is None
 
 
 def linear_fp8(x, weight, bias=None):
@@ -95,5 +83,6 @@ def linear_fp8(x, weight, bias=None):
         raise ValueError("a layer without input features")
     if x.numel() // x.shape[-1] > _MOST_ROWS or max(weight.shape) > _MOST_COLUMNS:
         raise ValueError(f"at most {_MOST_ROWS} tokens and {_MOST_COLUMNS} features")
-    _call("linear_fp8_backward", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")
-    return _LinearFp8.apply(x, weight, bias)
+    if torch._C._are_functorch_transforms_active() or not all(no_tangent(t) for t in (x, weight, bias) if t is not None):
+        raise RuntimeError("linear_fp8 has no rule for functional transforms and forward-mode differentiation")
+    return _call("linear_fp8", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")(x, weight, bias)

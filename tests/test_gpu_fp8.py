@@ -6,6 +6,7 @@ import sys
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from mini_nccl_b200.ops import gemm_fp8, linear_fp8, quantize_fp8
 
@@ -281,6 +282,7 @@ def test_first_product_of_a_process_may_be_captured():
     """What a product needs once for each process (the word for waits that ran out) is made without breaking a capture that is under way."""
     code = """
 import torch
+import torch.utils.checkpoint
 from mini_nccl_b200.ops import gemm_fp8
 a, s = torch.ones(16, 256, device="cuda").to(torch.float8_e4m3fn), torch.ones(16, 2, device="cuda")
 graph = torch.cuda.CUDAGraph()
@@ -389,6 +391,25 @@ def test_linear_strides_hooks_autocast_and_nothing():
     d, = torch.autograd.grad(linear_fp8(x, w).sum(), [x], create_graph=True)
     with pytest.raises(RuntimeError):
         d.float().sum().backward()
+    none = w[:0].detach().requires_grad_()   # a layer without output features
+    y = linear_fp8(x, none, w[:0, 0])
+    dx, dw = torch.autograd.grad(y, [x, none], torch.empty(60, 0, device="cuda", dtype=x.dtype))
+    assert y.shape == (60, 0) and dx.shape == x.shape and not dx.any() and dw.shape == (0, 256)
+    with torch.no_grad():
+        y = linear_fp8(x, w)
+    assert torch.equal(y, want[0]) and not y.requires_grad and y.grad_fn is None
+    with pytest.raises(RuntimeError, match="no rule"):
+        torch.func.vmap(lambda t: linear_fp8(t, w))(x)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="no rule"):
+            linear_fp8(torch.autograd.forward_ad.make_dual(x.detach(), grad[:, :1].expand(60, 256)), w)
+    y = linear_fp8(x, w)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+    x.grad = None
+    torch.utils.checkpoint.checkpoint(linear_fp8, x, w, use_reentrant=False).backward(grad)
+    assert torch.equal(x.grad, want[1])
 
 
 # ---- the binding
@@ -467,10 +488,25 @@ def test_calls_through_ctypes_do_the_same():
         for want_x, want_w, bias in ((True, True, b), (True, False, None), (False, True, b), (False, False, b)):
             results = []
             for c in (plain, ext):
-                y, *kept = c.linear_fp8_forward(x, w, bias, want_x, want_w)
-                results.append((y, *c.linear_fp8_backward(grad, *kept, 200, bias is not None)))
+                leaves = [t if t is None else t.detach().requires_grad_(want) for t, want in ((x, want_x), (w, want_w), (bias, True))]
+                y = c.linear_fp8(*leaves)
+                y.backward(grad)
+                results.append((y.detach(), *(None if t is None else t.grad for t in leaves)))
             assert all((a is None) == (q is None) and (a is None or torch.equal(a, q)) for a, q in zip(*results))
             assert [r is not None for r in results[0][1:]] == [want_x, want_w, bias is not None]
+    from mini_nccl_b200.ops.distill import _gradient_again
+
+    z, ids, top = torch.randn(4, 90, device="cuda"), torch.randint(0, 90, (4, 5), device="cuda"), torch.randn(4, 5, device="cuda")
+    for reduction in (0, 1, 2):
+        results = []
+        for c in (plain, ext):
+            leaf = z.detach().requires_grad_()
+            loss = c.distillation(leaf, ids, top, 2.0, reduction, _gradient_again)
+            first, = torch.autograd.grad(loss.sum(), [leaf], retain_graph=True)
+            dz, = torch.autograd.grad(loss.sum(), [leaf], create_graph=True)
+            results.append((loss.detach(), first, dz.detach(), *torch.autograd.grad(dz.square().sum(), [leaf])))
+        assert all(torch.equal(a, q) for a, q in zip(*results))
+        assert torch.allclose(results[0][1], results[0][2], rtol=1e-4, atol=1e-6)
     x = _input(70, 300, torch.bfloat16).cuda()
     for bad, error in ((lambda c: c.quantize_fp8(x.double(), 1, False, None), TypeError), (lambda c: c.quantize_fp8([1], 1, False, None), TypeError),
                        (lambda c: c.quantize_fp8(x, 2, False, None), ValueError), (lambda c: c.gemm_fp8(*args, None, torch.int8, None, None), TypeError),
