@@ -417,7 +417,7 @@ void quantize(const at::Tensor& x, int64_t ld, bool row, bool transposed, bool s
         "mncclQuantizeFp8");
 }
 
-// quantize_fp8(x, block_rows, transposed, stream | None) -> (q, scale, qt | None, scale_t | None), see Quantized
+// quantize_fp8(x, block_rows, transposed, stream | None) -> (q, scale) or (q, scale, qt, scale_t); see ops/fp8.py
 PyObject* quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!arg_count(n, 4)) return nullptr;
@@ -438,11 +438,21 @@ PyObject* quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   On o;
   if (!on(*x, args[3], &o)) return nullptr;
+  const int64_t M = x->size(0), K = x->size(1);
+  const bool row = block_rows == 1;
   Quantized q;
   {
     NoGil free;
-    quantize(*x, ld, block_rows == 1, transposed != 0, false, o.raw, &q);
+    c10::AutoGradMode no_grad(false);
+    quantize(*x, ld, row, transposed != 0, false, o.raw, &q);
+    if (q.q.size(1) != K) q.q = q.q.slice(1, 0, K);
+    if (transposed) {
+      if (q.qt.size(1) != M) q.qt = q.qt.slice(1, 0, M);
+      q.scale_t = row ? q.scale_t.t() : q.scale.t();
+    }
+    if (row) q.scale = q.scale.t();
   }
+  if (!transposed) return Py_BuildValue("(NN)", wrap(q.q), wrap(q.scale));
   return Py_BuildValue("(NNNN)", wrap(q.q), wrap(q.scale), wrap(q.qt), wrap(q.scale_t));
   END_HANDLE_TH_ERRORS
 }

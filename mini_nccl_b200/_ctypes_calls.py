@@ -201,7 +201,10 @@ def quantize_fp8(lib, x, block_rows, transposed, stream):
     if x.shape[1] > _MOST_COLUMNS:
         raise ValueError(f"x must have at most {_MOST_COLUMNS} columns")
     with _on(x.device, stream) as s:
-        return _quantize(lib, x, block_rows, transposed, False, s)[:4]
+        q, scale, qt, scale_t, _ = _quantize(lib, x, block_rows, transposed, False, s)
+    M, K = x.shape
+    out = (q[:, :K], scale.t() if block_rows == 1 else scale)
+    return out if not transposed else (*out, qt[:, :M], scale_t.t() if block_rows == 1 else scale.t())
 
 
 def _operand(t, name):

@@ -17,16 +17,12 @@ _calls = {}   # the extension's entry points, looked up on the first call
 
 
 def _call(name, symbol, source):
-    if name not in _calls:
+    call = _calls.get(name)
+    if call is None:
         if not hasattr(lib(), symbol):
             raise RuntimeError(f"libmini_nccl.so was built without {source}")
-        _calls[name] = getattr(ext(), name)
-    return _calls[name]
-
-
-def _quantize(x, block_rows, transposed, stream=None):
-    """Buffers with padded rows, [M, padded K] and [K, padded M], and scales as the kernels write them."""
-    return _call("quantize_fp8", "mncclQuantizeFp8", "csrc/kernels/fp8_quantize.cu")(x, block_rows, transposed, stream)
+        call = _calls[name] = getattr(ext(), name)
+    return call
 
 
 def quantize_fp8(x, block_rows=1, transposed=False, stream=None):
@@ -40,10 +36,7 @@ def quantize_fp8(x, block_rows=1, transposed=False, stream=None):
     ``transposed=True``: ``(q, scale, qt, scale_t)``, with the transpose ``qt [K, M]`` as well, from one reading of ``x``; with
     ``block_rows=1`` it is quantised anew, in blocks of 128 along M (``scale_t [K, ceil(M / 128)]``).  K is at most 65535 * 128.
     Not differentiable."""
-    q, scale, qt, scale_t = _quantize(x, block_rows, transposed, stream)
-    M, K = x.shape
-    out = (q[:, :K], scale.t() if block_rows == 1 else scale)
-    return out if not transposed else (*out, qt[:, :M], scale_t.t() if block_rows == 1 else scale.t())
+    return _call("quantize_fp8", "mncclQuantizeFp8", "csrc/kernels/fp8_quantize.cu")(x, block_rows, transposed, stream)
 
 
 def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=None, bias=None, stream=None):
