@@ -65,7 +65,6 @@ constexpr int kOutRow = 64;                                    // bytes of a row
 constexpr int kPieceBytes = 32 * kOutRow;
 constexpr int kScratchBytes = 2 * kPieceBytes;                 // per promotion warp: two pieces
 constexpr int kBiasFloats = 128;                               // per promotion warp: of its columns
-constexpr int kPitch = 33;                                     // floats of a scratch row where rows of C start anywhere
 template <int BN>
 constexpr int kPairStage = kTileBytes + BN / 2 * kBlockK;      // this CTA's 128 rows of A and BN / 2 rows of B
 
@@ -152,26 +151,22 @@ __device__ __forceinline__ void store_rows(const Args& g, const CUtensorMap* map
     }
     return;
   }
-  // Rows that start anywhere: 16 rows of 32 columns at a time through shared memory, a row per instruction.
-  T* c = static_cast<T*>(g.c);
-  float* rows = reinterpret_cast<float*>(scratch);
+  // Rows that start anywhere: 32 rows of 32 columns at a time through shared memory (column j of row r at j ^ r: no bank conflicts either way), a row
+  // per instruction.
+  T* c = static_cast<T*>(g.c) + static_cast<size_t>(row_base) * g.ldc;
+  float* square = reinterpret_cast<float*>(scratch);
+  const int rows = min(32, g.M - row_base);
 #pragma unroll
   for (int p = 0; p < NC / 32; ++p) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if ((lane >> 4) == half) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) rows[(lane & 15) * kPitch + j] = acc[p * 32 + j];
-      }
-      __syncwarp();
-      const int n = col + p * 32 + lane;
-#pragma unroll 4
-      for (int r = 0; r < 16; ++r) {
-        const int m = row_base + half * 16 + r;
-        if (m < g.M && n < g.N) c[static_cast<size_t>(m) * g.ldc + n] = round_to<T>(rows[r * kPitch + lane]);
-      }
-      __syncwarp();
+    for (int j = 0; j < 32; ++j) square[lane * 32 + (j ^ lane)] = acc[p * 32 + j];
+    __syncwarp();
+    const int n = col + p * 32 + lane;
+    if (n < g.N) {
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r) c[static_cast<size_t>(r) * g.ldc + n] = round_to<T>(square[r * 32 + (lane ^ r)]);
     }
+    __syncwarp();
   }
 }
 
@@ -437,7 +432,7 @@ cudaError_t fire(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap
   auto kernel = gemm_fp8_pair_kernel<BN, B_ROWS>;
   constexpr int smem_bytes = kStages * kPairStage<BN> + 1024 /*alignment slack*/ + static_cast<int>(sizeof(PairCtl)) + 2 * kSlot<BN, B_ROWS> * 4 +
                              kPromoters * (kScratchBytes + kBiasFloats * 4);
-  static_assert(kPairStage<BN> % 1024 == 0 && 16 * kPitch * 4 <= kScratchBytes, "layout of shared memory");
+  static_assert(kPairStage<BN> % 1024 == 0 && 32 * 32 * 4 <= kScratchBytes, "layout of shared memory");
   static_assert(smem_bytes <= 227 * 1024, "shared memory");
   static int most_dev[kMaxDevices] = {};   // pairs that the device holds at once, which a persistent kernel must not exceed
   int& most = most_dev[current_device_slot()];
@@ -489,8 +484,8 @@ bool make_tensor_map_out(CUtensorMap* map, const Args& g) {
 // The tile width with the least estimated time (ns): a wave of tiles takes about two microseconds and so much a block of K, more with a scale for
 // every row of B (measured, us without / with those: 256 x 4096 x 4096, one wave of 64, 13.5 / 14.4, and of 128, 15.4 / 18.0; 1001 x 1288 x 5000,
 // one of 128, 18.3 / 21.5; 1001 x 5000 x 1288, two of 192, 17.6 / 21.0; 4096 x 4096 x 4096, four of 256, 67 / 101; 8192 x 4096 x 1024, seven of 256,
-// 41).  Rows of C that the TMA unit cannot write cost a wave of 128 columns three more (777 x 1003 x 1544 with 128: 13.1, 777 x 1000 x 1544 10.1; with 64:
-// 10.3 and 8.4).  A narrower tile pays where it saves a wave or leaves fewer SMs idle; 64 columns on all SMs read 10 TB/s from the L2.
+// 41).  Rows of C that the TMA unit cannot write cost a wave of 128 columns one more (8192 x 4095 x 1024: 56).  A narrower tile pays where it saves
+// a wave or leaves fewer SMs idle; 64 columns on all SMs read 10 TB/s from the L2.
 int pick_width(int M, int N, int K, bool b_rows, bool mapped, int pairs, long* ns) {
   struct Width {
     int bn;
@@ -502,7 +497,7 @@ int pick_width(int M, int N, int K, bool b_rows, bool mapped, int pairs, long* n
   *ns = -1;
   for (const Width& w : kWidths) {
     const long tiles = static_cast<long>((M + 255) / 256) * ((N + w.bn - 1) / w.bn), waves = (tiles + pairs - 1) / pairs;
-    const long t = 3100 + waves * (2000 + (mapped ? 0 : 3000 * w.bn / 128) + num_kb * (b_rows ? w.per_block_rows : w.per_block));
+    const long t = 3100 + waves * (2000 + (mapped ? 0 : 1000 * w.bn / 128) + num_kb * (b_rows ? w.per_block_rows : w.per_block));
     if (*ns < 0 || t < *ns) {
       *ns = t;
       best = w.bn;

@@ -337,7 +337,7 @@ int per_slice(int num_kb, int slices, int tn) {
 //   1 x 4096 x 4096      16 / 4: 7.5 us, 16 / 8: 8.6, 16 / 2: 9.6          64 x 14336 x 4096   64 / 1: 20.2 us, 32 / 1: 23.1, pairs: 21.2
 //   16 x 4096 x 14336    16 / 8: 14.7 us, 16 / 4: 15.3, 16 / 2: 19.5       64 x 4096 x 4096    64 / 4: 11.9 us, 32 / 4: 13.1, pairs: 13.0
 //   256 x 1024 x 1024    16 / 1: 6.9 us, 64 / 4: 7.7                       128 x 4096 x 4096   64 / 2: 15.1 us, 32 / 1: 16.8, pairs: 13.0
-//   512 x 1024 x 1024    16 / 1: 8.6 us, pairs: 6.4                        777 x 1003 x 1544   64 / 1: 12.2 us, pairs: 10.3
+//   512 x 1024 x 1024    16 / 1: 8.6 us, pairs: 6.4                        777 x 1003 x 1544   64 / 1: 12.2 us, pairs: 8.9
 // So a tile takes a fixed time and one per block of K that grows with its width; two narrow tiles on an SM overlap by a third, two wide
 // ones hardly; and nothing is faster than the operands come from memory.  Tiles of 128 rows of A never won (128 x 4096 x 4096: 16.4 us).  A
 // tile that has its K and its SM to itself takes all of the shared memory as its ring (16 x 14336 x 4096: 16.9 -> 15.5 us);
