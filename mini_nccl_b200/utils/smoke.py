@@ -78,6 +78,23 @@ def run() -> None:
     torch.cuda.synchronize()
     for got, name in ((out, "GEMM->reduce-scatter"), (c2, "all-gather->GEMM")):
         assert (got.float() - ref).abs().max().item() <= 2e-2 * ref.abs().max().item(), name + " mismatch"
-    assert gemm_status() == 0
     solo.destroy()
-    print(f"smoke ok: loss={loss.item():.4f} buckets={len(ddp.buckets)} kernels=local,ll,oneshot,twoshot,gemm,gemm_pair,gemm_small")
+    # A student in 8 bits, distilled from the decoder above, and the three kernels of the 8-bit product on whole numbers, where they are exact.
+    from dataclasses import replace
+
+    from mini_nccl_b200.ops import gemm_fp8
+
+    student = GPT2Model(replace(cfg, linear="fp8")).cuda().to(torch.bfloat16)
+    with torch.no_grad():
+        top, top_ids = model(ids).float().topk(8)
+    gap = student(ids, teacher=(top_ids, top, 2.0))
+    gap.backward()
+    assert torch.isfinite(gap).item() and all(p.grad is not None and torch.isfinite(p.grad).all() for p in student.parameters())
+    for m in (1, 32, 512):
+        x, w = (torch.randint(-4, 5, (rows, 1024), device="cuda").float() for rows in (m, 1024))
+        ones = torch.ones(8, 8, device="cuda")
+        got = gemm_fp8(x.to(torch.float8_e4m3fn), torch.ones(m, 8, device="cuda"), w.to(torch.float8_e4m3fn), ones, out_dtype=torch.float32)
+        assert torch.equal(got.double(), x.double() @ w.double().t()), f"8-bit product of {m} rows"
+    assert gemm_status() == 0
+    print(f"smoke ok: loss={loss.item():.4f} distillation={gap.item():.4f} buckets={len(ddp.buckets)} "
+          "kernels=local,ll,oneshot,twoshot,gemm,gemm_pair,gemm_small,quantize_fp8,gemm_fp8,distill")
