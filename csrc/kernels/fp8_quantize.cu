@@ -19,6 +19,8 @@
 #include <cstring>
 #include <type_traits>
 
+#include "kernels/dependent_launch.cuh"
+
 namespace {
 
 constexpr int kBlock = 128;
@@ -45,11 +47,11 @@ struct Eight {
   uint32_t w[kWords];
 
   // Elements [c, c + 8) of a row of K, zeros beyond its end.
-  __device__ __forceinline__ void load(const T* __restrict__ row, int c, int K, bool vec) {
+  __device__ __forceinline__ void load(const T* row, int c, int K, bool vec) {
     if (vec && c + 8 <= K) {
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+        const uint4 v = mnccl::load_vector(reinterpret_cast<const uint4*>(row + c) + i);
         w[4 * i] = v.x;
         w[4 * i + 1] = v.y;
         w[4 * i + 2] = v.z;
@@ -135,7 +137,10 @@ __device__ __forceinline__ uint2 quantise8(const Eight<T>& v, float inverse) {
 // looked at, and a block's scales of 16 rows are 64 contiguous bytes: scales are stored [K blocks][M].
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)
-quantise_rows_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t* __restrict__ q, size_t ldq, float* __restrict__ scale, bool vec) {
+quantise_rows_kernel(const T* x, size_t ldx, int M, int K, uint8_t* __restrict__ q, size_t ldq, float* __restrict__ scale, bool vec) {
+  mnccl::wait_for_previous();
+  mnccl::let_next_start();
+  x = mnccl::since_wait(x);
   const int m = static_cast<int>(blockIdx.x) * 16 + static_cast<int>(threadIdx.x >> 4);
   const int first = static_cast<int>(blockIdx.y) * N, c = first * kBlock + static_cast<int>(threadIdx.x & 15) * 8;
   if (m >= M) return;   // all 16 lanes of a block
@@ -164,7 +169,7 @@ quantise_rows_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t*
 
 template <typename T, bool SQUARE>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
-quantise_tile_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t* __restrict__ q, size_t ldq, float* __restrict__ scale,
+quantise_tile_kernel(const T* x, size_t ldx, int M, int K, uint8_t* __restrict__ q, size_t ldq, float* __restrict__ scale,
                      uint8_t* __restrict__ qt, size_t ldt, float* __restrict__ scale_t, float* __restrict__ sums, bool vec) {
   __shared__ __align__(16) uint32_t tile[kBlock * 32];
   __shared__ uint32_t part[8][kBlock];   // a warp's largest magnitude of each column, then its sum
@@ -172,6 +177,9 @@ quantise_tile_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t*
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m0 = static_cast<int>(blockIdx.x) * kBlock, k0 = static_cast<int>(blockIdx.y) * kBlock;
   const int r0 = warp * 16 + (lane >> 3) * 4, c0 = (lane & 7) * 8;   // columns c0 .. and c0 + 64 ..
+  mnccl::wait_for_previous();
+  mnccl::let_next_start();
+  x = mnccl::since_wait(x);
   Eight<T> v[4][2];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -292,10 +300,12 @@ quantise_tile_kernel(const T* __restrict__ x, size_t ldx, int M, int K, uint8_t*
 
 // out[k] = the sum over the tiles' sums [tiles][K], in their order.  32 columns a block, eight threads a column.
 template <typename T>
-__global__ void __launch_bounds__(256) sum_tiles_kernel(const float* __restrict__ sums, int tiles, int K, T* __restrict__ out) {
+__global__ void __launch_bounds__(256) sum_tiles_kernel(const float* sums, int tiles, int K, T* __restrict__ out) {
   __shared__ float part[8][32];
   const int k = static_cast<int>(blockIdx.x) * 32 + static_cast<int>(threadIdx.x & 31), y = threadIdx.x >> 5;
   const int per = (tiles + 7) / 8;
+  mnccl::wait_for_previous();
+  mnccl::let_next_start();
   float s = 0.0f;
   if (k < K)
     for (int t = y * per; t < min(tiles, (y + 1) * per); ++t) s += sums[static_cast<size_t>(t) * K + k];
@@ -309,8 +319,7 @@ __global__ void __launch_bounds__(256) sum_tiles_kernel(const float* __restrict_
   else out[k] = __float2bfloat16_rn(s);
 }
 
-int status() {
-  const cudaError_t e = cudaGetLastError();
+int status(cudaError_t e) {
   return e == cudaSuccess ? 0 : static_cast<int>(e) + 1000;
 }
 
@@ -320,17 +329,14 @@ int quantise(const T* x, int64_t ldx, int M, int K, int block_rows, uint8_t* q, 
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (ldx * static_cast<int64_t>(sizeof(T))) % 16 == 0;
   const int blocks_k = (K + kBlock - 1) / kBlock, rows16 = (M + 15) / 16;
   const dim3 grid((M + kBlock - 1) / kBlock, blocks_k);
-  if (block_rows == 128) {
-    quantise_tile_kernel<T, true><<<grid, kThreads, 0, stream>>>(x, ldx, M, K, q, ldq, scale, qt, ldt, scale_t, nullptr, vec);
-  } else if (qt != nullptr) {
-    quantise_tile_kernel<T, false><<<grid, kThreads, 0, stream>>>(x, ldx, M, K, q, ldq, scale, qt, ldt, scale_t, sums, vec);
-  } else if (static_cast<int64_t>(rows16) * blocks_k >= 4 * 2048) {
-    // Enough for every SM several times over: four blocks a thread in flight (8192 x 4096 bf16: 24.7 us with one).
-    quantise_rows_kernel<T, 4><<<dim3(rows16, (blocks_k + 3) / 4), kThreads, 0, stream>>>(x, ldx, M, K, q, ldq, scale, vec);
-  } else {
-    quantise_rows_kernel<T, 1><<<dim3(rows16, blocks_k), kThreads, 0, stream>>>(x, ldx, M, K, q, ldq, scale, vec);
-  }
-  return status();
+  if (block_rows == 128)
+    return status(mnccl::launch_early(quantise_tile_kernel<T, true>, grid, dim3(kThreads), stream, x, ldx, M, K, q, ldq, scale, qt, ldt, scale_t, nullptr, vec));
+  if (qt != nullptr)
+    return status(mnccl::launch_early(quantise_tile_kernel<T, false>, grid, dim3(kThreads), stream, x, ldx, M, K, q, ldq, scale, qt, ldt, scale_t, sums, vec));
+  // Enough for every SM several times over: four blocks a thread in flight (8192 x 4096 bf16: 24.7 us with one).
+  if (static_cast<int64_t>(rows16) * blocks_k >= 4 * 2048)
+    return status(mnccl::launch_early(quantise_rows_kernel<T, 4>, dim3(rows16, (blocks_k + 3) / 4), dim3(kThreads), stream, x, ldx, M, K, q, ldq, scale, vec));
+  return status(mnccl::launch_early(quantise_rows_kernel<T, 1>, dim3(rows16, blocks_k), dim3(kThreads), stream, x, ldx, M, K, q, ldq, scale, vec));
 }
 
 constexpr int kMaxK = 65535 * kBlock;   // gridDim.y
@@ -367,14 +373,13 @@ MNCCL_EXPORT int mncclQuantizeFp8(const void* x, int type, int64_t ldx, int M, i
 // out[K] (type as above) = the columns' sums of mncclQuantizeFp8 over all `blocks` blocks of rows.  Returns as that.
 MNCCL_EXPORT int mncclSumBlocks(const float* sums, int blocks, int K, void* out, int type, cudaStream_t stream) {
   if (!sums || !out || blocks <= 0 || K <= 0) return -1;
-  const unsigned grid = static_cast<unsigned>((K + 31) / 32);
+  const dim3 grid(static_cast<unsigned>((K + 31) / 32));
   switch (type) {
-    case 6: sum_tiles_kernel<<<grid, 256, 0, stream>>>(sums, blocks, K, static_cast<__half*>(out)); break;
-    case 7: sum_tiles_kernel<<<grid, 256, 0, stream>>>(sums, blocks, K, static_cast<float*>(out)); break;
-    case 9: sum_tiles_kernel<<<grid, 256, 0, stream>>>(sums, blocks, K, static_cast<__nv_bfloat16*>(out)); break;
-    default: return -2;
+    case 6: return status(mnccl::launch_early(sum_tiles_kernel<__half>, grid, dim3(256), stream, sums, blocks, K, out));
+    case 7: return status(mnccl::launch_early(sum_tiles_kernel<float>, grid, dim3(256), stream, sums, blocks, K, out));
+    case 9: return status(mnccl::launch_early(sum_tiles_kernel<__nv_bfloat16>, grid, dim3(256), stream, sums, blocks, K, out));
   }
-  return status();
+  return -2;
 }
 
 }  // extern "C"

@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <cstdio>
 
+#include "kernels/dependent_launch.cuh"
 #include "kernels/gemm_fp8.cuh"
 #include "mem/cuda_driver.h"
 
@@ -105,7 +106,7 @@ __device__ __forceinline__ void load_bias(const Args& g, int col, float* bias, i
   const T* b = static_cast<const T*>(g.bias);
   __syncwarp();   // the tile before has been stored
 #pragma unroll
-  for (int j = 0; j < NC / 32; ++j) bias[j * 32 + lane] = to_float(__ldg(b + min(col + j * 32 + lane, g.N - 1)));
+  for (int j = 0; j < NC / 32; ++j) bias[j * 32 + lane] = to_float(b[min(col + j * 32 + lane, g.N - 1)]);
   __syncwarp();
 }
 
@@ -224,6 +225,8 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
   cluster_sync_all();   // the partner's barriers exist before anything arrives on them
   tc_fence_after_sync();
   const uint32_t tmem_base = ctl->tmem_base;
+  wait_for_previous();
+  let_next_start();
   const uint64_t budget = g.wait_budget_ns;
   const bool leader = elect_one();   // the lane that issues for its warp
 
@@ -441,13 +444,13 @@ cudaError_t fire(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap
   cfg.blockDim = dim3(kPairThreads);
   cfg.dynamicSmemBytes = smem_bytes;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2] = {{}, early_start()};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 1;   // the question below is about clusters alone
   if (most == 0) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
     if (e != cudaSuccess) return e;
@@ -459,6 +462,7 @@ cudaError_t fire(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap
     }
     most = n;
   }
+  cfg.numAttrs = 2;
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min(tiles, most)));
   return cudaLaunchKernelEx(&cfg, kernel, ta, tb, tc, g, mapped);
 }

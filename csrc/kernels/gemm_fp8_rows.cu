@@ -6,16 +6,19 @@
 // Eight lanes hold a block of 128: their sums are reduced and dealt out over them together, seven shuffles for the eight rows, so
 // that each lane ends with one whole block's sum, which it scales.  The warps meet in shared memory and are added in order.
 //
-// The tensor-core kernel for few rows spends three microseconds on descriptors, barriers, tensor memory and the meeting of its slices, which this one
-// saves; then this one runs at 4.8 TB/s for one token, bound by its instructions (two for three bytes), at 4 for two and at 2.3 for four, and that one at up to 5.5.
-// Measured (this kernel / that one, us): 1 x 1024 x 1024 2.6 / 4.5, 1 x 4096 x 1024 3.4 / 5.2, 1 x 4096 x 4096 5.8 / 7.5, 1 x 14336 x 4096
-// 14.7 / 13.4; 2 x 4096 x 4096 6.8 / 7.8; 4 x 1024 x 1024 3.2 / 5.1, 4 x 4096 x 4096 10.7 / 8.5.  64 registers and 1024 threads an SM matter:
-// with 80, 1 x 4096 x 4096 took 7.1 us.  (Widening to fp32 took 7.8, mma.sync m16n8k32 of the same bytes 7.5 for 8 tokens and 20.1 at 14336.)
+// The tensor-core kernel for few rows spends three microseconds on descriptors, barriers, tensor memory and the meeting of its slices, which this
+// one saves; then this one runs at 4.8 TB/s for one token, bound by its instructions (two for three bytes), at 4 for two and at 2.3 for
+// four, and that one at up to 5.5.  Measured alone (this kernel / that one, us): 1 x 1024 x 1024 2.6 / 4.5, 1 x 4096 x 1024 3.4 / 5.2, 1 x 4096
+// x 4096 5.8 / 7.5, 1 x 14336 x 4096 14.7 / 13.4; 2 x 4096 x 4096 6.8 / 7.8; 4 x 1024 x 1024 3.2 / 5.1, 4 x 4096 x 4096 10.7 / 8.5.  Calls that
+// follow one another overlap at their ends (dependent_launch.cuh): 1 x 1024 x 1024 2.2, 1 x 4096 x 4096 5.5.  64 registers and 1024 threads
+// an SM matter: with 80, 1 x 4096 x 4096 took 7.1 us.  (Widening to fp32 took 7.8, mma.sync m16n8k32 of the same bytes 7.5 for 8 tokens and
+// 20.1 at 14336.)
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include <algorithm>
 
+#include "kernels/dependent_launch.cuh"
 #include "kernels/gemm_fp8.cuh"
 
 namespace mnccl {
@@ -30,7 +33,7 @@ constexpr int kRows = 8, kSpan = 512, kMostWarps = 8;   // rows of B a CTA, byte
 __device__ __forceinline__ uint4 load16(const uint8_t* row, int64_t k, int K) {
   uint4 v = make_uint4(0, 0, 0, 0);
   if (k + 16 <= K) {
-    v = __ldg(reinterpret_cast<const uint4*>(row + k));
+    v = load_vector(row + k);
   } else if (k < K) {
     uint32_t w[4] = {};
     for (int i = 0; k + i < K; ++i) w[i >> 2] |= static_cast<uint32_t>(row[k + i]) << (i & 3) * 8;
@@ -49,12 +52,16 @@ __device__ __forceinline__ void fma_f16(float& d, unsigned short x, unsigned sho
 
 template <int TM>
 __global__ void __launch_bounds__(32 * kMostWarps, TM <= 2 ? 4 : 2)
-    gemm_fp8_rows_kernel(const uint8_t* __restrict__ a, int64_t lda, const uint8_t* __restrict__ b, int64_t ldb, const __grid_constant__ Args g) {
+    gemm_fp8_rows_kernel(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb, const __grid_constant__ Args g) {
   __shared__ float part[kMostWarps][kRows][TM];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int n0 = blockIdx.x * kRows, num_kb = (g.K + kBlockK - 1) / kBlockK;
   const int own = n0 + (lane & 7) * kRows / 8;   // the row of B whose blocks this lane scales
   float acc[TM] = {};
+  wait_for_previous();
+  let_next_start();
+  a = since_wait(a);
+  b = since_wait(b);
   for (int64_t k0 = static_cast<int64_t>(warp) * kSpan; k0 < g.K; k0 += static_cast<int64_t>(warps) * kSpan) {
     uint4 w[kRows], x[TM];
 #pragma unroll
@@ -64,9 +71,9 @@ __global__ void __launch_bounds__(32 * kMostWarps, TM <= 2 ? 4 : 2)
     const int64_t kb = k0 / kBlockK + (lane >> 3);
     float sb = 0.0f, sa[TM] = {};
     if (kb < num_kb) {
-      sb = __ldg(g.b.at(min(own, g.N - 1)) + kb * g.b.blk);
+      sb = g.b.at(min(own, g.N - 1))[kb * g.b.blk];
 #pragma unroll
-      for (int m = 0; m < TM; ++m) sa[m] = __ldg(g.a.at(min(m, g.M - 1)) + kb * g.a.blk);
+      for (int m = 0; m < TM; ++m) sa[m] = g.a.at(min(m, g.M - 1))[kb * g.a.blk];
     }
     float s[TM][kRows];   // sums of 16 products
     __half2_raw xh[TM][8];
@@ -136,14 +143,9 @@ cudaError_t launch_rows(const void* a, int64_t lda, const void* b, int64_t ldb, 
   const dim3 grid((g.N + kRows - 1) / kRows), block(32 * std::min(spans, kMostWarps));
   const auto* pa = static_cast<const uint8_t*>(a);
   const auto* pb = static_cast<const uint8_t*>(b);
-  if (g.M == 1) {
-    gemm_fp8_rows_kernel<1><<<grid, block, 0, stream>>>(pa, lda, pb, ldb, g);
-  } else if (g.M == 2) {
-    gemm_fp8_rows_kernel<2><<<grid, block, 0, stream>>>(pa, lda, pb, ldb, g);
-  } else {
-    gemm_fp8_rows_kernel<4><<<grid, block, 0, stream>>>(pa, lda, pb, ldb, g);
-  }
-  return cudaGetLastError();
+  if (g.M == 1) return launch_early(gemm_fp8_rows_kernel<1>, grid, block, stream, pa, lda, pb, ldb, g);
+  if (g.M == 2) return launch_early(gemm_fp8_rows_kernel<2>, grid, block, stream, pa, lda, pb, ldb, g);
+  return launch_early(gemm_fp8_rows_kernel<4>, grid, block, stream, pa, lda, pb, ldb, g);
 }
 
 }  // namespace fp8

@@ -9,6 +9,7 @@
 // ring stages hold two blocks where tiles are narrow.
 #include <algorithm>
 
+#include "kernels/dependent_launch.cuh"
 #include "kernels/gemm_fp8.cuh"
 
 namespace mnccl {
@@ -115,6 +116,7 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
       fence_proxy_async();
     }
     __syncwarp();
+    wait_for_previous();
     for (int i = 0; i < NS && i < stages; ++i)
       if (leader) load(i, i);
   }
@@ -127,6 +129,8 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = ctl->tmem_base;
+  wait_for_previous();
+  let_next_start();
 
   // promotion warps: warp's quarter of the lanes, its columns of the tile, this lane's row of B
   const int q = warp & 3, first_col = ((warp - 2) >> 2) * NC;
@@ -315,13 +319,13 @@ cudaError_t fire(const CUtensorMap& tw, const CUtensorMap& tx, const SmallArgs& 
   cfg.blockDim = dim3(kThreads<TN>);
   cfg.dynamicSmemBytes = smem_bytes;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2] = {{}, early_start()};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(p.slices);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, tw, tx, a);
 }
 

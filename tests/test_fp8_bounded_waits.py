@@ -42,3 +42,20 @@ def test_a_loop_of_a_role_ends_with_its_first_wait_that_ran_out():
             assert wait[1].startswith("if (!ok) break;"), wait[0]
     for loop in re.findall(r"for \(int t = pair; [^)]*\)", _source("gemm_fp8.cu")):
         assert "&& ok" in loop
+
+
+@pytest.mark.parametrize("name,kernels", [("gemm_fp8.cu", 1), ("gemm_fp8_small.cu", 1), ("gemm_fp8_rows.cu", 1), ("fp8_quantize.cu", 3)])
+def test_a_kernel_that_starts_early_waits_before_it_reads(name, kernels):
+    """Every kernel launched before the one ahead has ended waits for it, in all threads, before it lets the next one start, and reads nothing
+    through pointers that promise that nobody writes there."""
+    text = _source(name)
+    bodies = re.split(r"__global__ ", text)[1:]
+    assert len(bodies) == kernels
+    for body in bodies:
+        wait, start = body.index("wait_for_previous();\n"), body.index("let_next_start();")
+        assert wait < start and body.count("let_next_start();") == 1
+        assert not re.search(r"\breturn;", body[:wait])
+    assert "__ldg" not in text and not re.search(r"const \w+\*\s*__restrict__", text)
+    assert "early_start()" in text or "launch_early(" in text
+    if "tmem_alloc" in text:
+        assert text.index("tmem_alloc") < text.index("let_next_start();")

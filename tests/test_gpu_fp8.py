@@ -278,6 +278,35 @@ def test_offsets_behind_32_bits(M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 1024, 1024), (4, 2048, 2048), (16, 4096, 4096), (64, 4096, 4096), (300, 2000, 3000), (777, 1003, 1544), (2000, 3000, 1000)])
+def test_calls_that_follow_one_another_see_what_the_others_wrote(m, n, k):
+    """Kernels start before the one ahead of them has ended: chains of calls, whose memory is used again at once, against the same with a
+    synchronisation after every call."""
+    torch.manual_seed(m)
+    weights = [torch.randn(n, k, device="cuda", dtype=torch.bfloat16) * 0.05 for _ in range(2)]
+
+    def chain(x, then):
+        seen = []
+        for w in weights:
+            q = quantize_fp8(x)
+            then()
+            y = gemm_fp8(*q, *quantize_fp8(w, block_rows=128))
+            then()
+            q = quantize_fp8(y, transposed=True)[:2]
+            then()
+            x = gemm_fp8(*q, *quantize_fp8(w, block_rows=128, transposed=True)[2:])
+            then()
+            seen += [y, x]
+        return seen
+
+    for _ in range(10):
+        x = torch.randn(m, k, device="cuda", dtype=torch.bfloat16)
+        got = chain(x, lambda: None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, chain(x, torch.cuda.synchronize)))
+
+
+@pytest.mark.gpu
 def test_first_product_of_a_process_may_be_captured():
     """What a product needs once for each process (the word for waits that ran out) is made without breaking a capture that is under way."""
     code = """
