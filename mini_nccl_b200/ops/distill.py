@@ -115,20 +115,35 @@ def _native(logits, ids, top):
 
 def _arguments(shape, device, ids, top, temperature, reduction="mean"):
     """The teacher's entries as the kernels read them, and the temperature."""
+    lead = tuple(shape[:-1])
     for t, name in ((ids, "top_ids"), (top, "top_logits")):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch tensor")
-        if t.dim() != len(shape) or tuple(t.shape[:-1]) != tuple(shape[:-1]) or t.shape[-1] == 0 or t.device != device:
-            raise ValueError(f"{name} must be {[*shape[:-1], 'K']} on {device}")
+        if t.dim() != len(lead) + 1 or t.shape[:-1] != lead or t.shape[-1] == 0 or t.device != device:
+            raise ValueError(f"{name} must be {[*lead, 'K']} on {device}")
     if ids.shape != top.shape:
         raise ValueError("top_ids and top_logits must have one shape")
-    if ids.dtype not in (torch.int64, torch.int32) or not top.dtype.is_floating_point:
-        raise TypeError("top_ids must be int64 or int32, top_logits floating point")
-    if not 1e-3 <= float(temperature) <= 1e3:
+    if ids.dtype is not torch.int64:
+        if ids.dtype is not torch.int32:
+            raise TypeError("top_ids must be int64 or int32")
+        ids = ids.long()
+    if not top.dtype.is_floating_point:
+        raise TypeError("top_logits must be floating point")
+    temperature = float(temperature)
+    if not 1e-3 <= temperature <= 1e3:
         raise ValueError("the temperature must be between 1e-3 and 1e3")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}")
-    return ids.long(), top.detach() if top.requires_grad else top, float(temperature)
+    return ids, top.detach() if top.requires_grad else top, temperature
+
+
+def _rows_of_entries(t, dtype):
+    """[T, K], dense."""
+    if t.dtype is not dtype:
+        t = t.to(dtype)
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def distillation_loss(logits, top_ids, top_logits, temperature=1.0, reduction="mean"):
@@ -147,9 +162,8 @@ def distillation_loss(logits, top_ids, top_logits, temperature=1.0, reduction="m
     ids, top, tau = _arguments(logits.shape, logits.device, top_ids, top_logits, temperature, reduction)
     if not _native(logits, ids, top):
         return _reference(logits, ids, top, tau, reduction)
-    K = ids.shape[-1]
     return _call("distillation", "mncclDistillForward", "csrc/kernels/distill.cu")(
-        logits, ids.reshape(-1, K).contiguous(), top.float().reshape(-1, K).contiguous(), tau, _REDUCTIONS.index(reduction), _gradient_again)
+        logits, _rows_of_entries(ids, torch.int64), _rows_of_entries(top, torch.float32), tau, _REDUCTIONS.index(reduction), _gradient_again)
 
 
 def lm_head_distillation(x, weight, top_ids, top_logits, temperature=1.0):
@@ -166,5 +180,4 @@ def lm_head_distillation(x, weight, top_ids, top_logits, temperature=1.0):
               and no_tangent(weight))
     if not native or not _pays(T, V, d):
         return distillation_loss(F.linear(x, weight), ids, top, tau)
-    K = ids.shape[-1]
-    return _LmHeadDistillation.apply(x, weight, ids.reshape(-1, K).contiguous(), top.float().reshape(-1, K).contiguous(), tau)
+    return _LmHeadDistillation.apply(x, weight, _rows_of_entries(ids, torch.int64), _rows_of_entries(top, torch.float32), tau)
