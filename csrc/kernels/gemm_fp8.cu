@@ -113,9 +113,10 @@ __device__ __forceinline__ void load_bias(const Args& g, int col, float* bias, i
 // A lane's NC sums of row `row`, columns [col, col + NC): bias, one rounding, out.  With a tensor map of C a warp's 32 rows leave as pieces of 64
 // bytes a row that it lays out in shared memory (64-byte swizzle: no bank conflicts) and the TMA unit writes while the next tile is
 // begun.  (Each lane storing its own row, 32 bytes at a time, held the tensor cores up for a fifth of the time at K = 4096 and for two fifths
-// at K = 1024.)
+// at K = 1024.)  `pieces` counts them over all of the warp's tiles: the two places in shared memory alternate, so a place is free once all stores
+// but the latest have been read, and a tile may have an odd number of them (192 or 64 columns of a 16-bit type; a ragged right edge).
 template <typename T, int NC>
-__device__ __forceinline__ void store_rows(const Args& g, const CUtensorMap* map, bool mapped, int row, int col, float (&acc)[NC], uint8_t* scratch, const float* bias, int lane) {
+__device__ __forceinline__ void store_rows(const Args& g, const CUtensorMap* map, bool mapped, int row, int col, float (&acc)[NC], uint8_t* scratch, uint32_t& pieces, const float* bias, int lane) {
   const int row_base = row - lane;
   if (row_base >= g.M) return;   // the same for the whole warp
   if (g.bias != nullptr) {
@@ -133,7 +134,7 @@ __device__ __forceinline__ void store_rows(const Args& g, const CUtensorMap* map
 #pragma unroll
     for (int p = 0; p < NC / kPer; ++p) {
       if (col + p * kPer >= g.N) break;
-      uint8_t* piece = scratch + (p & 1) * kPieceBytes;
+      uint8_t* piece = scratch + (pieces++ & 1u) * kPieceBytes;
       if (lane == 0) bulk_wait_read<1>();   // the piece before the last has been read
       __syncwarp();
 #pragma unroll
@@ -338,6 +339,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
     const uint32_t acc_full = smem_u32(&ctl->acc_full[0][half]), acc_empty = map_to_cta(smem_u32(&ctl->acc_empty[0][half]), 0);
     uint32_t group = 0;
     uint32_t it = 0;
+    uint32_t pieces = 0;   // of results that have been sent out
     bool ok = true, ready = false;
     for (int t = pair; t < num_tiles && ok; t += n_pairs) {
       int tm, tn;
@@ -411,9 +413,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
       if (!ok) break;
       if (col < g.N) {
         switch (g.type) {
-          case 6: store_rows<__half>(g, &tma_c, mapped, row, col, acc, scratch, bias, lane); break;
-          case 7: store_rows<float>(g, &tma_c, mapped, row, col, acc, scratch, bias, lane); break;
-          default: store_rows<__nv_bfloat16>(g, &tma_c, mapped, row, col, acc, scratch, bias, lane);
+          case 6: store_rows<__half>(g, &tma_c, mapped, row, col, acc, scratch, pieces, bias, lane); break;
+          case 7: store_rows<float>(g, &tma_c, mapped, row, col, acc, scratch, pieces, bias, lane); break;
+          default: store_rows<__nv_bfloat16>(g, &tma_c, mapped, row, col, acc, scratch, pieces, bias, lane);
         }
       }
     }
