@@ -13,6 +13,8 @@ from .._lib import ext, lib
 BLOCK = 128
 _MOST_ROWS, _MOST_COLUMNS = 2**31 - 1 - 2**16, 65535 * BLOCK   # mncclQuantizeFp8
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_RECORDING = tuple(getattr(torch._C._TorchDispatchModeKey, name) for name in ("FAKE", "PROXY", "FUNCTIONAL"))
 _calls = {}   # the extension's entry points, looked up on the first call
 
 
@@ -23,6 +25,18 @@ def _call(name, symbol, source):
             raise RuntimeError(f"libmini_nccl.so was built without {source}")
         call = _calls[name] = getattr(ext(), name)
     return call
+
+
+def _plain_calls_only(name, *tensors):
+    """What is active may record or replace the single operators: a tracer would keep the allocation of a result and not the kernel that fills it, so
+    that what it recorded returns memory as it was found.  Modes that only look on (FLOP counters, selective checkpointing) do no harm."""
+    if torch.jit.is_tracing() or torch._C._are_functorch_transforms_active() or (
+            torch._C._len_torch_dispatch_stack() and any(torch._C._get_dispatch_mode(mode) is not None for mode in _RECORDING)):
+        raise RuntimeError(f"{name} has no rule for tracing, functional transforms and fake tensors")
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and type(t) not in _PLAIN and (
+                type(t).__torch_function__ is not torch._C._disabled_torch_function_impl or torch._C._dispatch_keys(t).has(torch._C.DispatchKey.Python)):
+            raise TypeError(f"{name} has no rule for {type(t).__name__}, only for plain tensors")
 
 
 def quantize_fp8(x, block_rows=1, transposed=False, stream=None):
@@ -36,6 +50,7 @@ def quantize_fp8(x, block_rows=1, transposed=False, stream=None):
     ``transposed=True``: ``(q, scale, qt, scale_t)``, with the transpose ``qt [K, M]`` as well, from one reading of ``x``; with
     ``block_rows=1`` it is quantised anew, in blocks of 128 along M (``scale_t [K, ceil(M / 128)]``).  K is at most 65535 * 128.
     Not differentiable."""
+    _plain_calls_only("quantize_fp8", x)
     return _call("quantize_fp8", "mncclQuantizeFp8", "csrc/kernels/fp8_quantize.cu")(x, block_rows, transposed, stream)
 
 
@@ -45,6 +60,7 @@ def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=None, bias=None, stream
 
     A block's products are summed in fp32, scaled and added up in fp32; with the bias added, one rounding to ``out``'s type (bf16 by
     default, fp16 or fp32).  ``bias`` has that type.  Operands have rows that start on 16 bytes.  Not differentiable."""
+    _plain_calls_only("gemm_fp8", a, a_scale, b, b_scale, out, bias)
     return _call("gemm_fp8", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")(a, a_scale, b, b_scale, out, out_dtype, bias, stream)
 
 
@@ -59,7 +75,10 @@ def linear_fp8(x, weight, bias=None):
 
     Differentiable once, straight through the roundings: with ``Q`` for quantisation along the summed dimension, the gradients
     are ``dx = Q(dy) Q(weight)`` (the forward pass's 8-bit weight), ``dweight = Q(dy).T Q(x)`` with blocks along the tokens, and
-    ``dbias`` the fp32 sum of ``dy``.  What is kept for the backward pass is in 8 bits."""
+    ``dbias`` the fp32 sum of ``dy``.  What is kept for the backward pass is in 8 bits.
+
+    All three refuse to be traced or transformed, and tensor subclasses with rules of their own."""
+    _plain_calls_only("linear_fp8", x, weight, bias)
     if torch.is_autocast_enabled("cuda"):
         to = torch.get_autocast_dtype("cuda")
         x, weight, bias = x.to(to), weight.to(to), None if bias is None else bias.to(to)
@@ -76,6 +95,6 @@ def linear_fp8(x, weight, bias=None):
         raise ValueError("a layer without input features")
     if x.numel() // x.shape[-1] > _MOST_ROWS or max(weight.shape) > _MOST_COLUMNS:
         raise ValueError(f"at most {_MOST_ROWS} tokens and {_MOST_COLUMNS} features")
-    if torch._C._are_functorch_transforms_active() or not all(no_tangent(t) for t in (x, weight, bias) if t is not None):
-        raise RuntimeError("linear_fp8 has no rule for functional transforms and forward-mode differentiation")
+    if not all(no_tangent(t) for t in (x, weight, bias) if t is not None):
+        raise RuntimeError("linear_fp8 has no rule for forward-mode differentiation")
     return _call("linear_fp8", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")(x, weight, bias)
