@@ -13,8 +13,8 @@
 //                           of its row and BN / 2 columns in registers, then adds the bias, rounds and stores them
 //
 // The tensor cores take 512 cycles for a block of 128 x 256 x 128 an SM; reading it (64 KB from tensor memory) and 256 fused multiply-adds
-// a scheduler overlap with the next block.  Where B has a scale for every row (the gradient of a weight) a column's scale is a second
-// factor, which comes from shared memory at a cycle a warp and column: 4096 x 4096 x 4096 takes 101 us against 67.
+// a scheduler overlap with the next block.  Where B has a scale for every row (the gradient of a weight) every column has a product of scales of
+// its own, which costs a read of shared memory and half an instruction a warp and column: 4096 x 4096 x 4096 takes 97 us against 67.
 //
 // What bounds it: the hand-over of accumulators at short clocks, and power in long runs.  4096 x 14336 x 4096 (481 GFLOP) takes 223 us alone, 2.2
 // PFLOP/s, and 275 repeated for seconds; 8192 x 4096 x 1024 41 us, where each tile's first block and its 128 KB of results count most.
@@ -366,7 +366,14 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
         const float* slot = slots + (group & 1u) * kSlot<BN, B_ROWS>;
         const float* cols = slot + kGroup * 128 + (B_ROWS ? i * BN + first_col : i * 4 + half * 2);
         const float r = slot[i * 128 + q * 32 + lane];
-        float x[2];   // the row's scale, or its products with B's
+        float x[2];   // its products with the scales of the two blocks of B's rows
+        // A narrow tile's scales of columns are on their way before the block is there, and multiplied one at a time (256 x 4096 x 4096: 13.6 us; fetched
+        // behind the block 14.2, two at a time 14.0).
+        float4 ahead[8];
+        if constexpr (B_ROWS && NC == 32) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ahead[j] = *reinterpret_cast<const float4*>(cols + 4 * j);
+        }
         if constexpr (!B_ROWS) {
           x[0] = r * cols[0];
           x[1] = r * cols[1];
@@ -383,11 +390,18 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
               if constexpr (B_ROWS) {
 #pragma unroll
                 for (int j = 0; j < kPiece; j += 4) {
-                  const float4 b = *reinterpret_cast<const float4*>(cols + c + j);
-                  acc[c + j] += __uint_as_float(v[j]) * r * b.x;
-                  acc[c + j + 1] += __uint_as_float(v[j + 1]) * r * b.y;
-                  acc[c + j + 2] += __uint_as_float(v[j + 2]) * r * b.z;
-                  acc[c + j + 3] += __uint_as_float(v[j + 3]) * r * b.w;
+                  float y[4];   // the products of the two scales
+                  if constexpr (NC == 32) {
+                    const float4& b = ahead[j / 4];
+                    y[0] = r * b.x;
+                    y[1] = r * b.y;
+                    y[2] = r * b.z;
+                    y[3] = r * b.w;
+                  } else {
+                    times_four(*reinterpret_cast<const float4*>(cols + c + j), r, y);
+                  }
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) acc[c + j + k] += __uint_as_float(v[j + k]) * y[k];
                 }
               } else {
 #pragma unroll

@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(32 * kMostWarps, TM <= 2 ? 4 : 2)
           s[m][0] += __shfl_xor_sync(0xffffffffu, s[m][0], d);
         }
       }
-      if (kb < num_kb) acc[m] += s[m][0] * sb * sa[m];
+      if (kb < num_kb) acc[m] += s[m][0] * (sa[m] * sb);
     }
   }
 #pragma unroll

@@ -247,11 +247,10 @@ gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_co
         }
 #pragma unroll
         for (int j = 0; j < NC; j += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(cols + j);
-          acc[j] += __uint_as_float(v[j]) * r * s.x;
-          acc[j + 1] += __uint_as_float(v[j + 1]) * r * s.y;
-          acc[j + 2] += __uint_as_float(v[j + 2]) * r * s.z;
-          acc[j + 3] += __uint_as_float(v[j + 3]) * r * s.w;
+          float x[4];
+          times_four(*reinterpret_cast<const float4*>(cols + j), r, x);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[j + k] += __uint_as_float(v[j + k]) * x[k];
         }
       }
       if ((i0 + U) % kGroup == 0 || i0 + U >= nkb) {   // this group's scales have been read

@@ -114,9 +114,9 @@ int mncclTransposeBf16(const void* src, int64_t lds, int rows, int cols, void* d
 int mncclQuantizeFp8(const void* x, int type, int64_t ldx, int M, int K, int block_rows, void* q, int64_t ldq, float* scale, void* qt,
                      int64_t ldt, float* scale_t, float* sums, cudaStream_t stream);
 int mncclSumBlocks(const float* sums, int blocks, int K, void* out, int type, cudaStream_t stream);
-/* C[M, N] = A[M, K] * B[N, K]^T (+ bias[N]) of e4m3 operands: the fp32 sum of each block of 128 along K times
- * sa[(m / sa_rows) * sa_row + block * sa_blk] and sb likewise (any fp32 scales), added in fp32 and rounded once.  C and
- * bias (null: none) are of `type`. */
+/* C[M, N] = A[M, K] * B[N, K]^T (+ bias[N]) of e4m3 operands: the fp32 sum of each block of 128 along K times the fp32 product of
+ * sa[(m / sa_rows) * sa_row + block * sa_blk] and sb likewise (any fp32 scales; beyond fp32's range their product is infinite or 0), added in fp32 and
+ * rounded once.  C and bias (null: none) are of `type`. */
 int mncclGemmFp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_blk, int sa_rows, const void* b, int64_t ldb,
                  const float* sb, int64_t sb_row, int64_t sb_blk, int sb_rows, void* c, int64_t ldc, int type, const void* bias, int M, int N,
                  int K, cudaStream_t stream);

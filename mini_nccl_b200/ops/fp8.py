@@ -58,7 +58,8 @@ def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=None, bias=None, stream
     """``out[M, N] = a[M, K] @ b[N, K].T (+ bias[N])`` of e4m3 operands with a scale for each block of 128 along K; a scale covers one
     row or 128 rows: ``a_scale [M or ceil(M / 128), ceil(K / 128)]``, ``b_scale`` likewise, any fp32 values and strides.
 
-    A block's products are summed in fp32, scaled and added up in fp32; with the bias added, one rounding to ``out``'s type (bf16 by
+    A block's products are summed in fp32, multiplied by the fp32 product of its two scales (which has to stay in fp32's range: beyond it the block
+    counts as infinite or NaN, below it as 0) and added up in fp32; with the bias added, one rounding to ``out``'s type (bf16 by
     default, fp16 or fp32).  ``bias`` has that type.  Operands have rows that start on 16 bytes.  Not differentiable."""
     _plain_calls_only("gemm_fp8", a, a_scale, b, b_scale, out, bias)
     return _call("gemm_fp8", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")(a, a_scale, b, b_scale, out, out_dtype, bias, stream)
