@@ -88,13 +88,8 @@ class _LmHeadDistillation(torch.autograd.Function):
         V = weight.shape[0]
         rows, logits = _dense_rows(x).view(-1, x.shape[-1]), _dense_rows(logits)
         d = _backward(logits[:, :V], ids, *kept, ctx.tau, "mean", grad)   # in padded rows, as the logits
-        dx = dw = None
-        if want_x and V % 8 == 0:
-            dx = gemm_bf16(d, _transposed(_dense_rows(weight), stream)).view(x.shape)
-        elif want_x:   # (why the library: ops/lm_loss.py)
-            dx = torch.mm(d.contiguous(), _dense_rows(weight)).view(x.shape)
-        if want_w:
-            dw = gemm_bf16(_transposed(d, stream), _transposed(rows, stream))
+        dx = gemm_bf16(d, _transposed(_dense_rows(weight), stream)).view(x.shape) if want_x else None
+        dw = gemm_bf16(_transposed(d, stream), _transposed(rows, stream)) if want_w else None
         return dx, dw, None, None, None
 
 
