@@ -378,6 +378,8 @@ bool matrix(const at::Tensor& t, const char* name, bool right_type, int64_t* ld)
     PyErr_Format(PyExc_ValueError, "%s must be a matrix of at most %lld rows and columns", name, static_cast<long long>(kMost));
   } else if (t.size(1) > 1 && t.stride(1) != 1) {
     PyErr_Format(PyExc_ValueError, "%s needs a unit inner stride", name);
+  } else if (t.is_neg()) {
+    PyErr_Format(PyExc_ValueError, "%s is a view of numbers with the other sign (resolve_neg() makes them its own)", name);
   } else {
     *ld = t.size(0) > 1 ? t.stride(0) : padded(t.size(1));
     if (*ld >= t.size(1)) return true;
@@ -469,6 +471,10 @@ bool scales(const at::Tensor& t, const char* name, int64_t rows, int64_t K, cons
     PyErr_Format(PyExc_TypeError, "%s must be an fp32 tensor on the operands' GPU", name);
     return false;
   }
+  if (t.is_neg()) {
+    PyErr_Format(PyExc_ValueError, "%s is a view of numbers with the other sign (resolve_neg() makes them its own)", name);
+    return false;
+  }
   if (t.dim() != 2 || t.size(1) != blocks(K) || (t.size(0) != rows && t.size(0) != blocks(rows))) {
     PyErr_Format(PyExc_ValueError, "%s must be [%lld or %lld, %lld]", name, static_cast<long long>(rows), static_cast<long long>(blocks(rows)),
                  static_cast<long long>(blocks(K)));
@@ -527,7 +533,7 @@ PyObject* gemm_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (args[6] != Py_None) {
     bias = tensor_arg(args[6], "bias");
     if (!bias) return nullptr;
-    if (bias->scalar_type() != out->scalar_type() || bias->device() != a->device() || bias->dim() != 1 || bias->size(0) != N || (N > 1 && bias->stride(0) != 1)) {
+    if (bias->scalar_type() != out->scalar_type() || bias->device() != a->device() || bias->dim() != 1 || bias->size(0) != N || (N > 1 && bias->stride(0) != 1) || bias->is_neg()) {
       PyErr_SetString(PyExc_ValueError, "bias must be [N], dense, of out's type and on its GPU");
       return nullptr;
     }
@@ -549,10 +555,11 @@ PyObject* gemm_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// `t [..., cols]` as a matrix that the kernels can read (a copy only where the strides need one), and its row stride.
+// `t [..., cols]` as a matrix that the kernels can read (a copy only where the strides need one, or where `t` is a view of numbers with the other sign, as
+// the imaginary part of a conjugate is), and its row stride.
 at::Tensor rows_of(const at::Tensor& t, int64_t cols, int64_t* ld) {
   c10::AutoGradMode no_grad(false);
-  at::Tensor r = t.dim() == 2 ? t : t.reshape({cols > 0 ? t.numel() / cols : 0, cols});
+  at::Tensor r = (t.dim() == 2 ? t : t.reshape({cols > 0 ? t.numel() / cols : 0, cols})).resolve_neg();
   if ((cols > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < cols)) r = r.contiguous();
   *ld = r.size(0) > 1 ? r.stride(0) : padded(cols);
   return r;
@@ -654,7 +661,7 @@ PyObject* linear_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
       c10::AutoGradMode no_grad(false);
       const int64_t N = weight->size(0), K = weight->size(1);
       int64_t ldx = 0, ldw = 0;
-      const at::Tensor rows = rows_of(*x, K, &ldx), w = rows_of(*weight, K, &ldw), dense = b.defined() ? b.contiguous() : b;
+      const at::Tensor rows = rows_of(*x, K, &ldx), w = rows_of(*weight, K, &ldw), dense = b.defined() ? b.resolve_neg().contiguous() : b;
       quantize(rows, ldx, true, want_w, false, o.raw, &qx);
       quantize(w, ldw, false, want_x, false, o.raw, &qw);
       auto shape = x->sizes().vec();
@@ -709,7 +716,7 @@ at::Tensor distill_gradient(const at::Tensor& logits, const at::Tensor& ids, con
                             const at::Tensor& tokens, double tau, const at::Tensor& of_loss, cudaStream_t stream) {
   const int64_t V = logits.size(-1);
   int64_t ld = 0;
-  const at::Tensor rows = rows_of(logits, V, &ld), grad = of_loss.contiguous();
+  const at::Tensor rows = rows_of(logits, V, &ld), grad = of_loss.resolve_neg().contiguous();
   // the gradient's rows lie to 16 bytes as the logits' do: padded where those are
   const int64_t T = rows.size(0), per = 16 / rows.element_size(), ldd = rows.stride(0) != V ? (V + per - 1) / per * per : V;
   at::Tensor d = at::empty({T, ldd}, rows.options().requires_grad(false));

@@ -174,6 +174,8 @@ def _matrix(t, name, dtypes):
     rows, cols = t.shape
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name} needs a unit inner stride")
+    if t.is_neg():
+        raise ValueError(f"{name} is a view of numbers with the other sign (resolve_neg() makes them its own)")
     ld = t.stride(0) if rows > 1 else _padded(cols)
     if ld < cols:
         raise ValueError(f"{name}'s rows overlap")
@@ -218,6 +220,8 @@ def _scales(t, name, rows, K, device):
     """(row stride, block stride, rows of a scale) of the scales of an operand [rows, K]."""
     if _tensor(t, name).dtype != torch.float32 or t.device != device:
         raise TypeError(f"{name} must be an fp32 tensor on the operands' GPU")
+    if t.is_neg():
+        raise ValueError(f"{name} is a view of numbers with the other sign (resolve_neg() makes them its own)")
     if t.dim() != 2 or t.shape[1] != _blocks(K) or t.shape[0] not in (rows, _blocks(rows)):
         raise ValueError(f"{name} must be [{rows} or {_blocks(rows)}, {_blocks(K)}]")
     return t.stride(0), t.stride(1), 1 if t.shape[0] == rows else _BLOCK
@@ -241,7 +245,7 @@ def gemm_fp8(lib, a, a_scale, b, b_scale, out, out_dtype, bias, stream):
             raise ValueError("out must be [M, N] on the operands' GPU")
         ldc = _matrix(out, "out", _FLOATS)[2]
         if bias is not None and (_tensor(bias, "bias").dtype != out.dtype or bias.device != a.device or tuple(bias.shape) != (N,)
-                                 or (N > 1 and bias.stride(0) != 1)):
+                                 or (N > 1 and bias.stride(0) != 1) or bias.is_neg()):
             raise ValueError("bias must be [N], dense, of out's type and on its GPU")
         if K == 0:
             with torch.no_grad():
@@ -253,8 +257,8 @@ def gemm_fp8(lib, a, a_scale, b, b_scale, out, out_dtype, bias, stream):
 
 
 def _rows(t, cols):
-    """``t [..., cols]`` as a matrix that the kernels can read (a copy only where the strides need one)."""
-    t = t.detach()
+    """``t [..., cols]`` as a matrix that the kernels can read (a copy only where the strides need one, or where ``t`` is a view of numbers with the other sign)."""
+    t = t.detach().resolve_neg()
     t = t if t.dim() == 2 else t.reshape(t.numel() // cols if cols else 0, cols)
     return t if (cols <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= cols) else t.contiguous()
 
@@ -266,7 +270,7 @@ def _linear_forward(lib, x, weight, bias, want_x, want_w):
     with _on(x.device, None) as s:
         q, scale, qt, scale_t, _ = _quantize(lib, rows, 1, want_w, False, s)
         wq, w_scale, wt, _, _ = _quantize(lib, w, _BLOCK, want_x, False, s)
-    y = gemm_fp8(lib, q[:, :K], scale.t(), wq[:, :K], w_scale, None, x.dtype, None if bias is None else bias.detach().contiguous(), None)
+    y = gemm_fp8(lib, q[:, :K], scale.t(), wq[:, :K], w_scale, None, x.dtype, None if bias is None else bias.detach().resolve_neg().contiguous(), None)
     return y.view(*x.shape[:-1], N), qt, scale_t, wt, w_scale if want_x else None
 
 
@@ -324,7 +328,7 @@ def distill_forward(lib, logits, ids, top, tau, reduction):
 
 
 def distill_backward(lib, logits, ids, p, stats, counts, tokens, tau, grad):
-    rows, grad = _rows(logits, logits.shape[-1]), grad.contiguous()
+    rows, grad = _rows(logits, logits.shape[-1]), grad.resolve_neg().contiguous()
     T, V = rows.shape
     per = 16 // rows.element_size()
     with _on(rows.device, None) as s:

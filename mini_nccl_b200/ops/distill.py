@@ -133,7 +133,9 @@ def _arguments(shape, device, ids, top, temperature, reduction="mean"):
 
 
 def _rows_of_entries(t, dtype):
-    """[T, K], dense."""
+    """[T, K], dense, with its own signs."""
+    if t.is_neg():
+        t = t.resolve_neg()
     if t.dtype is not dtype:
         t = t.to(dtype)
     if t.dim() != 2:
