@@ -23,6 +23,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxEntries = 1024;
 constexpr int kMaxParts = 8;   // blocks that share a row of logits
+constexpr int kMostIndex = 0x7ffff000;   // tokens, classes: counters pass the last one by up to four blocks' worth of threads before they are compared
 constexpr float kLog2e = 1.4426950408889634f;
 
 // 2^x to 2^-22 of the value, 0 below 2^-126; exp2 of -infinity is 0, of a NaN a NaN.
@@ -404,14 +405,14 @@ int backward(const void* logits, int64_t ld, int T_, int V, const int64_t* ids, 
 extern "C" {
 #define MNCCL_EXPORT __attribute__((visibility("default")))
 
-// logits [T, V] (type 6 fp16, 7 fp32, 9 bf16; row stride ld elements), ids and top [T, K], K at most 1024, tau in [1e-3, 1e3].  Writes for
+// logits [T, V] (type 6 fp16, 7 fp32, 9 bf16; row stride ld elements; T and V at most 2^31 - 2^12), ids and top [T, K], K at most 1024, tau in [1e-3, 1e3].  Writes for
 // the backward pass p [T, K], stats [T, 2] (8-byte aligned), counts [T] and tokens[1] (how many count); row_loss [T], sum and mean (either may be null).
 // Returns 0, -1 null or empty, -2 shape, type or alignment, or a cudaError_t + 1000.
 MNCCL_EXPORT int mncclDistillForward(const void* logits, int type, int64_t ld, int T, int V, const int64_t* ids, const float* top, int K,
                                      float tau, float* p, float* stats, float* row_loss, int* counts, float* sum, float* mean, float* tokens,
                                      cudaStream_t stream) {
   if (!logits || !ids || !top || !p || !stats || !row_loss || !counts || !tokens || T <= 0 || V <= 0 || K <= 0) return -1;
-  if (K > kMaxEntries || !good_tau(tau) || (reinterpret_cast<uintptr_t>(stats) & 7u) != 0) return -2;
+  if (std::max(T, V) > kMostIndex || K > kMaxEntries || !good_tau(tau) || (reinterpret_cast<uintptr_t>(stats) & 7u) != 0) return -2;
   switch (type) {
     case 6: return forward<__half>(logits, ld, T, V, ids, top, K, tau, p, stats, row_loss, counts, sum, mean, tokens, stream);
     case 7: return forward<float>(logits, ld, T, V, ids, top, K, tau, p, stats, row_loss, counts, sum, mean, tokens, stream);
@@ -426,7 +427,7 @@ MNCCL_EXPORT int mncclDistillBackward(const void* logits, int type, int64_t ld, 
                                       const float* stats, const int* counts, const float* grad, int grad_per_row, const float* tokens,
                                       void* d, int64_t ldd, cudaStream_t stream) {
   if (!logits || !ids || !p || !stats || !counts || !grad || !d || T <= 0 || V <= 0 || K <= 0) return -1;
-  if (K > kMaxEntries || !good_tau(tau) || (reinterpret_cast<uintptr_t>(stats) & 7u) != 0) return -2;
+  if (std::max(T, V) > kMostIndex || K > kMaxEntries || !good_tau(tau) || (reinterpret_cast<uintptr_t>(stats) & 7u) != 0) return -2;
   switch (type) {
     case 6: return backward<__half>(logits, ld, T, V, ids, p, K, tau, stats, counts, grad, grad_per_row, tokens, d, ldd, stream);
     case 7: return backward<float>(logits, ld, T, V, ids, p, K, tau, stats, counts, grad, grad_per_row, tokens, d, ldd, stream);

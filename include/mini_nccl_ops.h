@@ -126,7 +126,7 @@ int mncclGemmFp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, in
 int mncclGemmFp8Plan(int M, int N, int K, int b_rows, int aligned, int sms, int* tile, int* slices);
 
 /* ---- distillation from a teacher's top logits -----------------------------------------------------------
- * Student logits [T, V] of `type` (6, 7 or 9), row stride ld; ids and top [T, K], K <= 1024, tau in [1e-3, 1e3].  With
+ * Student logits [T, V] of `type` (6, 7 or 9; T and V <= 2^31 - 2^12), row stride ld; ids and top [T, K], K <= 1024, tau in [1e-3, 1e3].  With
  * p = softmax(top / tau) over the entries whose id is not negative and whose logit is above -infinity, a token's loss is
  * tau^2 * sum p (log p - log softmax(logits / tau)[id]); tokens without entries count for nothing; an id of V or more makes
  * its token NaN.  Forward writes p [T, K], stats [T, 2] (8-byte aligned), counts [T] and tokens[1] (how many count) for the

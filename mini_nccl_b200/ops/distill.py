@@ -15,7 +15,7 @@ from .gemm import gemm_bf16
 from .lm_loss import _MAX_ROWS, _eight, _pays, _plain, _transposed
 from .lm_loss import _rows as _dense_rows
 
-_MAX_ENTRIES = 1024   # mncclDistillForward
+_MAX_ENTRIES, _MOST = 1024, 2**31 - 2**12   # mncclDistillForward
 _REDUCTIONS = ("none", "sum", "mean")
 
 
@@ -103,7 +103,7 @@ def _native(logits, ids, top):
     """Whether the kernels take the call; the plain operators take the others."""
     if not (logits.is_cuda and _plain(logits) and _plain(ids) and _plain(top) and logits.dtype in _FLOATS):
         return False
-    if not (0 < ids.shape[-1] <= _MAX_ENTRIES and 0 < ids.numel() // ids.shape[-1] < 2**31 and 0 < logits.shape[-1] < 2**31 - 2**12) or not _plain_call():
+    if not (0 < ids.shape[-1] <= _MAX_ENTRIES and 0 < ids.numel() // ids.shape[-1] <= _MOST and 0 < logits.shape[-1] <= _MOST) or not _plain_call():
         return False
     return no_tangent(logits)
 
