@@ -373,6 +373,7 @@ MNCCL_EXPORT int mncclQuantizeFp8(const void* x, int type, int64_t ldx, int M, i
 // out[K] (type as above) = the columns' sums of mncclQuantizeFp8 over all `blocks` blocks of rows.  Returns as that.
 MNCCL_EXPORT int mncclSumBlocks(const float* sums, int blocks, int K, void* out, int type, cudaStream_t stream) {
   if (!sums || !out || blocks <= 0 || K <= 0) return -1;
+  if (K > kMaxK || blocks > 0x7fffff00 / kBlock) return -2;   // of what mncclQuantizeFp8 takes
   const dim3 grid(static_cast<unsigned>((K + 31) / 32));
   switch (type) {
     case 6: return status(mnccl::launch_early(sum_tiles_kernel<__half>, grid, dim3(256), stream, sums, blocks, K, out));
