@@ -14,6 +14,8 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -24,7 +26,9 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
+#include <initializer_list>
 #include <optional>
 
 #include "mini_nccl_api.h"
@@ -362,6 +366,28 @@ bool on(const at::Tensor& t, PyObject* stream, On* o) {
   return true;
 }
 
+// Whether nothing is active that may record or replace the single operators, and the arguments (None: left out) are plain tensors.  Where something is,
+// ops/fp8.py says whether the call is refused.
+bool plain_calls(const char* name, std::initializer_list<PyObject*> tensors) {
+  bool plain = !torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+               !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
+  for (PyObject* t : tensors) plain = plain && (t == Py_None || THPVariable_CheckExact(t));
+  if (plain) return true;
+  PyObject* rules = PyImport_ImportModule("mini_nccl_b200.ops.fp8");
+  PyObject* rule = rules ? PyObject_GetAttrString(rules, "plain_calls_only") : nullptr;
+  PyObject* args = rule ? PyTuple_New(static_cast<Py_ssize_t>(tensors.size()) + 1) : nullptr;
+  PyObject* said = nullptr;
+  if (args) {
+    PyObject* who = PyUnicode_FromString(name);
+    PyTuple_SET_ITEM(args, 0, who);
+    Py_ssize_t i = 1;
+    for (PyObject* t : tensors) PyTuple_SET_ITEM(args, i++, Py_NewRef(t));
+    said = who ? PyObject_CallObject(rule, args) : nullptr;
+  }
+  for (PyObject* o : {rules, rule, args, said}) Py_XDECREF(o);
+  return said != nullptr;
+}
+
 // fp16, fp32 and bf16, by the library's codes; -1 for another type
 int float_code(const at::Tensor& t) {
   const int c = type_code(t.scalar_type());
@@ -422,7 +448,7 @@ void quantize(const at::Tensor& x, int64_t ld, bool row, bool transposed, bool s
 // quantize_fp8(x, block_rows, transposed, stream | None) -> (q, scale) or (q, scale, qt, scale_t); see ops/fp8.py
 PyObject* quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arg_count(n, 4)) return nullptr;
+  if (!arg_count(n, 4) || !plain_calls("quantize_fp8", {args[0]})) return nullptr;
   const at::Tensor* x = tensor_arg(args[0], "x");
   if (!x) return nullptr;
   const long block_rows = PyLong_AsLong(args[1]);
@@ -487,7 +513,7 @@ bool scales(const at::Tensor& t, const char* name, int64_t rows, int64_t K, cons
 // gemm_fp8(a, a_scale, b, b_scale, out | None, out_dtype | None, bias | None, stream | None) -> out; see ops/fp8.py
 PyObject* gemm_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arg_count(n, 8)) return nullptr;
+  if (!arg_count(n, 8) || !plain_calls("gemm_fp8", {args[0], args[1], args[2], args[3], args[4], args[6]})) return nullptr;
   const at::Tensor *a = tensor_arg(args[0], "a"), *sa = a ? tensor_arg(args[1], "a_scale") : nullptr, *b = sa ? tensor_arg(args[2], "b") : nullptr,
                    *sb = b ? tensor_arg(args[3], "b_scale") : nullptr;
   if (!sb) return nullptr;

@@ -196,7 +196,14 @@ def _quantize(lib, x, block_rows, transposed, sums, s):
     return q, scale, qt, scale_t, sums
 
 
+def _plain_calls(name, *tensors):
+    from .ops.fp8 import plain_calls_only
+
+    plain_calls_only(name, *tensors)
+
+
 def quantize_fp8(lib, x, block_rows, transposed, stream):
+    _plain_calls("quantize_fp8", x)
     _matrix(x, "x", _FLOATS)
     if block_rows not in (1, _BLOCK):
         raise ValueError("block_rows must be 1 or 128")
@@ -228,6 +235,7 @@ def _scales(t, name, rows, K, device):
 
 
 def gemm_fp8(lib, a, a_scale, b, b_scale, out, out_dtype, bias, stream):
+    _plain_calls("gemm_fp8", a, a_scale, b, b_scale, out, bias)
     M, K, lda = _operand(a, "a")
     N, Kb, ldb = _operand(b, "b")
     if K != Kb or b.device != a.device:

@@ -27,9 +27,10 @@ def _call(name, symbol, source):
     return call
 
 
-def _plain_calls_only(name, *tensors):
+def plain_calls_only(name, *tensors):
     """What is active may record or replace the single operators: a tracer would keep the allocation of a result and not the kernel that fills it, so
-    that what it recorded returns memory as it was found.  Modes that only look on (FLOP counters, selective checkpointing) do no harm."""
+    that what it recorded returns memory as it was found.  Modes that only look on (FLOP counters, selective checkpointing) do no harm.  The
+    extension asks here for quantize_fp8 and gemm_fp8, where one of these may be the case: asked every time it would cost those a microsecond."""
     if torch.jit.is_tracing() or torch._C._are_functorch_transforms_active() or (
             torch._C._len_torch_dispatch_stack() and any(torch._C._get_dispatch_mode(mode) is not None for mode in _RECORDING)):
         raise RuntimeError(f"{name} has no rule for tracing, functional transforms and fake tensors")
@@ -50,7 +51,6 @@ def quantize_fp8(x, block_rows=1, transposed=False, stream=None):
     ``transposed=True``: ``(q, scale, qt, scale_t)``, with the transpose ``qt [K, M]`` as well, from one reading of ``x``; with
     ``block_rows=1`` it is quantised anew, in blocks of 128 along M (``scale_t [K, ceil(M / 128)]``).  K is at most 65535 * 128.
     Not differentiable."""
-    _plain_calls_only("quantize_fp8", x)
     return _call("quantize_fp8", "mncclQuantizeFp8", "csrc/kernels/fp8_quantize.cu")(x, block_rows, transposed, stream)
 
 
@@ -61,7 +61,6 @@ def gemm_fp8(a, a_scale, b, b_scale, out=None, out_dtype=None, bias=None, stream
     A block's products are summed in fp32, multiplied by the fp32 product of its two scales (which has to stay in fp32's range: beyond it the block
     counts as infinite or NaN, below it as 0) and added up in fp32; with the bias added, one rounding to ``out``'s type (bf16 by
     default, fp16 or fp32).  ``bias`` has that type.  Operands have rows that start on 16 bytes.  Not differentiable."""
-    _plain_calls_only("gemm_fp8", a, a_scale, b, b_scale, out, bias)
     return _call("gemm_fp8", "mncclGemmFp8", "csrc/kernels/gemm_fp8.cu")(a, a_scale, b, b_scale, out, out_dtype, bias, stream)
 
 
@@ -79,7 +78,7 @@ def linear_fp8(x, weight, bias=None):
     ``dbias`` the fp32 sum of ``dy``.  What is kept for the backward pass is in 8 bits.
 
     All three refuse to be traced or transformed, and tensor subclasses with rules of their own."""
-    _plain_calls_only("linear_fp8", x, weight, bias)
+    plain_calls_only("linear_fp8", x, weight, bias)
     if torch.is_autocast_enabled("cuda"):
         to = torch.get_autocast_dtype("cuda")
         x, weight, bias = x.to(to), weight.to(to), None if bias is None else bias.to(to)
