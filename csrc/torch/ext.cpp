@@ -576,6 +576,8 @@ PyObject* gemm_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
                       static_cast<int>(K), o.raw);
     Py_END_ALLOW_THREADS
     check(rc, "mncclGemmFp8");
+    // autograd notices that an operand it has kept was written, as for PyTorch's own calls with out=
+    if (!fresh.defined() && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
   }
   return fresh.defined() ? THPVariable_Wrap(fresh) : Py_NewRef(args[4]);
   END_HANDLE_TH_ERRORS

@@ -244,8 +244,9 @@ def gemm_fp8(lib, a, a_scale, b, b_scale, out, out_dtype, bias, stream):
     sb = _scales(b_scale, "b_scale", N, K, a.device)
     if out_dtype is not None and not isinstance(out_dtype, torch.dtype):
         raise TypeError("out_dtype must be a torch dtype")
+    given = out is not None
     with _on(a.device, stream) as s:
-        if out is None:
+        if not given:
             out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=a.device)
         elif out_dtype not in (None, _tensor(out, "out").dtype):
             raise ValueError("out has another type than out_dtype")
@@ -261,6 +262,8 @@ def gemm_fp8(lib, a, a_scale, b, b_scale, out, out_dtype, bias, stream):
         if M and N:
             _check(lib.mncclGemmFp8(a.data_ptr(), lda, a_scale.data_ptr(), *sa, b.data_ptr(), ldb, b_scale.data_ptr(), *sb, out.data_ptr(), ldc,
                                     _FLOATS[out.dtype], bias.data_ptr() if bias is not None else None, M, N, K, s), "mncclGemmFp8")
+            if given and not out.is_inference():
+                torch.autograd.graph.increment_version(out)
     return out
 
 
