@@ -5,7 +5,8 @@
 // half of the tile's rows of B (32 KB a block of K for BN = 256, which is what lets L2 keep up) and holds the sums of its 128 rows:
 //
 //   both CTAs   warp 0      TMA producer; bytes are counted on the leader's barriers
-//   leader      warps 1, 2  for half of the tile's columns each, one lane issues the four MMAs of a block into one of two accumulators and commits:
+//   leader      warps 1, 2  for half of the tile's columns each, one lane issues the four MMAs of a block into one of two accumulators (four
+//                           for tiles of up to 128 columns) and commits:
 //                           the ring stage and the half's accumulator.  Halves are handed over by themselves, so that the tensor cores
 //                           work on one while the other is being read
 //   both CTAs   warp 3      brings the scales
@@ -14,10 +15,10 @@
 //
 // The tensor cores take 512 cycles for a block of 128 x 256 x 128 an SM; reading it (64 KB from tensor memory) and 256 fused multiply-adds
 // a scheduler overlap with the next block.  Where B has a scale for every row (the gradient of a weight) every column has a product of scales of
-// its own, which costs a read of shared memory and half an instruction a warp and column: 4096 x 4096 x 4096 takes 97 us against 67.
+// its own, which costs a read of shared memory and half an instruction a warp and column: 4096 x 4096 x 4096 takes 97 us against 69.
 //
-// What bounds it: the hand-over of accumulators at short clocks, and power in long runs.  4096 x 14336 x 4096 (481 GFLOP) takes 223 us alone, 2.2
-// PFLOP/s, and 275 repeated for seconds; 8192 x 4096 x 1024 41 us, where each tile's first block and its 128 KB of results count most.
+// What bounds it: the hand-over of accumulators at short clocks, and power in long runs.  4096 x 14336 x 4096 (481 GFLOP) takes 227 us in short bursts,
+// 2.1 PFLOP/s, and 275 repeated for seconds; 8192 x 4096 x 1024 41 us, where each tile's first block and its 128 KB of results count most.
 #include <algorithm>
 #include <cstdio>
 
@@ -502,10 +503,12 @@ bool make_tensor_map_out(CUtensorMap* map, const Args& g) {
 }
 
 // The tile width with the least estimated time (ns): a wave of tiles takes about two microseconds and so much a block of K, more with a scale for
-// every row of B (measured, us without / with those: 256 x 4096 x 4096, one wave of 64, 13.5 / 14.4, and of 128, 15.4 / 18.0; 1001 x 1288 x 5000,
-// one of 128, 18.3 / 21.5; 1001 x 5000 x 1288, two of 192, 17.6 / 21.0; 4096 x 4096 x 4096, four of 256, 67 / 101; 8192 x 4096 x 1024, seven of 256,
-// 41).  Rows of C that the TMA unit cannot write cost a wave of 128 columns one more (8192 x 4095 x 1024: 56).  A narrower tile pays where it saves
-// a wave or leaves fewer SMs idle; 64 columns on all SMs read 10 TB/s from the L2.
+// every row of B.  The constants describe a kernel by itself; calls that follow one another overlap and take about a microsecond less each, whatever the
+// width.  Measured so, operands not in the L2 (us without / with a scale for every row): 256 x 4096 x 4096, one wave of 64, 12.2 / 13.3, and of 128, 13.6
+// / 17.4; 1001 x 1288 x 5000, one of 128, 17.2 / 21.5; 1001 x 5000 x 1288, two of 192, 15.5 / 19.1; 4096 x 4096 x 4096, four of 256, 69 / 96, and
+// five of 192, 73 / 95; 8192 x 4096 x 1024, seven of 256, 42 / 55: in these and seven others the width chosen is the fastest of the four.  Rows of C that the TMA unit cannot write
+// cost a wave of 128 columns one more (8192 x 4095 x 1024: 57).  A narrower tile pays where it saves a wave or leaves fewer SMs idle; 64 columns on
+// all SMs read 10 TB/s from the L2.
 int pick_width(int M, int N, int K, bool b_rows, bool mapped, int pairs, long* ns) {
   struct Width {
     int bn;

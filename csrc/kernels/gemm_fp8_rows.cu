@@ -6,13 +6,13 @@
 // Eight lanes hold a block of 128: their sums are reduced and dealt out over them together, seven shuffles for the eight rows, so
 // that each lane ends with one whole block's sum, which it scales.  The warps meet in shared memory and are added in order.
 //
-// The tensor-core kernel for few rows spends three microseconds on descriptors, barriers, tensor memory and the meeting of its slices, which this
-// one saves; then this one runs at 4.8 TB/s for one token, bound by its instructions (two for three bytes), at 4 for two and at 2.3 for
-// four, and that one at up to 5.5.  Measured alone (this kernel / that one, us): 1 x 1024 x 1024 2.6 / 4.5, 1 x 4096 x 1024 3.4 / 5.2, 1 x 4096
-// x 4096 5.8 / 7.5, 1 x 14336 x 4096 14.7 / 13.4; 2 x 4096 x 4096 6.8 / 7.8; 4 x 1024 x 1024 3.2 / 5.1, 4 x 4096 x 4096 10.7 / 8.5.  Calls that
-// follow one another overlap at their ends (dependent_launch.cuh): 1 x 1024 x 1024 2.2, 1 x 4096 x 4096 5.5.  64 registers and 1024 threads
-// an SM matter: with 80, 1 x 4096 x 4096 took 7.1 us.  (Widening to fp32 took 7.8, mma.sync m16n8k32 of the same bytes 7.5 for 8 tokens and
-// 20.1 at 14336.)
+// The tensor-core kernel for few rows spends more than a microsecond more on descriptors, barriers, tensor memory and the meeting of its slices, which
+// this one saves; then this one runs at 4.6 TB/s for one token, bound by its instructions (two for three bytes), at 4 for two and at 2.3 for
+// four, and that one at up to 5.5.  Measured in graphs, calls that follow one another (and overlap at their ends, dependent_launch.cuh), weights not in the L2
+// (this kernel / that one, us): 1 x 1024 x 1024 2.1 / 3.5, 1 x 4096 x 1024 3.0 / 4.1, 1 x 4096 x 4096 5.5 / 6.7, 1 x 14336 x 4096 14.7 / 12.3; 2 x 4096 x 4096
+// 6.5 / 7.0; 4 x 1024 x 1024 2.5 / 4.0, 4 x 4096 x 4096 9.7 / 7.4.  The same weight over and over, which then lies in the L2, 1 x 4096 x 4096: 3.9.  rows_ns is
+// fitted to a kernel by itself and a weight from memory (5.8 there).  64 registers and 1024 threads an SM matter: with 80, 1 x 4096 x 4096 took 7.1 us by
+// itself.  (Widening to fp32 took 7.8, mma.sync m16n8k32 of the same bytes 7.5 for 8 tokens and 20.1 at 14336.)
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 

@@ -336,15 +336,17 @@ int per_slice(int num_kb, int slices, int tn) {
   return (stages + slices - 1) / slices * per_stage;
 }
 
-// The plan with the least estimated time (ns).  Measured on 148 SMs, operands not in L2 (M x N x K, tile's rows of A / slices):
-//   1 x 4096 x 4096      16 / 4: 7.5 us, 16 / 8: 8.6, 16 / 2: 9.6          64 x 14336 x 4096   64 / 1: 20.2 us, 32 / 1: 23.1, pairs: 21.2
-//   16 x 4096 x 14336    16 / 8: 14.7 us, 16 / 4: 15.3, 16 / 2: 19.5       64 x 4096 x 4096    64 / 4: 11.9 us, 32 / 4: 13.1, pairs: 13.0
-//   256 x 1024 x 1024    16 / 1: 6.9 us, 64 / 4: 7.7                       128 x 4096 x 4096   64 / 2: 15.1 us, 32 / 1: 16.8, pairs: 13.0
-//   512 x 1024 x 1024    16 / 1: 8.6 us, pairs: 6.4                        777 x 1003 x 1544   64 / 1: 12.2 us, pairs: 8.9
+// The plan with the least estimated time (ns).  The constants describe a kernel by itself.  Measured on 148 SMs, calls that follow one another and
+// overlap (about a microsecond less each), operands not in L2 (M x N x K, tile's rows of A / slices):
+//   1 x 4096 x 4096      16 / 4: 6.7 us, 16 / 8: 6.8, 16 / 2: 8.3          64 x 14336 x 4096   64 / 1: 16.7 us, 32 / 1: 19.1, pairs: 19.8
+//   16 x 4096 x 14336    16 / 8: 13.3 us, 16 / 4: 15.0, 16 / 2: 21.5       64 x 4096 x 4096    64 / 4: 9.7 us, 32 / 4: 10.2, pairs: 11.9
+//   256 x 1024 x 1024    16 / 1: 5.4 us, 64 / 4: 6.7, pairs: 5.2           128 x 4096 x 4096   64 / 2: 12.5 us, 32 / 1: 13.8, pairs: 12.1
+//   512 x 1024 x 1024    16 / 1: 6.4 us, pairs: 5.6                        777 x 1003 x 1544   64 / 1: 10.6 us, pairs: 7.8
+// The choice is the fastest of all in 28 of 32 products tried so, within 4 % in three more, and 13 % off for 16 x 4096 x 14336 (it takes 16 / 4).
 // So a tile takes a fixed time and one per block of K that grows with its width; two narrow tiles on an SM overlap by a third, two wide
-// ones hardly; and nothing is faster than the operands come from memory.  Tiles of 128 rows of A never won (128 x 4096 x 4096: 16.4 us).  A
-// tile that has its K and its SM to itself takes all of the shared memory as its ring (16 x 14336 x 4096: 16.9 -> 15.5 us);
-// slices do better with half, which lets the next wave's CTAs in early (1 x 4096 x 4096: 9.0 -> 8.2 us).
+// ones hardly; and nothing is faster than the operands come from memory.  Tiles of 128 rows of A never won (128 x 4096 x 4096 by itself: 16.4 us).  A
+// tile that has its K and its SM to itself takes all of the shared memory as its ring (16 x 14336 x 4096 by itself: 16.9 -> 15.5 us);
+// slices do better with half, which lets the next wave's CTAs in early (1 x 4096 x 4096 by itself: 9.0 -> 8.2 us).
 bool plan_small(int M, int N, int K, int sms, SmallPlan* p, long* ns) {
   struct Cost {
     int tn;
