@@ -132,10 +132,14 @@ __device__ __forceinline__ void store_rows(const Args& g, const CUtensorMap* map
   }
   if (mapped) {
     constexpr int kPer = kOutRow / static_cast<int>(sizeof(T)), kChunk = 16 / static_cast<int>(sizeof(T));
+    // The TMA unit cuts a row off behind the 16 bytes that hold the tensor's last column: where these hold columns behind the result as well, the warp
+    // stores the last piece by itself.
+    const bool ragged = g.N % kChunk != 0;
+    uint8_t* piece = scratch;
 #pragma unroll
     for (int p = 0; p < NC / kPer; ++p) {
       if (col + p * kPer >= g.N) break;
-      uint8_t* piece = scratch + (pieces++ & 1u) * kPieceBytes;
+      piece = scratch + (pieces++ & 1u) * kPieceBytes;
       if (lane == 0) bulk_wait_read<1>();   // the piece before the last has been read
       __syncwarp();
 #pragma unroll
@@ -147,9 +151,18 @@ __device__ __forceinline__ void store_rows(const Args& g, const CUtensorMap* map
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) {
-        tma_store_2d(map, smem_u32(piece), col + p * kPer, row_base);
+      if (lane == 0) {   // (a group of nothing for a piece that does not go out so: groups are counted as pieces are)
+        if (!ragged || col + (p + 1) * kPer <= g.N) tma_store_2d(map, smem_u32(piece), col + p * kPer, row_base);
         bulk_commit();
+      }
+    }
+    if (ragged && g.N - col < NC) {
+      const int n = g.N / kPer * kPer;   // the last piece's first column
+      T* c = static_cast<T*>(g.c) + static_cast<size_t>(row_base) * g.ldc + n;
+      for (int i = lane; i < 32 * kPer; i += 32) {
+        const int r = i / kPer, k = i % kPer;
+        if (row_base + r < g.M && n + k < g.N)
+          c[static_cast<size_t>(r) * g.ldc + k] = reinterpret_cast<const T*>(piece + r * kOutRow + ((k / kChunk ^ (r >> 1)) & 3) * 16)[k % kChunk];
       }
     }
     return;

@@ -181,7 +181,8 @@ __device__ __forceinline__ bool mbar_wait_both(uint32_t bar, uint32_t parity, ui
   return mbar_wait_warp(bar, parity, abort_flag, budget_ns) && mbar_wait_warp(bar2, parity2, abort_flag, budget_ns);
 }
 
-// Tiled store shared -> global, tracked by bulk async-groups; what lies outside the tensor is not written.
+// Tiled store shared -> global, tracked by bulk async-groups; what lies outside the tensor is not written, but for the rest of the 16 bytes in which a row
+// of it ends (seen on a B200: columns behind the last, up to a multiple of 16 bytes, came out overwritten).
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t smem_src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_src), "r"(c0),
                "r"(c1)
